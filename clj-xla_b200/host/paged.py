@@ -1,0 +1,386 @@
+"""Serving over a paged key-value cache: append, attend, verify.
+
+Python mirror of the paged-cache entries of ``include/cljxla_b200.h`` (the
+reference's paged cache is a design note only,
+``docs/xla/paged_attention_vram.md:38-94``).  A Clojure host binds the C entries
+and passes device pointers; here they are taken from torch CUDA tensors.
+
+One step of a serving loop over a cache of ``[kv_heads, page_size, head_dim]``
+pages::
+
+    cache = PagedKV(k_pages, v_pages, page_table, seq_lens)   # once
+    ...                                                       # seq_lens += rows of the step
+    cache.append(k, v, q=q, q_out=q, starts=starts, rope=rope)
+    cache.attend(q, out=context, starts=starts, max_tokens=5)
+    ...                                                       # logits of the rows
+    verify_draft(logits, tokens, starts, out_tokens=..., accepted=..., seq_lens=seq_lens, new_lens=seq_lens, ...)
+
+A step's rows are packed: sequence ``b`` has rows ``starts[b]`` to
+``starts[b + 1]`` (without ``starts``: equally many each), the last of them at
+position ``seq_lens[b] - 1``.  The kernels read ``starts``, ``seq_lens`` and
+``page_table`` when they run, so a captured CUDA graph follows their contents;
+rows behind the last sequence are left alone.
+
+Calls enqueue on torch's current stream of the tensors' device and never
+synchronise.  Tensors of another shape, type, device or layout raise
+``ValueError``; what the library refuses raises :class:`~.pjrt.PJRTError`.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+import threading
+from typing import Optional
+
+import torch
+
+from .core import default_library_path
+from .pjrt import DTYPE_ENUM, PJRTError
+
+_TYPES = {torch.float32: DTYPE_ENUM["f32"], torch.bfloat16: DTYPE_ENUM["bf16"], torch.float16: DTYPE_ENUM["f16"]}
+
+_P, _I, _N = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_size_t), ("k_pages", _P), ("v_pages", _P),
+                ("k_page_stride", _I), ("k_head_stride", _I), ("k_row_stride", _I),
+                ("v_page_stride", _I), ("v_head_stride", _I), ("v_row_stride", _I),
+                ("num_pages", _I), ("kv_heads", _I), ("page_size", _I), ("head_dim", _I),
+                ("page_table", _P), ("seq_lens", _P), ("num_seqs", _I), ("pages_per_seq", _I),
+                ("page_table_stride", _I), ("dtype", _N), ("reserved", _N)]
+
+
+class _AppendArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_size_t), ("k", _P), ("v", _P), ("q", _P), ("q_out", _P),
+                ("tokens", _I), ("q_heads", _I), ("k_token_stride", _I), ("k_head_stride", _I),
+                ("v_token_stride", _I), ("v_head_stride", _I), ("q_token_stride", _I), ("q_head_stride", _I),
+                ("q_out_token_stride", _I), ("q_out_head_stride", _I), ("starts", _P), ("inv_freq", _P),
+                ("rotary_dim", _I), ("interleaved", _N), ("rope_scale", ctypes.c_float)]
+
+
+class _AttentionArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_size_t), ("q", _P), ("out", _P), ("tokens", _I), ("q_heads", _I),
+                ("q_token_stride", _I), ("q_head_stride", _I), ("out_token_stride", _I), ("out_head_stride", _I),
+                ("starts", _P), ("max_tokens", _I), ("window", _I), ("scale", ctypes.c_float),
+                ("softcap", ctypes.c_float), ("out_dtype", _N), ("reserved", _N), ("workspace", _P),
+                ("workspace_bytes", _I)]
+
+
+class _VerifyArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_size_t), ("target", _P), ("draft", _P), ("tokens_in", _P), ("starts", _P),
+                ("uniform", _P), ("race", _P), ("tokens", _I), ("num_seqs", _I), ("vocab", _I), ("max_tokens", _I),
+                ("target_stride", _I), ("draft_stride", _I), ("race_stride", _I), ("temperature", ctypes.c_float),
+                ("draft_temperature", ctypes.c_float), ("dtype", _N), ("greedy", _N), ("tokens_out", _P),
+                ("accepted", _P), ("logprobs", _P), ("seq_lens", _P), ("new_lens", _P), ("workspace", _P),
+                ("workspace_bytes", _I)]
+
+
+class _Calls:
+    """The library's entries, bound once."""
+
+    def __init__(self, path: str):
+        lib = ctypes.CDLL(path)
+        call = [_P, ctypes.c_char_p, ctypes.c_size_t]
+        size = [ctypes.POINTER(_I), ctypes.c_char_p, ctypes.c_size_t]
+        self.append = self._bind(lib.cljxla_b200_paged_append, [_P, _P] + call)
+        self.attend = self._bind(lib.cljxla_b200_paged_attention, [_P, _P] + call)
+        self.attend_size = self._bind(lib.cljxla_b200_paged_attention_workspace, [_P, _P] + size)
+        self.verify = self._bind(lib.cljxla_b200_verify_draft, [_P] + call)
+        self.verify_size = self._bind(lib.cljxla_b200_verify_draft_workspace, [_P] + size)
+
+    @staticmethod
+    def _bind(f, types):
+        f.argtypes, f.restype = types, ctypes.c_int
+        return f
+
+
+_calls: Optional[_Calls] = None
+_local = threading.local()
+
+
+def _library() -> _Calls:
+    global _calls
+    if _calls is None:
+        _calls = _Calls(default_library_path())
+    return _calls
+
+
+def _err():
+    try:
+        return _local.err
+    except AttributeError:
+        _local.err = ctypes.create_string_buffer(512)
+        return _local.err
+
+
+def _raise(rc: int):
+    raise PJRTError(_err().value.decode(), rc)
+
+
+def _enqueue(device: int, call, *args):
+    """Calls a library entry with torch's current stream of `device`, which is
+    made the current device for the call."""
+    err = _err()
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            rc = call(*args, torch.cuda.current_stream(device).cuda_stream, err, 512)
+    else:
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(device), err, 512)
+    if rc:
+        _raise(rc)
+
+
+def _rows(t: torch.Tensor, name: str, shape, dtype, device: int):
+    """Strides of a [rows, heads, head_dim] tensor whose last axis is contiguous."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+        raise ValueError(f"{name}: {tuple(shape)} {dtype} on cuda:{device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    s = t.stride()
+    if s[2] != 1:
+        raise ValueError(f"{name}: head_dim must be contiguous, got strides {s}")
+    return s
+
+
+def _vector(t: torch.Tensor, name: str, n: Optional[int], dtype, device: int):
+    if t.dtype is not dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.get_device() != device \
+            or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous [{'n' if n is None else n}] {dtype} on cuda:{device} expected, "
+                         f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, device=None, proportion: float = 1.0, factor: float = 1.0,
+                  low_turns: Optional[float] = None, high_turns: Optional[float] = None,
+                  trained_positions: Optional[int] = None) -> torch.Tensor:
+    """Angle per position of each rotated pair: ``theta ** (-2 i / rotary_dim)``.
+
+    ``proportion`` < 1 leaves the trailing pairs unrotated (angle 0), as the
+    reference's ``rope-proportion`` does (attention.clj:19-61).  ``factor``
+    stretches the positions for contexts longer than the trained ones: every
+    frequency is divided by it, or, with ``low_turns``, ``high_turns`` and
+    ``trained_positions``, only those of pairs that make at most ``low_turns``
+    turns within the trained positions; pairs of at least ``high_turns`` keep
+    theirs, and between the two the division fades in linearly.
+    """
+    if rotary_dim < 0 or rotary_dim % 2 or not theta > 0 or not factor > 0 or not 0 <= proportion <= 1:
+        raise ValueError("rope_inv_freq: rotary_dim must be even, theta and factor positive, proportion in [0, 1]")
+    half = rotary_dim // 2
+    freq = [theta ** (-2.0 * i / rotary_dim) if i < int(proportion * half) else 0.0 for i in range(half)]
+    if factor != 1.0:
+        if (low_turns is None) != (high_turns is None) or (low_turns is None) != (trained_positions is None):
+            raise ValueError("rope_inv_freq: low_turns, high_turns and trained_positions go together")
+        if low_turns is None:
+            freq = [f / factor for f in freq]
+        else:
+            if not low_turns < high_turns:
+                raise ValueError("rope_inv_freq: low_turns must be below high_turns")
+            for i, f in enumerate(freq):
+                turns = trained_positions * f / (2.0 * math.pi)
+                keep = min(1.0, max(0.0, (turns - low_turns) / (high_turns - low_turns)))
+                freq[i] = f * keep + f / factor * (1.0 - keep)
+    return torch.tensor(freq, dtype=torch.float32, device=device)
+
+
+class Rope:
+    """The rotation of one kind of layer: ``inv_freq`` f32 on the device (twice
+    as many elements of each head are rotated), pairs ``(i, i + n)`` or, with
+    ``interleaved``, ``(2 i, 2 i + 1)``; ``scale`` multiplies cos and sin."""
+
+    def __init__(self, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0):
+        if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
+                or not inv_freq.is_cuda:
+            raise ValueError("Rope: inv_freq must be a contiguous f32 vector on a CUDA device")
+        self.inv_freq, self.interleaved, self.scale = inv_freq, bool(interleaved), float(scale)
+
+
+class PagedKV:
+    """A paged cache of one layer: ``k_pages`` / ``v_pages`` ``[num_pages,
+    kv_heads, page_size, head_dim]`` (any strides with 16-byte aligned rows: a
+    ``[num_pages, page_size, kv_heads, head_dim]`` pool goes in transposed),
+    ``page_table`` ``[num_seqs, pages_per_seq]`` i32 and ``seq_lens``
+    ``[num_seqs]`` i32.  Holds references, no copies; calls from several threads
+    or streams may overlap as far as the tensors they write allow."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor):
+        if not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.dtype not in _TYPES:
+            raise ValueError("k_pages: [num_pages, kv_heads, page_size, head_dim] f32, f16 or bf16 on a CUDA device expected")
+        dev = k_pages.get_device()
+        if v_pages.shape != k_pages.shape or v_pages.dtype is not k_pages.dtype or v_pages.get_device() != dev:
+            raise ValueError("v_pages: the shape, type and device of k_pages expected")
+        if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+            raise ValueError("pages: head_dim must be contiguous")
+        if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != dev \
+                or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table: [num_seqs, pages_per_seq] int32 with contiguous rows on the pages' device expected")
+        lens = _vector(seq_lens, "seq_lens", page_table.shape[0], torch.int32, dev)
+        self.k_pages, self.v_pages, self.page_table, self.seq_lens = k_pages, v_pages, page_table, seq_lens
+        pages, heads, size, dim = k_pages.shape
+        self.num_seqs, self.kv_heads, self.head_dim, self.dtype, self.device = page_table.shape[0], heads, dim, k_pages.dtype, dev
+        k, v = k_pages.stride(), v_pages.stride()
+        self._cache = _Cache(ctypes.sizeof(_Cache), k_pages.data_ptr(), v_pages.data_ptr(), k[0], k[1], k[2], v[0], v[1],
+                             v[2], pages, heads, size, dim, page_table.data_ptr(), lens, self.num_seqs,
+                             page_table.shape[1], page_table.stride(0), _TYPES[self.dtype], 0)
+        self._at = ctypes.addressof(self._cache)
+        self._lib = _library()
+        self._sizes = {}
+
+    def _starts(self, starts):
+        return None if starts is None else _vector(starts, "starts", self.num_seqs + 1, torch.int32, self.device)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, q: Optional[torch.Tensor] = None,
+               q_out: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, rope: Optional[Rope] = None):
+        """Writes the step's ``k`` and ``v`` ``[rows, kv_heads, head_dim]`` into
+        their pages, ``k`` rotated by ``rope``, and the rotated ``q`` ``[rows,
+        q_heads, head_dim]`` into ``q_out`` (``q`` itself by default).  Rows whose
+        page the table does not name are left out.  Returns ``q_out``."""
+        n, heads, dim, dt, dev = k.shape[0], self.kv_heads, self.head_dim, self.dtype, self.device
+        ks = _rows(k, "k", (n, heads, dim), dt, dev)
+        vs = _rows(v, "v", (n, heads, dim), dt, dev)
+        a = _AppendArgs(ctypes.sizeof(_AppendArgs), k.data_ptr(), v.data_ptr(), None, None, n, 0, ks[0], ks[1], vs[0], vs[1])
+        if q is not None:
+            if q_out is None:
+                q_out = q
+            if q.dim() != 3:
+                raise ValueError("q: [rows, q_heads, head_dim] expected")
+            nq = q.shape[1]
+            qs = _rows(q, "q", (n, nq, dim), dt, dev)
+            os = _rows(q_out, "q_out", (n, nq, dim), dt, dev)
+            a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), nq
+            a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride = qs[0], qs[1], os[0], os[1]
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if starts is not None:
+            a.starts = self._starts(starts)
+        if rope is not None:
+            if rope.inv_freq.get_device() != dev:
+                raise ValueError("rope: inv_freq must be on the pages' device")
+            a.inv_freq, a.rotary_dim = rope.inv_freq.data_ptr(), 2 * rope.inv_freq.shape[0]
+            a.interleaved, a.rope_scale = rope.interleaved, rope.scale
+        _enqueue(dev, self._lib.append, self._at, ctypes.addressof(a))
+        return q_out
+
+    def attend(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+               max_tokens: Optional[int] = None, scale: Optional[float] = None, softcap: float = 0.0, window: int = -1):
+        """Attention of the step's rows ``q`` ``[rows, q_heads, head_dim]`` over
+        their sequences' pages, into ``out`` (same shape; the pages' type or
+        f32).  A row sees the positions up to its own, with ``window`` >= 0 only
+        that many before its own; a row that sees nothing is zero.  ``max_tokens``
+        bounds a sequence's rows (default: all rows), ``scale`` is ``head_dim **
+        -0.5`` by default, ``softcap`` > 0 caps the scores as ``softcap *
+        tanh(score / softcap)``.  Returns ``out``."""
+        dt, dev, dim = self.dtype, self.device, self.head_dim
+        if q.dim() != 3:
+            raise ValueError("q: [rows, q_heads, head_dim] expected")
+        n, nq = q.shape[0], q.shape[1]
+        qs = _rows(q, "q", (n, nq, dim), dt, dev)
+        if out is None:
+            out = torch.empty((n, nq, dim), dtype=dt, device=q.device)
+        odt = out.dtype
+        if odt is not dt and odt is not torch.float32:
+            raise ValueError(f"out: {dt} or torch.float32 expected, got {odt}")
+        os = _rows(out, "out", (n, nq, dim), odt, dev)
+        if max_tokens is None:
+            max_tokens = n
+        a = _AttentionArgs(ctypes.sizeof(_AttentionArgs), q.data_ptr(), out.data_ptr(), n, nq, qs[0], qs[1], os[0], os[1],
+                           self._starts(starts), max_tokens, window, dim ** -0.5 if scale is None else scale, softcap,
+                           _TYPES[odt])
+        at = ctypes.addressof(a)
+        key = (n, nq, max_tokens, starts is None, window)
+        need = self._sizes.get(key)
+        if need is None:
+            need = self._sizes[key] = _size(dev, self._lib.attend_size, self._at, at)
+        if need:
+            # from torch's allocator on this call's stream: calls that overlap, and captured graphs, have one each
+            work = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = work.data_ptr(), need
+        _enqueue(dev, self._lib.attend, self._at, at)
+        return out
+
+
+def _size(device: int, call, *args) -> int:
+    """A workspace query, with `device` as the current one."""
+    got = _I()
+    with torch.cuda.device(device):
+        rc = call(*args, ctypes.byref(got), _err(), 512)
+    if rc:
+        _raise(rc)
+    return got.value
+
+
+_verify_sizes = {}
+
+
+def _matrix(t, name, rows, cols, dtype, device):
+    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != device or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: [{rows}, {cols}] {dtype} with contiguous rows on cuda:{device} expected, "
+                         f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
+                 out_tokens: torch.Tensor, accepted: torch.Tensor, logprobs: Optional[torch.Tensor] = None,
+                 draft_logits: Optional[torch.Tensor] = None, uniform: Optional[torch.Tensor] = None,
+                 race: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                 draft_temperature: Optional[float] = None, greedy: bool = False,
+                 seq_lens: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None):
+    """Accepts or replaces the drafted tokens of a step.
+
+    ``target_logits`` ``[rows, vocab]``: row r is the distribution of the token
+    behind row r; ``tokens`` ``[rows]`` i32: what the rows were fed, so the rows
+    past a sequence's first are its drafts.  ``draft_logits``: row r is what row
+    r + 1's token was drawn from (None: the guesses have no distribution, each
+    counts as certain).  With p and q the softmaxes at ``temperature`` and
+    ``draft_temperature`` (the same by default), drafts x are accepted in order
+    while ``uniform[r] * q(x) < p(x)``; the token behind them is ``argmax w /
+    race[b]`` with w = max(p - q, 0) at a rejection and p behind the last draft, a
+    draw from w when ``race`` ``[num_seqs, vocab]`` is exponentially distributed.
+    ``greedy``: x is accepted while it is the argmax (ties: the lowest index),
+    and no random numbers or ``draft_logits`` are needed.
+
+    Writes ``out_tokens`` ``[num_seqs, max_tokens]`` i32 (accepted drafts, the new
+    token, -1 behind), ``accepted`` ``[num_seqs]`` i32, ``logprobs`` f32 (log p of
+    each token) and ``new_lens`` = ``seq_lens`` less the rejected drafts (which
+    may be ``seq_lens`` itself): the lengths that the next append starts from.
+    """
+    if not target_logits.is_cuda or target_logits.dim() != 2 or target_logits.dtype not in _TYPES or out_tokens.dim() != 2:
+        raise ValueError("target_logits: [rows, vocab] f32, f16 or bf16 on a CUDA device, out_tokens: [num_seqs, max_tokens] expected")
+    dev, dt = target_logits.get_device(), target_logits.dtype
+    rows, vocab = target_logits.shape
+    seqs, most = out_tokens.shape
+    a = _VerifyArgs(ctypes.sizeof(_VerifyArgs), _matrix(target_logits, "target_logits", rows, vocab, dt, dev), None,
+                    _vector(tokens, "tokens", rows, torch.int32, dev))
+    if starts is not None:
+        a.starts = _vector(starts, "starts", seqs + 1, torch.int32, dev)
+    a.tokens, a.num_seqs, a.vocab, a.max_tokens = rows, seqs, vocab, most
+    a.target_stride = target_logits.stride(0)
+    a.temperature, a.dtype, a.greedy = temperature, _TYPES[dt], greedy
+    if not greedy:
+        if uniform is None or race is None:
+            raise ValueError("uniform and race are needed unless greedy")
+        a.uniform = _vector(uniform, "uniform", rows, torch.float32, dev)
+        a.race, a.race_stride = _matrix(race, "race", seqs, vocab, torch.float32, dev), race.stride(0)
+        if draft_logits is not None:
+            a.draft, a.draft_stride = _matrix(draft_logits, "draft_logits", rows, vocab, dt, dev), draft_logits.stride(0)
+            a.draft_temperature = temperature if draft_temperature is None else draft_temperature
+    if not out_tokens.is_contiguous():
+        raise ValueError("out_tokens must be contiguous")
+    a.tokens_out = _matrix(out_tokens, "out_tokens", seqs, most, torch.int32, dev)
+    a.accepted = _vector(accepted, "accepted", seqs, torch.int32, dev)
+    if logprobs is not None:
+        if not logprobs.is_contiguous():
+            raise ValueError("logprobs must be contiguous")
+        a.logprobs = _matrix(logprobs, "logprobs", seqs, most, torch.float32, dev)
+    if new_lens is not None:
+        if seq_lens is None:
+            raise ValueError("new_lens needs seq_lens")
+        a.seq_lens = _vector(seq_lens, "seq_lens", seqs, torch.int32, dev)
+        a.new_lens = _vector(new_lens, "new_lens", seqs, torch.int32, dev)
+    lib, at = _library(), ctypes.addressof(a)
+    key = (dev, rows, seqs, vocab, most, starts is None, a.draft is None)
+    need = _verify_sizes.get(key)
+    if need is None:
+        need = _verify_sizes[key] = _size(dev, lib.verify_size, at)
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=target_logits.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
+    _enqueue(dev, lib.verify, at)

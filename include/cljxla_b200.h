@@ -147,6 +147,144 @@ CLJXLA_EXPORT int cljxla_b200_attention_decode_static(const void* q, const void*
                                                       int64_t kv_heads, int64_t positions, int64_t head_dim,
                                                       float scale, void* stream, char* err, size_t errcap);
 
+/* ------------------------------------------------- paged key-value cache
+ * Serving over a paged cache, for hosts that own device memory themselves (as
+ * with cljxla_b200_attention_decode_static).  No counterpart in the
+ * reference, whose paged cache is a design note only
+ * (docs/xla/paged_attention_vram.md:38-94).  One step of a serving loop is
+ *
+ *   paged_append     new K / V rows into their pages, K and Q rotated on the way
+ *   paged_attention  the step's queries over each sequence's pages
+ *   verify_draft     the drafted tokens among them accepted or replaced
+ *
+ * A step's tokens are packed rows: sequence b has rows starts[b] ..
+ * starts[b + 1] - 1, and seq_lens[b] counts its positions, those rows
+ * included, so row starts[b] + i is position seq_lens[b] - count + i.  Position
+ * j lives in row j % page_size of page page_table[b][j / page_size], for every
+ * KV head.  Rows at or behind starts[num_seqs] belong to nobody: nothing is
+ * read from or written to them, so a captured graph may carry padding.
+ *
+ * Every pointer below is a device pointer unless it says otherwise.  starts,
+ * seq_lens and page_table are read by the kernels when they run, so a captured
+ * graph follows their contents.  What the host cannot see is bounded in the
+ * kernels: seq_lens is clamped to [0, pages_per_seq * page_size], starts to
+ * [0, tokens], and a page number outside [0, num_pages) is a page that is not
+ * there: append leaves its rows out, attention leaves its positions out (so a
+ * sliding-window layer may give pages back and mark them -1).
+ *
+ * Work is enqueued on `stream` (a cudaStream_t; NULL = legacy default stream)
+ * of the calling thread's current device, without synchronising and without
+ * allocating device memory.  The argument structs are read before the call returns.
+ * struct_size is sizeof the struct.  Functions return 0, or a PJRT_Error_Code
+ * with the message in err[errcap]; a refused call has enqueued nothing. */
+typedef struct CLJXLA_PagedKV {
+  size_t struct_size;
+  void* k_pages; /* [num_pages, kv_heads, page_size, head_dim], strides below */
+  void* v_pages;
+  int64_t k_page_stride, k_head_stride, k_row_stride; /* in elements, >= 0; head_dim is contiguous */
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+  int64_t num_pages, kv_heads, page_size, head_dim;   /* head_dim 32, 64, 128 or 256 */
+  const int32_t* page_table; /* [num_seqs, pages_per_seq], row stride below */
+  const int32_t* seq_lens;   /* [num_seqs] */
+  int64_t num_seqs, pages_per_seq, page_table_stride;
+  int32_t dtype; /* PJRT_Buffer_Type F32, F16 or BF16: of the pages, and of q, k and v */
+  int32_t reserved;
+} CLJXLA_PagedKV;
+
+typedef struct CLJXLA_PagedAppendArgs {
+  size_t struct_size;
+  const void* k; /* [tokens, kv_heads, head_dim], strides in elements, head_dim contiguous */
+  const void* v;
+  const void* q; /* [tokens, q_heads, head_dim], or NULL: no queries */
+  void* q_out;   /* the rotated queries; may be q itself (same strides) */
+  int64_t tokens, q_heads;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+  const int32_t* starts;  /* [num_seqs + 1], ascending; NULL: tokens / num_seqs rows each */
+  const float* inv_freq;  /* [rotary_dim / 2] angle per position of each pair; NULL with rotary_dim 0 */
+  int64_t rotary_dim;     /* even, <= head_dim: elements past it are copied */
+  int32_t interleaved;    /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+  float rope_scale;       /* factor on cos and sin (1 for none) */
+} CLJXLA_PagedAppendArgs;
+
+/* Rotates K and Q rows by their positions and writes K and V into the pages:
+ * (x1, x2) -> rope_scale * (x1 cos a - x2 sin a, x2 cos a + x1 sin a) with a =
+ * position * inv_freq[i] (the angle reduced in 64 bits), computed in f32 and
+ * rounded once.  Two rows of one call must not share a (page, row): which of
+ * them stays is not defined.  Tensors of any element alignment; 16-byte
+ * aligned ones with rotary_dim / 2 (interleaved: rotary_dim) a multiple of 16
+ * bytes are the fast ones. */
+CLJXLA_EXPORT int cljxla_b200_paged_append(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAppendArgs* args, void* stream,
+                                           char* err, size_t errcap);
+
+typedef struct CLJXLA_PagedAttentionArgs {
+  size_t struct_size;
+  const void* q; /* [tokens, q_heads, head_dim], strides in elements, 16-byte aligned rows */
+  void* out;     /* same shape, out_dtype, 16-byte aligned rows */
+  int64_t tokens, q_heads; /* q_heads a multiple of kv_heads */
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  const int32_t* starts; /* [num_seqs + 1], ascending; NULL: tokens / num_seqs rows each */
+  int64_t max_tokens;    /* upper bound of a sequence's rows (rows past it are not computed) */
+  int64_t window;        /* >= 0: a row sees its own position and `window` before it; < 0: all */
+  float scale, softcap;  /* score = softcap * tanh(scale * q.k / softcap), or scale * q.k with softcap 0 */
+  int32_t out_dtype;     /* the pages' type, or F32 */
+  int32_t reserved;
+  void* workspace;       /* of cljxla_b200_paged_attention_workspace bytes, 16-byte aligned; needs no
+                            initialisation; calls that may overlap need one each */
+  int64_t workspace_bytes;
+} CLJXLA_PagedAttentionArgs;
+
+/* Row r at position p of its sequence: out = sum_j w_j v_j / sum_j w_j over the
+ * positions j <= p (and j >= p - window) of the sequence's pages, w_j =
+ * exp(score_j - max).  A row that sees no position is zero.  What a row does
+ * not see (later drafts, evicted pages, page tails) may hold anything, NaN and
+ * infinities included.  K and V pages must be 16-byte aligned rows. */
+CLJXLA_EXPORT int cljxla_b200_paged_attention(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAttentionArgs* args,
+                                              void* stream, char* err, size_t errcap);
+
+/* Bytes of workspace the call above needs on the current device (0: none;
+ * pointers are not looked at).  Depends on the sizes, not on the contents. */
+CLJXLA_EXPORT int cljxla_b200_paged_attention_workspace(const CLJXLA_PagedKV* kv,
+                                                        const CLJXLA_PagedAttentionArgs* args, int64_t* bytes,
+                                                        char* err, size_t errcap);
+
+typedef struct CLJXLA_VerifyDraftArgs {
+  size_t struct_size;
+  const void* target; /* [tokens, vocab] logits: row r is the distribution of the token behind row r */
+  const void* draft;  /* [tokens, vocab] logits row r + 1's token was drawn from; NULL: the guesses have no
+                         distribution (each counts as certain). A sequence's last row is not read */
+  const int32_t* tokens_in; /* [tokens] the tokens the rows were fed: rows past a sequence's first are drafts */
+  const int32_t* starts;    /* [num_seqs + 1], ascending; NULL: tokens / num_seqs rows each */
+  const float* uniform;     /* [tokens] in [0, 1): row r decides on row r + 1's token; NULL when greedy */
+  const float* race;        /* [num_seqs, vocab] positive, exponentially distributed; NULL when greedy */
+  int64_t tokens, num_seqs, vocab, max_tokens; /* max_tokens: upper bound of a sequence's rows, at most 128 */
+  int64_t target_stride, draft_stride, race_stride; /* elements from row to row */
+  float temperature, draft_temperature; /* logits are divided by these, > 0 */
+  int32_t dtype;  /* of target and draft: F32, F16 or BF16 */
+  int32_t greedy;
+  int32_t* tokens_out; /* [num_seqs, max_tokens]: accepted drafts, then the target's own token, then -1 */
+  int32_t* accepted;   /* [num_seqs]: accepted drafts */
+  float* logprobs;     /* [num_seqs, max_tokens] log p of each token in tokens_out (0 behind them), or NULL */
+  const int32_t* seq_lens; /* [num_seqs], or NULL with new_lens */
+  int32_t* new_lens;       /* seq_lens less the rejected drafts; may be seq_lens itself */
+  void* workspace;         /* of cljxla_b200_verify_draft_workspace bytes, 16-byte aligned; as above */
+  int64_t workspace_bytes;
+} CLJXLA_VerifyDraftArgs;
+
+/* With p = softmax(target / temperature) and q = softmax(draft /
+ * draft_temperature), a sequence's drafts x are accepted in order while
+ * uniform * q(x) < p(x).  The token behind the accepted ones is argmax_v
+ * w_v / race_v, a draw from w / sum w: w = max(p - q, 0) at a rejection (p
+ * without x where draft is NULL; p where that leaves nothing), p behind the last
+ * draft.  greedy: x is accepted while it is the argmax, and the argmax follows.
+ * Ties go to the lowest index.  A draft outside [0, vocab) is rejected.  Logits
+ * may be -inf (probability 0); a row without a finite maximum gives token -1. A
+ * sequence without rows gives 0 accepted, -1 throughout and its length. */
+CLJXLA_EXPORT int cljxla_b200_verify_draft(const CLJXLA_VerifyDraftArgs* args, void* stream, char* err,
+                                           size_t errcap);
+CLJXLA_EXPORT int cljxla_b200_verify_draft_workspace(const CLJXLA_VerifyDraftArgs* args, int64_t* bytes, char* err,
+                                                     size_t errcap);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,8 +38,12 @@ struct PagedAttnParams {
   int32_t group, hd, dt, out_f32, max_rows, pad_;  // max_rows: rows of a sequence at most
   int64_t window;  // < 0: none
   float scale, softcap;
-  float* part;
-  int32_t* meta;
+  // set at the launch: positions of a schedule unit, the factor from q.k to the
+  // argument of 2^x (with a cap: of tanh), log2(e) * softcap
+  int32_t unit;
+  float mul, cap2;
+  float* part;    // per CTA: two slots of rows and their (max, sum)
+  int32_t* meta;  // per CTA: CTAs that share the segment starting there (0: none), sequence, head, first row
 };
 
 struct VerifyParams {
@@ -60,8 +64,13 @@ struct VerifyParams {
 };
 
 void launch_paged_append(const PagedAppendParams& p, cudaStream_t s);
-void launch_paged_attention(const PagedAttnParams& p, cudaStream_t s);
-int64_t paged_attention_workspace(const PagedAttnParams& p);
+// by element type (one translation unit each)
+void launch_paged_attention_bf16(const PagedAttnParams& p, cudaStream_t s);
+void launch_paged_attention_f16(const PagedAttnParams& p, cudaStream_t s);
+void launch_paged_attention_f32(const PagedAttnParams& p, cudaStream_t s);
+int64_t paged_attention_workspace_bf16(const PagedAttnParams& p);
+int64_t paged_attention_workspace_f16(const PagedAttnParams& p);
+int64_t paged_attention_workspace_f32(const PagedAttnParams& p);
 void launch_verify(const VerifyParams& p, cudaStream_t s);
 int verify_splits(int64_t tokens, int64_t vocab, bool draft);
 int64_t verify_workspace(const VerifyParams& p);

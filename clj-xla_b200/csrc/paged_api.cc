@@ -124,6 +124,11 @@ PagedView view_of(const CLJXLA_PagedKV* kv, int64_t tokens, const int32_t* start
   return c;
 }
 
+int64_t attention_workspace(const PagedAttnParams& p) {
+  return p.dt == KDT_F32 ? paged_attention_workspace_f32(p)
+                         : (p.dt == KDT_F16 ? paged_attention_workspace_f16(p) : paged_attention_workspace_bf16(p));
+}
+
 bool nothing_to_do(const PagedView& c) { return c.tokens == 0 || c.num_seqs == 0; }
 
 PagedAttnParams attention_params(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAttentionArgs* a, bool pointers) {
@@ -304,7 +309,7 @@ extern "C" CLJXLA_EXPORT int cljxla_b200_paged_attention_workspace(const CLJXLA_
   return entry("paged_attention_workspace", err, errcap, [&] {
     need(bytes != nullptr, "null bytes");
     const PagedAttnParams p = attention_params(kv, a, false);
-    *bytes = nothing_to_do(p.c) ? 0 : paged_attention_workspace(p);
+    *bytes = nothing_to_do(p.c) ? 0 : attention_workspace(p);
   });
 }
 
@@ -313,12 +318,14 @@ extern "C" CLJXLA_EXPORT int cljxla_b200_paged_attention(const CLJXLA_PagedKV* k
   return entry("paged_attention", err, errcap, [&] {
     PagedAttnParams p = attention_params(kv, a, true);
     if (nothing_to_do(p.c)) return;
-    const int64_t want = paged_attention_workspace(p);
+    const int64_t want = attention_workspace(p);
     if (want > 0 && (!a->workspace || a->workspace_bytes < want))
       fail(E_INVALID, "workspace of " + std::to_string(a->workspace ? a->workspace_bytes : 0) + " bytes, " +
                           std::to_string(want) + " needed");
     p.part = (float*)a->workspace;
-    launch_paged_attention(p, (cudaStream_t)stream);
+    if (p.dt == KDT_F32) launch_paged_attention_f32(p, (cudaStream_t)stream);
+    else if (p.dt == KDT_F16) launch_paged_attention_f16(p, (cudaStream_t)stream);
+    else launch_paged_attention_bf16(p, (cudaStream_t)stream);
   });
 }
 

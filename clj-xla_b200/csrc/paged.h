@@ -38,9 +38,8 @@ struct PagedAttnParams {
   int32_t group, hd, dt, out_f32, max_rows, pad_;  // max_rows: rows of a sequence at most
   int64_t window;  // < 0: none
   float scale, softcap;
-  // set at the launch: positions of a schedule unit, the factor from q.k to the
-  // argument of 2^x (with a cap: of tanh), log2(e) * softcap
-  int32_t unit;
+  // set at the launch: the factor from q.k to the argument of 2^x (with a cap:
+  // of tanh), log2(e) * softcap
   float mul, cap2;
   float* part;    // per CTA: two slots of rows and their (max, sum)
   int32_t* meta;  // per CTA: CTAs that share the segment starting there (0: none), sequence, head, first row

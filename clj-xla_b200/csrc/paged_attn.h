@@ -10,22 +10,22 @@
 // bound is HBM bandwidth as long as enough copies are in flight.
 //
 // Split.  A segment is (sequence, KV head, up to ROWS query rows of that head's
-// group); its positions come in units of 16.  All units of the call, laid end
-// to end, are cut into one equal range per CTA, whatever the sequences'
-// lengths: one long context fills the GPU as well as many ragged ones do.  Each
+// group), a row of tiles of its positions.  All tiles of the call, laid end to
+// end, are cut into one equal range per CTA, whatever the sequences' lengths: one long context fills the GPU as well as many ragged ones do.  Each
 // CTA finds its range itself from seq_lens (a scan over the sequences), so a
 // captured graph follows the lengths.  A segment that lies within one CTA is
 // finished there; a cut one leaves (m, sum, unnormalised row) partials that
 // paged_attn_join_kernel, launched as a programmatic dependent, adds up in
 // range order: no atomics, the same bits every time.
 //
-// Tile.  64 positions (32 in f32) of K and V rows are copied by all threads
-// with 16-byte cp.async into a ring of stages, rows gathered through the page
-// table (any page size, any strides), positions nobody sees filled with zeros
-// and not read.  The page numbers of a tile are fetched one iteration before
-// its copies start.  Four warps score 16 (8) positions each on mma.sync, share
-// row maxima and weights through shared memory, and each adds P.V for a quarter
-// of head_dim, so the accumulators stay small and no warp holds partials.
+// Tile.  64 positions (32 in f32) of K and V rows go through a ring of stages.
+// Warp 4 is the producer: it walks the schedule, looks the pages of a tile up
+// one tile ahead, and gathers the rows with 16-byte cp.async (any page size, any
+// strides; positions nobody sees are filled with zeros and not read).  Warps 0
+// to 3 score 16 (8) positions each on mma.sync, share row maxima and weights
+// through shared memory, and each adds P.V for a quarter of head_dim, so the
+// accumulators stay small and no warp holds partials.  Stages change hands over
+// named barriers.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -40,7 +40,7 @@
 namespace cljxla {
 namespace {
 
-constexpr int AT_THREADS = 128;
+constexpr int AT_CONSUMERS = 128, AT_THREADS = AT_CONSUMERS + 32, AT_JOIN_THREADS = 128;
 constexpr int kAttnMaxCtas = 1024;  // SMs times CTAs on one, at most
 
 // ------------------------------------------------------------------ layout
@@ -58,16 +58,14 @@ struct Tile {
   // weights as two 16-bit parts or one f32: in the tile's K rows once they are scored, if they fit
   static constexpr int PB = ROWS * TP * 4;
   static constexpr bool P_IN_K = PB <= KB;
-  static constexpr int fixed(int nst) {
-    return (P_IN_K ? 0 : PB) + nst * TP * 16 + 2 * 4 * ROWS * 4 + (nst + 1) * 64 + 80;
-  }
+  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 64 + TP * 16; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
     int n = 0;
     while (n < 4 && fixed(n + 1) + (n + 1) * STAGE <= 233472 / ctas - 1024) ++n;
     return n;
   }
   static constexpr int pick() {
-    int ctas = HD >= 256 ? 1 : HD == 128 ? 2 : HD == 64 ? 3 : 4;
+    int ctas = HD >= 256 ? 1 : HD == 128 ? 2 : 3;
     while (ctas > 1 && fit(ctas) < 3) --ctas;
     return ctas;
   }
@@ -94,12 +92,20 @@ __device__ __forceinline__ int swz_v(int c, int r) {
 // -------------------------------------------------------------- primitives
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));  // ordered by the commit, not among themselves
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bar_arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -162,26 +168,43 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*(const __half2*)&v);
   else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
+// tanh: from 2^x where that is accurate (1 - 2 / (1 + e^2y) is off by about
+// 2^-23), from its series where that would cancel (|y| < 0.1: the next term is
+// below 2^-32 of the result)
+__device__ __forceinline__ float tanh_f(float y) {
+  const float big = 1.f - __fdividef(2.f, 1.f + ex2(y * 2.8853900817779268f));
+  const float z = y * y;
+  const float small = y * fmaf(z, fmaf(z, fmaf(z, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  return fabsf(y) < 0.1f ? small : big;
+}
 // whether either 16-bit value is an infinity or NaN
 template <typename T>
 __device__ __forceinline__ bool odd2(uint32_t v) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return (v & e) == e || ((v >> 16) & e) == e;
 }
-__device__ __forceinline__ bool odd1(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+template <typename T>
+__device__ __forceinline__ bool odd_chunk(const uint4& v) {
+  if constexpr (sizeof(T) == 2) {
+    return odd2<T>(v.x) || odd2<T>(v.y) || odd2<T>(v.z) || odd2<T>(v.w);
+  } else {
+    constexpr uint32_t e = 0x7f800000u;
+    return (v.x & e) == e || (v.y & e) == e || (v.z & e) == e || (v.w & e) == e;
+  }
+}
 
 // --------------------------------------------------------------- schedule
 // A tile: positions [pos0, pos0 + npos) of segment (b, head, rows row0 ..).
 struct TileDesc {
-  int b, head, row0, pos0, npos, flags, qslot, first, count, p0;  // p0: position of the sequence's first row
+  int head, row0, pos0, npos, flags, qslot, first, count, p0;  // p0: position of the sequence's first row
   uint32_t mask[2];  // positions whose page is there
 };
-enum { T_FIRST = 1, T_LAST = 2, T_FROM0 = 4, T_TOEND = 8, T_FULL = 16 };
+enum { T_FIRST = 1, T_LAST = 2, T_FROM0 = 4, T_TOEND = 8, T_FULL = 16, T_END = 32 };  // T_END: the CTA's last tile
 
 // One sequence's share of the schedule.
 struct SeqPlan {
   int first, count, rows, p0, lo, hi, units, tiles;  // rows: computed ones; tiles: row tiles
-  __device__ __forceinline__ void load(const PagedAttnParams& P, int b, int unit, int row_tile) {
+  __device__ __forceinline__ void load(const PagedAttnParams& P, int b, int tile, int row_tile) {
     int n;
     seq_rows(P.c, b, first, n);
     count = min(n, P.max_rows);
@@ -190,7 +213,7 @@ struct SeqPlan {
     p0 = seq_len(P.c, b) - n;
     lo = P.window < 0 ? 0 : (int)max((int64_t)p0 - P.window, (int64_t)0);
     hi = min(p0 + count, capacity(P.c));
-    units = max((hi - lo + unit - 1) / unit, 1);
+    units = max((hi - lo + tile - 1) / tile, 1);
   }
   __device__ __forceinline__ int64_t cost(int nkv) const { return (int64_t)units * nkv * tiles; }
 };
@@ -201,30 +224,28 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
   using L = Tile<T, HD, MT>;
   constexpr int TP = L::TP, WP = L::WP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST;
   constexpr int NT = HD / 32;  // 8-column output tiles of a warp
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* const ring = smem;
   unsigned char* const p_own = smem + NST * L::STAGE;
-  int64_t* const offs = (int64_t*)(p_own + (L::P_IN_K ? 0 : L::PB));  // [NST][TP][K, V]
-  float* const wmax = (float*)(offs + NST * TP * 2);                  // [4][ROWS]
+  float* const wmax = (float*)(p_own + (L::P_IN_K ? 0 : L::PB));  // [4][ROWS]
   float* const wsum = wmax + 4 * ROWS;
-  TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST + 1]
-  int64_t* const sh = (int64_t*)((unsigned char*)desc + (NST + 1) * 64);
-  int* const posted = (int*)(sh + 8);  // tiles the cursor has posted
+  TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
+  int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
+  longlong2* const offs = (longlong2*)(sh + 8);  // [TP] the producer's K and V row offsets
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedView& c = P.c;
-  const int unit = P.unit;
   pdl_enter();
 
-  // ---- this CTA's range of units
-  int64_t left;
+  // ---- this CTA's range of tiles
+  int64_t left, total = 0, ctas;
   {
     SeqPlan sp;
     const int per = (c.num_seqs + AT_THREADS - 1) / AT_THREADS;
     const int b0 = min(tid * per, c.num_seqs), b1 = min(b0 + per, c.num_seqs);
     int64_t mine = 0;
     for (int i = b0; i < b1; ++i) {
-      sp.load(P, i, unit, ROWS);
+      sp.load(P, i, TP, ROWS);
       mine += sp.cost(c.nkv);
     }
     int64_t incl = mine;
@@ -235,34 +256,30 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
     }
     if (lane == 31) sh[warp] = incl;
     __syncthreads();
-    int64_t total = 0;
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < AT_THREADS / 32; ++w) {
       if (w < warp) incl += sh[w];
       total += sh[w];
     }
-    // at least a tile each
-    const int64_t ctas = min((int64_t)gridDim.x, (total * unit + TP - 1) / TP);
+    ctas = min((int64_t)gridDim.x, total);
     if ((int64_t)blockIdx.x >= ctas) {
       if (tid == 0 && P.meta) P.meta[blockIdx.x * 4] = 0;
       return;
     }
     const int64_t beg = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
     left = end - beg;
+    __syncthreads();
     if (tid == 0) {
-      *posted = 0;
-      sh[4] = sh[5] = 0;
-      sh[6] = total;
-      sh[7] = ctas;
+      sh[0] = sh[1] = 0;
       if (P.meta) P.meta[blockIdx.x * 4] = 0;  // no segment that starts here is cut, so far
     }
     __syncthreads();
     int64_t excl = incl - mine;
     if (beg >= excl && beg < incl) {
       for (int i = b0; i < b1; ++i) {
-        sp.load(P, i, unit, ROWS);
+        sp.load(P, i, TP, ROWS);
         if (beg < excl + sp.cost(c.nkv)) {
-          sh[4] = i;
-          sh[5] = beg - excl;
+          sh[0] = i;
+          sh[1] = beg - excl;
           break;
         }
         excl += sp.cost(c.nkv);
@@ -271,140 +288,186 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
     __syncthreads();
   }
 
-  // ---- the schedule's cursor, run by warp 0 alone: what the other warps do
-  // follows what it posts in shared memory
-  int b = 0, seg = 0, at = 0;  // sequence, segment of it (head, row tile), unit of that
-  SeqPlan sp{};
-  if (warp == 0) {
-    b = (int)sh[4];
-    const int64_t off = sh[5];
-    sp.load(P, b, unit, ROWS);
+  // Stage hand-over: full[s] (producer arrives, consumers wait), empty[s] the other way round.
+  constexpr int FULL = 2, EMPTY = FULL + NST, INNER = 1;
+
+  if (warp == AT_CONSUMERS / 32) {
+    // ================================================================ producer
+    int b = (int)sh[0];  // cursor: sequence, segment of it (head, row tile), tile of that
+    SeqPlan sp;
+    sp.load(P, b, TP, ROWS);
+    const int64_t off = sh[1];
     if (off >= sp.cost(c.nkv)) left = 0;  // lengths that change under the kernel: stay in bounds
-    seg = (int)(off / sp.units);
-    at = (int)(off % sp.units);
-  }
-  int qslot = -1;
-  bool fresh = true;  // the next tile is the first of its piece
-  TileDesc nd;
-  int page[TP / 32], in_page[TP / 32];
-  auto next = [&]() -> bool {  // the cursor's next tile into nd; starts its page lookup
-    if (left == 0) return false;
-    if (at >= sp.units) {
-      at = 0;
-      if (++seg >= c.nkv * sp.tiles) {
-        seg = 0;
-        do {
-          if (++b >= c.num_seqs) {
-            left = 0;
-            return false;
+    int seg = (int)(off / sp.units), at = (int)(off % sp.units), qslot = -1;
+    bool fresh = true;  // the next tile is the first of its piece
+    bool piece0 = false;  // whether the piece starts its segment
+    TileDesc nd;
+    int page[TP / 32], in_page[TP / 32];
+    auto next = [&]() -> bool {  // the cursor's next tile into nd; starts its page lookup
+      if (left == 0) return false;
+      if (at >= sp.units) {
+        at = 0;
+        if (++seg >= c.nkv * sp.tiles) {
+          seg = 0;
+          do {
+            if (++b >= c.num_seqs) {
+              left = 0;
+              return false;
+            }
+            sp.load(P, b, TP, ROWS);
+          } while (sp.tiles == 0);
+        }
+        fresh = true;
+      }
+      if (fresh) {
+        qslot = qslot + 1 == NST ? 0 : qslot + 1;
+        piece0 = at == 0;
+      }
+      nd.head = sp.tiles == 1 ? seg : seg / sp.tiles;
+      nd.row0 = (seg - nd.head * sp.tiles) * ROWS;
+      nd.pos0 = sp.lo + at * TP;
+      nd.npos = max(min(TP, sp.hi - nd.pos0), 0);
+      nd.qslot = qslot;
+      nd.first = sp.first;
+      nd.count = sp.count;
+      nd.p0 = sp.p0;
+      nd.flags = (fresh ? T_FIRST : 0) | (piece0 ? T_FROM0 : 0);
+      ++at;
+      --left;
+      if (at == sp.units) nd.flags |= T_LAST | T_TOEND;
+      if (left == 0) {
+        nd.flags |= T_LAST;
+        if (piece0 && at < sp.units && lane == 0) {
+          // the range ends inside a segment that starts here: its last tile belongs to CTA `to`
+          const int64_t end = total * (blockIdx.x + 1) / ctas;
+          const int64_t to = ((end + (sp.units - at)) * ctas - 1) / total;
+          int32_t* meta = P.meta + blockIdx.x * 4;
+          meta[0] = (int32_t)(min(to, ctas - 1) - blockIdx.x + 1);
+          meta[1] = b;
+          meta[2] = nd.head;
+          meta[3] = nd.row0;
+        }
+      }
+      // every row sees every position, were all pages there
+      if (nd.npos == TP && nd.pos0 + TP - 1 <= nd.p0 && (P.window < 0 || nd.pos0 >= nd.p0 + nd.count - 1 - P.window))
+        nd.flags |= T_FULL;
+      fresh = false;
+#pragma unroll
+      for (int i = 0; i < TP / 32; ++i) {
+        const int j = nd.pos0 + i * 32 + lane;
+        page[i] = -1;
+        in_page[i] = 0;
+        if (i * 32 + lane < nd.npos) {
+          const int slot = j / c.page_size;
+          page[i] = c.table[(int64_t)b * c.table_stride + slot];
+          in_page[i] = j - slot * c.page_size;
+        }
+      }
+      return true;
+    };
+
+    constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
+    constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
+    constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
+    const int my_row = lane / LANES, my_chunk = lane % LANES;
+    int tile = 0;
+    bool have = next();
+    if (!have) {  // only if lengths change under the kernel: a tile of nothing ends the consumers
+      if (lane == 0) *(TileDesc*)desc = TileDesc{0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
+      bar_arrive<AT_THREADS>(FULL);
+      return;
+    }
+    while (have) {
+      // tell the consumers of the oldest tile in flight before waiting for a free stage
+      if (tile >= NST - 1) {
+        cp_wait<NST - 2>();
+        bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
+      }
+      const int slot = tile % NST;
+      if (tile >= NST) bar_sync<AT_THREADS>(EMPTY + slot);
+      __syncwarp();  // offs of the tile before are read
+#pragma unroll
+      for (int i = 0; i < TP / 32; ++i) {
+        const bool ok = (unsigned)page[i] < (unsigned)c.num_pages;
+        longlong2 o;
+        o.x = ok ? page[i] * c.k_page + nd.head * c.k_head + in_page[i] * c.k_row : -1;
+        o.y = ok ? page[i] * c.v_page + nd.head * c.v_head + in_page[i] * c.v_row : -1;
+        offs[i * 32 + lane] = o;
+        nd.mask[i] = __ballot_sync(0xffffffffu, ok);
+      }
+      if (lane == 0) *(TileDesc*)((char*)desc + slot * 64) = nd;
+      __syncwarp();
+      const uint32_t kd = smem_u32(ring + slot * L::STAGE), vd = kd + L::KB;
+      // eight rows' offsets are fetched before their copies are issued: the warp's
+      // time goes to issue, not to the latency of each row's address
+      constexpr int BATCH = 8;
+      static_assert(TP % (BATCH * RPI) == 0, "whole batches");
+#pragma unroll 1
+      for (int r0 = 0; r0 < TP; r0 += BATCH * RPI) {
+        longlong2 o[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) o[i] = offs[r0 + i * RPI + my_row];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const int r = r0 + i * RPI + my_row, rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
+          const int size = o[i].x >= 0 ? 16 : 0;
+          const char* kp = (size ? c.k + o[i].x : P.q) + my_chunk * 16;
+          const char* vp = (size ? c.v + o[i].y : P.q) + my_chunk * 16;
+#pragma unroll
+          for (int e = 0; e < CPL; ++e) {
+            const int ch = my_chunk + e * LANES;
+            cp16(kd + r * RB + swz<CPR>(ch, rr) * 16, kp + (size ? e * LANES * 16 : 0), size);
+            cp16(vd + r * RB + swz_v<T, CPR>(ch, rr) * 16, vp + (size ? e * LANES * 16 : 0), size);
           }
-          sp.load(P, b, unit, ROWS);
-        } while (sp.tiles == 0);
+        }
       }
-      fresh = true;
-    }
-    if (fresh) qslot = qslot + 1 == NST ? 0 : qslot + 1;
-    const int k = (int)min((int64_t)min(TP / unit, sp.units - at), left);
-    nd.b = b;
-    nd.head = seg / sp.tiles;
-    nd.row0 = (seg % sp.tiles) * ROWS;
-    nd.pos0 = sp.lo + at * unit;
-    nd.npos = max(min(k * unit, sp.hi - nd.pos0), 0);
-    nd.qslot = qslot;
-    nd.first = sp.first;
-    nd.count = sp.count;
-    nd.p0 = sp.p0;
-    nd.flags = (fresh ? T_FIRST : 0) | (at == 0 ? T_FROM0 : 0);
-    at += k;
-    left -= k;
-    if (at == sp.units) nd.flags |= T_LAST | T_TOEND;
-    if (left == 0) nd.flags |= T_LAST;
-    // every row sees every position, were all pages there
-    if (nd.npos == TP && nd.pos0 + TP - 1 <= nd.p0 && (P.window < 0 || nd.pos0 >= nd.p0 + nd.count - 1 - P.window))
-      nd.flags |= T_FULL;
-    fresh = false;
+      if (nd.flags & T_FIRST) {
+        const uint32_t qd = smem_u32(ring + qslot * L::STAGE + 2 * L::KB);
+        for (int r0 = 0; r0 < ROWS; r0 += RPI) {
+          const int r = r0 + my_row, row = nd.row0 + r;
+          const bool ok = row < nd.count * P.group;
+          const int qi = row / P.group;
+          const char* src = ok ? P.q + (int64_t)(nd.first + qi) * P.q_tok +
+                                     (int64_t)(nd.head * P.group + row - qi * P.group) * P.q_head
+                               : P.q;
 #pragma unroll
-    for (int i = 0; i < TP / 32; ++i) {
-      const int j = nd.pos0 + i * 32 + lane;
-      page[i] = -1;
-      in_page[i] = 0;
-      if (i * 32 + lane < nd.npos) {
-        page[i] = c.table[(int64_t)b * c.table_stride + j / c.page_size];
-        in_page[i] = j % c.page_size;
+          for (int e = 0; e < CPL; ++e) {
+            const int ch = my_chunk + e * LANES;
+            cp16(qd + r * RB + swz<CPR>(ch, r) * 16, src + (ok ? ch * 16 : 0), ok ? 16 : 0);
+          }
+        }
       }
+      cp_commit();
+      have = next();
+      if (!have && lane == 0) ((TileDesc*)((char*)desc + slot * 64))->flags |= T_END;
+      ++tile;
     }
-    return true;
-  };
-  auto post = [&](int tile) {  // nd and its rows' offsets, visible at the next barrier
-    const int slot = tile % NST;
-    TileDesc& d = desc[tile % (NST + 1)];
+    // the tiles still in flight
 #pragma unroll
-    for (int i = 0; i < TP / 32; ++i) {
-      const bool ok = (unsigned)page[i] < (unsigned)c.num_pages;
-      int64_t* o = offs + (slot * TP + i * 32 + lane) * 2;
-      o[0] = ok ? page[i] * c.k_page + nd.head * c.k_head + in_page[i] * c.k_row : -1;
-      o[1] = ok ? page[i] * c.v_page + nd.head * c.v_head + in_page[i] * c.v_row : -1;
-      nd.mask[i] = __ballot_sync(0xffffffffu, ok);
+    for (int k = NST - 2; k >= 0; --k) {
+      if (tile - 1 - k < 0) continue;
+      if (k == 0) cp_wait<0>();
+      else if (k == 1) cp_wait<1>();
+      else cp_wait<2>();
+      bar_arrive<AT_THREADS>(FULL + (tile - 1 - k) % NST);
     }
-    if (lane == 0) {
-      d = nd;
-      *posted = tile + 1;
-    }
-  };
-  auto copy = [&](int tile) {
-    const int slot = tile % NST;
-    const TileDesc& d = desc[tile % (NST + 1)];
-    const uint32_t kd = smem_u32(ring + slot * L::STAGE), vd = kd + L::KB;
-    const int64_t* of = offs + slot * TP * 2;
-#pragma unroll 4
-    for (int i = tid; i < TP * CPR; i += AT_THREADS) {
-      const int r = i / CPR, ch = i % CPR;
-      const int64_t ko = of[r * 2], vo = of[r * 2 + 1];
-      cp16(kd + r * RB + swz<CPR>(ch, r) * 16, ko >= 0 ? c.k + ko + ch * 16 : P.q, ko >= 0 ? 16 : 0);
-      cp16(vd + r * RB + swz_v<T, CPR>(ch, r) * 16, vo >= 0 ? c.v + vo + ch * 16 : P.q, vo >= 0 ? 16 : 0);
-    }
-    if (d.flags & T_FIRST) {
-      const uint32_t qd = smem_u32(ring + d.qslot * L::STAGE + 2 * L::KB);
-      for (int i = tid; i < ROWS * CPR; i += AT_THREADS) {
-        const int r = i / CPR, ch = i % CPR, row = d.row0 + r;
-        const bool ok = row < d.count * P.group;
-        const char* src = ok ? P.q + (int64_t)(d.first + row / P.group) * P.q_tok +
-                                   (int64_t)(d.head * P.group + row % P.group) * P.q_head + ch * 16
-                             : P.q;
-        cp16(qd + r * RB + swz<CPR>(ch, r) * 16, src, ok ? 16 : 0);
-      }
-    }
-  };
-
-  if (warp == 0)
-    for (int i = 0; i < NST && next(); ++i) post(i);
-  __syncthreads();
-  int tiles = *posted;
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s) {
-    if (s < tiles) copy(s);
-    cp_commit();
+    for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<AT_THREADS>(EMPTY + k % NST);  // no arrival is left over
+    return;
   }
 
+  // ================================================================ consumers
   float acc[MT][NT][4], m[MT][2], l[MT][2];
-  bool from0 = false;  // whether the piece in work starts its segment
   const int g = lane >> 2, t4 = lane & 3;
-  for (int tile = 0; tile < tiles; ++tile) {
-    cp_wait<NST - 2>();
-    __syncthreads();  // this tile is there, and the one before it is done with
-    tiles = *posted;
-    if (tile + NST - 1 < tiles) copy(tile + NST - 1);
-    cp_commit();
-    const bool more = warp == 0 && next();
-
-    const TileDesc d = desc[tile % (NST + 1)];
-    unsigned char* const stage = ring + (tile % NST) * L::STAGE;
+  for (int tile = 0;; ++tile) {
+    const int slot = tile % NST;
+    bar_sync<AT_THREADS>(FULL + slot);
+    const TileDesc d = *(const TileDesc*)((char*)desc + slot * 64);
+    unsigned char* const stage = ring + slot * L::STAGE;
     const uint32_t ks = smem_u32(stage), vs = ks + L::KB, qs = smem_u32(ring + d.qslot * L::STAGE + 2 * L::KB);
     unsigned char* const pw = L::P_IN_K ? stage : p_own;
     const uint64_t vis = TP == 64 ? (uint64_t)d.mask[1] << 32 | d.mask[0] : d.mask[0];
     const bool plain = (d.flags & T_FULL) && vis == (TP == 64 ? ~0ull : 0xffffffffull);
     if (d.flags & T_FIRST) {
-      from0 = d.flags & T_FROM0;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         m[i][0] = m[i][1] = -INFINITY;
@@ -422,19 +485,34 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
 #pragma unroll
       for (int n = 0; n < SN; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
     if constexpr (L::ES == 2) {
-      const int kr = warp * WP + (lane >> 4) * 8 + (lane & 7), kc = (lane >> 3) & 1;
-      const int qr = (lane & 15), qc = lane >> 4;
+      // chunk 2 k + (0 or 1) of a row: its swizzled address differs from chunk
+      // 0 or 1's by an exclusive or with 32 k
+      const int kr = warp * WP + (lane >> 4) * 8 + (lane & 7), qr = lane & 15;
+      const uint32_t ka = ks + kr * RB + swz<CPR>((lane >> 3) & 1, kr) * 16;
+      const uint32_t qa = qs + qr * RB + swz<CPR>(lane >> 4, qr) * 16;
+      float s2[SN][4];  // one row tile: even and odd steps apart, to halve the chain of dependent products
+      if constexpr (MT == 1) {
+#pragma unroll
+        for (int n = 0; n < SN; ++n) s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
+      }
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         uint32_t kb[4];
-        ldsm4(ks + kr * RB + swz<CPR>(2 * k + kc, kr) * 16, kb);
+        ldsm4(ka ^ (k * 32), kb);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          uint32_t qa[4];
-          ldsm4(qs + (i * 16 + qr) * RB + swz<CPR>(2 * k + qc, qr) * 16, qa);
-          mma16<T>(s[i][0], qa, kb[0], kb[1]);
-          mma16<T>(s[i][SN - 1], qa, kb[2], kb[3]);
+          uint32_t a[4];
+          ldsm4((qa ^ (k * 32)) + i * 16 * RB, a);
+          float(*t)[4] = MT == 1 && (k & 1) ? s2 : s[i];
+          mma16<T>(t[0], a, kb[0], kb[1]);
+          mma16<T>(t[SN - 1], a, kb[2], kb[3]);
         }
+      }
+      if constexpr (MT == 1) {
+#pragma unroll
+        for (int n = 0; n < SN; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][n][e] += s2[n][e];
       }
     } else {
       const int kr = warp * WP + g;
@@ -463,7 +541,7 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = s[i][n][e] * P.mul;
-          if (P.softcap > 0.f) x = P.cap2 * tanhf(x);
+          if (P.softcap > 0.f) x = P.cap2 * tanh_f(x);
           s[i][n][e] = x;
         }
     int jhi[MT][2], jlo[MT][2];  // positions of this tile each of the thread's rows sees
@@ -484,8 +562,7 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int j = warp * WP + n * 8 + t4 * 2 + (e & 1);
-            const bool see = j <= jhi[i][e >> 1] && j >= jlo[i][e >> 1] && (vis >> j & 1u);
-            if (!see) s[i][n][e] = -INFINITY;
+            if (!(j <= jhi[i][e >> 1] && j >= jlo[i][e >> 1] && (vis >> j & 1u))) s[i][n][e] = -INFINITY;
           }
     }
 #pragma unroll
@@ -498,7 +575,7 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
         if (t4 == 0) wmax[warp * ROWS + i * 16 + r * 8 + g] = x;
       }
-    __syncthreads();  // maxima are there, and K is read: its rows may take the weights
+    bar_sync<AT_CONSUMERS>(INNER);  // maxima are there, and K is read: its rows may take the weights
 
     float alpha[MT][2];
 #pragma unroll
@@ -533,7 +610,7 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
         }
         l[i][r] = l[i][r] * alpha[i][r] + sum;
       }
-    __syncthreads();  // weights are there
+    bar_sync<AT_CONSUMERS>(INNER);  // weights are there
 
     // ---- P.V for this warp's quarter of head_dim
 #pragma unroll
@@ -546,80 +623,75 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
         acc[i][n][3] *= alpha[i][1];
       }
     // A position that some rows see and others do not may hold an infinity or
-    // NaN, which a weight of zero does not keep out of a matrix product.  Such
-    // values (found in the tiles with row-dependent masks only) are multiplied
-    // one by one for the rows that do see them.
-    auto one_by_one = [&](int j0, int nj, int n) {
-      for (int j = j0; j < j0 + nj; ++j) {
+    // NaN, which a weight of zero does not keep out of a matrix product.  Tiles
+    // with row-dependent masks look for such values first; with one of them in
+    // this warp's columns the products are made one by one, for the rows that
+    // do see the position.
+    bool odd = false;
+    if (!plain && d.count > 1) {
+      constexpr int W = RB / 64;  // 16-byte chunks of a row in a quarter of it
+#pragma unroll 1
+      for (int i = lane; i < TP * W; i += 32) {
+        const int j = i / W;
+        const uint4 v = *(const uint4*)(stage + L::KB + j * RB + swz_v<T, CPR>(warp * W + i % W, j) * 16);
+        odd = odd || odd_chunk<T>(v);
+      }
+      odd = __any_sync(0xffffffffu, odd);
+    }
+    if (odd) {
+#pragma unroll 1
+      for (int j = 0; j < TP; ++j) {
         if (!(vis >> j & 1u)) continue;
-        const int col = warp * (HD / 4) + n * 8 + t4 * 2;
-        float v0, v1;
-        if constexpr (L::ES == 2) {
-          const uint32_t vv = *(const uint32_t*)(stage + L::KB + j * RB + swz_v<T, CPR>(col / 8, j) * 16 + (col % 8) * 2);
-          const float2 f = unpack2<T>(vv);
-          v0 = f.x;
-          v1 = f.y;
-        } else {
-          const float* vp = (const float*)(stage + L::KB + j * RB);
-          v0 = vp[swz_v<T, CPR>(col / 4, j) * 4 + col % 4];
-          v1 = vp[swz_v<T, CPR>((col + 1) / 4, j) * 4 + (col + 1) % 4];
-        }
+        float p[MT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            if (j > jhi[i][r] || j < jlo[i][r]) continue;
             const int row = i * 16 + r * 8 + g;
-            float p;
             if constexpr (L::ES == 2) {
               const unsigned char* at16 = pw + row * (TP * 2) + (((j >> 3) ^ (row & 7)) * 16) + (j & 7) * 2;
-              p = (float)*(const T*)at16 + (float)*(const T*)(at16 + ROWS * TP * 2);
+              p[i][r] = (float)*(const T*)at16 + (float)*(const T*)(at16 + ROWS * TP * 2);
             } else {
-              p = *(const float*)(pw + row * (TP * 4) + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4);
+              p[i][r] = *(const float*)(pw + row * (TP * 4) + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4);
             }
-            acc[i][n][2 * r] += p * v0;
-            acc[i][n][2 * r + 1] += p * v1;
+          }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = warp * (HD / 4) + n * 8 + t4 * 2 + e;
+            constexpr int PC = 16 / L::ES;  // elements of a chunk
+            const float v = (float)((const T*)(stage + L::KB + j * RB + swz_v<T, CPR>(col / PC, j) * 16))[col % PC];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                if (j <= jhi[i][r] && j >= jlo[i][r]) acc[i][n][2 * r + e] += p[i][r] * v;
           }
       }
-    };
-    const bool wary = !plain && d.count > 1;
-    if constexpr (L::ES == 2) {
-      const uint32_t ps = smem_u32(pw);
+    } else if constexpr (L::ES == 2) {
+      const int pr = lane & 15;
+      const uint32_t pa = smem_u32(pw) + pr * (TP * 2) + (((lane >> 4) ^ (pr & 7)) * 16);
+      const uint32_t va = vs + pr * RB + swz_v<T, CPR>(warp * NT + (NT > 1 ? lane >> 4 : 0), pr) * 16;
 #pragma unroll
       for (int k = 0; k < TP / 16; ++k) {
         uint32_t ph[MT][4], pl[MT][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const int pr = i * 16 + (lane & 15);
-          const uint32_t a = ps + pr * (TP * 2) + (((2 * k + (lane >> 4)) ^ (pr & 7)) * 16);
-          ldsm4(a, ph[i]);
-          ldsm4(a + ROWS * TP * 2, pl[i]);
+          ldsm4((pa ^ (k * 32)) + i * 16 * TP * 2, ph[i]);
+          ldsm4((pa ^ (k * 32)) + (ROWS + i * 16) * TP * 2, pl[i]);
         }
-        const int vr = k * 16 + (lane & 15);
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
           uint32_t vb[4];
-          if constexpr (NT == 1) ldsm2t(vs + vr * RB + swz_v<T, CPR>(warp, vr) * 16, vb);
-          else ldsm4t(vs + vr * RB + swz_v<T, CPR>(warp * NT + n + (lane >> 4), vr) * 16, vb);
-          bool odd = false;
-          if (wary) {
-            odd = odd2<T>(vb[0]) || odd2<T>(vb[1]);
-            if (NT > 1) odd = odd || odd2<T>(vb[2]) || odd2<T>(vb[3]);
-            odd = __any_sync(0xffffffffu, odd);
-          }
-          if (odd) {
-            one_by_one(k * 16, 16, n);
-            if (NT > 1) one_by_one(k * 16, 16, n + 1);
-            continue;
-          }
+          if constexpr (NT == 1) ldsm2t(va + k * 16 * RB, vb);
+          else ldsm4t((va ^ (n * 16)) + k * 16 * RB, vb);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             mma16<T>(acc[i][n], ph[i], vb[0], vb[1]);
+            if constexpr (NT > 1) mma16<T>(acc[i][n + 1], ph[i], vb[2], vb[3]);
             mma16<T>(acc[i][n], pl[i], vb[0], vb[1]);
-            if constexpr (NT > 1) {
-              mma16<T>(acc[i][n + 1], ph[i], vb[2], vb[3]);
-              mma16<T>(acc[i][n + 1], pl[i], vb[2], vb[3]);
-            }
+            if constexpr (NT > 1) mma16<T>(acc[i][n + 1], pl[i], vb[2], vb[3]);
           }
         }
       }
@@ -641,15 +713,12 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
         for (int n = 0; n < NT; ++n) {
           const int col = warp * (HD / 4) + n * 8 + g;
           const float b0 = v0p[swz_v<T, CPR>(col / 4, r0) * 4 + col % 4], b1 = v1p[swz_v<T, CPR>(col / 4, r1) * 4 + col % 4];
-          if (wary && __any_sync(0xffffffffu, odd1(b0) || odd1(b1))) {
-            one_by_one(k * 8, 8, n);
-            continue;
-          }
 #pragma unroll
           for (int i = 0; i < MT; ++i) mma_f32(acc[i][n], ph[i], pl[i], b0, b1);
         }
       }
     }
+    if (!(d.flags & T_END)) bar_arrive<AT_THREADS>(EMPTY + slot);
 
     // ---- the piece ends: the rows, or partials of them
     if (d.flags & T_LAST) {
@@ -662,8 +731,8 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
           x += __shfl_xor_sync(0xffffffffu, x, 2);
           if (t4 == 0) wsum[warp * ROWS + i * 16 + r * 8 + g] = x;
         }
-      __syncthreads();
-      const bool whole = from0 && (d.flags & T_TOEND);
+      bar_sync<AT_CONSUMERS>(INNER);
+      const bool from0 = d.flags & T_FROM0, whole = from0 && (d.flags & T_TOEND);
       float* const part = P.part + ((int64_t)blockIdx.x * 2 + (from0 ? 1 : 0)) * (ROWS * (HD + 2));
 #pragma unroll
       for (int i = 0; i < MT; ++i)
@@ -674,8 +743,9 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
           const float sum = wsum[in_tile] + wsum[ROWS + in_tile] + wsum[2 * ROWS + in_tile] + wsum[3 * ROWS + in_tile];
           if (whole) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
-            char* o = P.out + (int64_t)(d.first + row / P.group) * P.o_tok +
-                      (int64_t)(d.head * P.group + row % P.group) * P.o_head;
+            const int qi = row / P.group;
+            char* o = P.out + (int64_t)(d.first + qi) * P.o_tok +
+                      (int64_t)(d.head * P.group + row - qi * P.group) * P.o_head;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const int col = warp * (HD / 4) + n * 8 + t4 * 2;
@@ -691,26 +761,16 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
             if (warp == 0 && t4 == 0) *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(m[i][r], sum);
           }
         }
-      if (tid == 0 && from0 && !whole) {
-        // the range ends inside this segment: its last unit belongs to CTA `to`
-        const int64_t total = sh[6], ctas = sh[7], end = total * (blockIdx.x + 1) / ctas;
-        const int64_t to = ((end + (sp.units - at)) * ctas - 1) / total;
-        int32_t* meta = P.meta + blockIdx.x * 4;
-        meta[0] = (int32_t)(min(to, ctas - 1) - blockIdx.x + 1);
-        meta[1] = d.b;
-        meta[2] = d.head;
-        meta[3] = d.row0;
-      }
     }
-    if (more) post(tile + NST);
+    if (d.flags & T_END) break;
   }
 }
 
 // Adds up the partials of the segment that starts in CTA blockIdx.x and is cut
 // by its end: one row of it per blockIdx.y.
 template <typename T, int HD, int ROWS>
-__global__ void __launch_bounds__(AT_THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams P) {
-  constexpr int LANES = HD / 4, GROUPS = AT_THREADS / LANES;
+__global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams P) {
+  constexpr int LANES = HD / 4, GROUPS = AT_JOIN_THREADS / LANES;
   __shared__ float weight[kAttnMaxCtas];
   __shared__ float red[2][4];
   __shared__ float4 sums[GROUPS][LANES];
@@ -726,7 +786,7 @@ __global__ void __launch_bounds__(AT_THREADS) paged_attn_join_kernel(const __gri
   // partial i: slot 1 of this CTA, then slot 0 of the ones behind it
   auto part = [&](int i) { return P.part + ((int64_t)(blockIdx.x + i) * 2 + (i == 0)) * (ROWS * (HD + 2)); };
   float m = -INFINITY;
-  for (int i = tid; i < n; i += AT_THREADS) m = fmaxf(m, part(i)[ROWS * HD + r * 2]);
+  for (int i = tid; i < n; i += AT_JOIN_THREADS) m = fmaxf(m, part(i)[ROWS * HD + r * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((tid & 31) == 0) red[0][tid >> 5] = m;
@@ -734,7 +794,7 @@ __global__ void __launch_bounds__(AT_THREADS) paged_attn_join_kernel(const __gri
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  for (int i = tid; i < n; i += AT_THREADS) {
+  for (int i = tid; i < n; i += AT_JOIN_THREADS) {
     const float2 ml = *(const float2*)(part(i) + ROWS * HD + r * 2);
     const float w = ex2(ml.x - base);
     weight[i] = w;
@@ -789,8 +849,7 @@ int pick_mt(const PagedAttnParams& p) {
   return rows <= 16 ? 1 : (rows <= 32 || max_mt<T, HD>() == 2 ? 2 : 4);
 }
 
-// A CTA's worth of positions at most in any segment: no cut can pay, and the
-// unit becomes a whole tile so that none happens and nothing needs joining.
+// One tile at most in any segment: none is cut, and nothing needs joining.
 template <typename T, int HD, int MT>
 bool uncut(const PagedAttnParams& p) {
   int64_t span = (int64_t)p.c.pages_per_seq * p.c.page_size;
@@ -811,7 +870,6 @@ void launch_mt(PagedAttnParams p, cudaStream_t s) {
   const int ctas = device_sm_count() * L::CTAS;
   check(ctas <= kAttnMaxCtas, E_INTERNAL, "more SMs than the attention join holds");
   const bool cut = !uncut<T, HD, MT>(p);
-  p.unit = cut ? 16 : L::TP;
   p.mul = p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f;
   p.cap2 = p.softcap * 1.4426950408889634f;
   p.meta = cut ? (int32_t*)(p.part + (int64_t)ctas * 2 * L::ROWS * (HD + 2)) : nullptr;
@@ -819,7 +877,7 @@ void launch_mt(PagedAttnParams p, cudaStream_t s) {
   launch_k(paged_attn_kernel<T, HD, MT>, dim3(ctas), AT_THREADS, L::SMEM, s, 1, p);
   if (cut) {
     const int rows = (int)std::min<int64_t>((int64_t)p.max_rows * p.group, L::ROWS);
-    launch_k(paged_attn_join_kernel<T, HD, L::ROWS>, dim3(ctas, rows), AT_THREADS, 0, s, 1, p);
+    launch_k(paged_attn_join_kernel<T, HD, L::ROWS>, dim3(ctas, rows), AT_JOIN_THREADS, 0, s, 1, p);
   }
 }
 

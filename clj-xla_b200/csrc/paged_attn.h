@@ -18,14 +18,16 @@
 // paged_attn_join_kernel, launched as a programmatic dependent, adds up in
 // range order: no atomics, the same bits every time.
 //
-// Tile.  64 positions (32 in f32) of K and V rows go through a ring of stages.
-// Warp 4 is the producer: it walks the schedule, looks the pages of a tile up
-// one tile ahead, and gathers the rows with 16-byte cp.async (any page size, any
-// strides; positions nobody sees are filled with zeros and not read).  Warps 0
-// to 3 score 16 (8) positions each on mma.sync, share row maxima and weights
-// through shared memory, and each adds P.V for a quarter of head_dim, so the
-// accumulators stay small and no warp holds partials.  Stages change hands over
-// named barriers.
+// Tile.  64 positions (32 for f32 rows of 256) of K and V rows go through a ring
+// of stages.  The producer warps behind the four consumer warps walk the
+// schedule, look the pages of a tile up one tile ahead, and gather the rows
+// with 16-byte cp.async (any page size, any strides; positions nobody sees are
+// filled with zeros and not read).  Products run on mma.sync with the positions
+// (scores) and the columns (P.V) as its 16 rows and 8 query rows as its columns:
+// a decode step has few query rows, so this wastes the least.  Each consumer
+// warp scores 16 positions, row maxima and weights are shared through shared
+// memory, and each warp adds P.V for its part of head_dim, so the accumulators
+// stay small and no warp holds partials.  Stages change hands over named barriers.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -40,17 +42,16 @@
 namespace cljxla {
 namespace {
 
-constexpr int AT_CONSUMERS = 128, AT_THREADS = AT_CONSUMERS + 32, AT_JOIN_THREADS = 128;
+constexpr int AT_CONSUMERS = 128, AT_JOIN_THREADS = 128;
 constexpr int kAttnMaxCtas = 1024;  // SMs times CTAs on one, at most
 
 // ------------------------------------------------------------------ layout
-template <typename T, int HD, int MT>
+template <typename T, int HD, int NR>
 struct Tile {
   static constexpr int ES = sizeof(T);
-  static constexpr int TP = ES == 2 ? 64 : 32;  // positions of a tile
-  static constexpr int WP = TP / 4;             // positions a warp scores
-  static constexpr int ROWS = MT * 16;
   static constexpr int RB = HD * ES;            // bytes of a row
+  static constexpr int TP = RB > 512 ? 32 : 64; // positions of a tile
+  static constexpr int ROWS = NR * 8;           // query rows
   static constexpr int CPR = RB / 16;           // 16-byte chunks of a row
   static constexpr int KB = TP * RB;
   static constexpr int QB = ROWS * RB;
@@ -58,20 +59,23 @@ struct Tile {
   // weights as two 16-bit parts or one f32: in the tile's K rows once they are scored, if they fit
   static constexpr int PB = ROWS * TP * 4;
   static constexpr bool P_IN_K = PB <= KB;
-  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 64 + TP * 16; }
+  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 64 + 2 * TP * 16; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
     int n = 0;
     while (n < 4 && fixed(n + 1) + (n + 1) * STAGE <= 233472 / ctas - 1024) ++n;
     return n;
   }
   static constexpr int pick() {
-    int ctas = HD >= 256 ? 1 : HD == 128 ? 2 : 3;
+    int ctas = KB > 16384 ? 1 : KB > 8192 ? 2 : 3;
     while (ctas > 1 && fit(ctas) < 3) --ctas;
     return ctas;
   }
   static constexpr int CTAS = pick();
   static constexpr int NST = fit(CTAS);
   static constexpr int SMEM = fixed(NST) + NST * STAGE;
+  // one warp issues the copies of about 3 TB/s over the GPU, so an SM needs two
+  static constexpr int PRODUCERS = CTAS == 1 ? 2 : 1;
+  static constexpr int THREADS = AT_CONSUMERS + 32 * PRODUCERS;
   static_assert(NST >= 2, "a ring needs two stages");
 };
 
@@ -120,9 +124,10 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void ldsm2t(uint32_t addr, uint32_t* r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-               : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+__device__ __forceinline__ void stsm4t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1),
+               "r"(r2), "r"(r3)
+               : "memory");
 }
 template <typename T>
 __device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -145,13 +150,11 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
-__device__ __forceinline__ void mma_f32(float* c, const uint32_t* ah, const uint32_t* al, float b0, float b1) {
-  uint32_t h0, l0, h1, l1;
-  split_tf32(b0, h0, l0);
-  split_tf32(b1, h1, l1);
-  mma_tf32(c, al, h0, h1);
-  mma_tf32(c, ah, l0, l1);
-  mma_tf32(c, ah, h0, h1);
+__device__ __forceinline__ void mma_f32(float* c, const uint32_t* ah, const uint32_t* al, const uint32_t* bh,
+                                        const uint32_t* bl) {
+  mma_tf32(c, al, bh[0], bh[1]);
+  mma_tf32(c, ah, bl[0], bl[1]);
+  mma_tf32(c, ah, bh[0], bh[1]);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -162,6 +165,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&v;
   }
+}
+template <typename T>
+__device__ __forceinline__ T narrow(float x) {
+  if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
 }
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
@@ -218,12 +226,19 @@ struct SeqPlan {
   __device__ __forceinline__ int64_t cost(int nkv) const { return (int64_t)units * nkv * tiles; }
 };
 
-template <typename T, int HD, int MT>
-__global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
+// The positions of tile `d` that query row `in_tile` of it sees: [jlo, jhi].
+__device__ __forceinline__ void row_view(const PagedAttnParams& P, const TileDesc& d, int in_tile, int& jlo, int& jhi) {
+  const int row = d.row0 + in_tile;
+  const int pos = d.p0 + row / P.group;  // the row's own position
+  jhi = row < d.count * P.group ? pos - d.pos0 : -1;
+  jlo = P.window < 0 ? 0 : (int)max((int64_t)pos - P.window - d.pos0, (int64_t)0);
+}
+
+template <typename T, int HD, int NR>
+__global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTAS)
     paged_attn_kernel(const __grid_constant__ PagedAttnParams P) {
-  using L = Tile<T, HD, MT>;
-  constexpr int TP = L::TP, WP = L::WP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST;
-  constexpr int NT = HD / 32;  // 8-column output tiles of a warp
+  using L = Tile<T, HD, NR>;
+  constexpr int TP = L::TP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST, AT_THREADS = L::THREADS;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* const ring = smem;
   unsigned char* const p_own = smem + NST * L::STAGE;
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
   float* const wsum = wmax + 4 * ROWS;
   TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
   int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
-  longlong2* const offs = (longlong2*)(sh + 8);  // [TP] the producer's K and V row offsets
+  longlong2* const offs = (longlong2*)(sh + 8);  // [2][TP] the producers' K and V row offsets
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedView& c = P.c;
@@ -288,11 +303,75 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
     __syncthreads();
   }
 
-  // Stage hand-over: full[s] (producer arrives, consumers wait), empty[s] the other way round.
-  constexpr int FULL = 2, EMPTY = FULL + NST, INNER = 1;
+  // Stage hand-over: full[s] (producers arrive, consumers wait), empty[s] (consumers
+  // arrive, the first producer waits); ahead: the producers among themselves.
+  constexpr int INNER = 1, AHEAD = 2, FULL = 3, EMPTY = FULL + NST;
+  constexpr int EMPTY_THREADS = AT_CONSUMERS + 32;
 
+  constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
+  constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
+  constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
+  const int my_row = lane / LANES, my_chunk = lane % LANES;
+  // a producer's part of a tile's rows
+  auto copy = [&](int tile, int part) {
+    const int slot = tile % NST;
+    const uint32_t kd = smem_u32(ring + slot * L::STAGE), vd = kd + L::KB;
+    const longlong2* const of = offs + (tile & 1) * TP;
+    // eight rows' offsets are fetched before their copies are issued: the warp's
+    // time goes to issue, not to the latency of each row's address
+    constexpr int BATCH = 8, MINE = TP / L::PRODUCERS;
+    static_assert(MINE % (BATCH * RPI) == 0, "whole batches");
+#pragma unroll 1
+    for (int r0 = part * MINE; r0 < (part + 1) * MINE; r0 += BATCH * RPI) {
+      longlong2 o[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) o[i] = of[r0 + i * RPI + my_row];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = r0 + i * RPI + my_row, rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
+        const int size = o[i].x >= 0 ? 16 : 0;
+        const char* kp = (size ? c.k + o[i].x : P.q) + my_chunk * 16;
+        const char* vp = (size ? c.v + o[i].y : P.q) + my_chunk * 16;
+#pragma unroll
+        for (int e = 0; e < CPL; ++e) {
+          const int ch = my_chunk + e * LANES;
+          cp16(kd + r * RB + swz<CPR>(ch, rr) * 16, kp + (size ? e * LANES * 16 : 0), size);
+          cp16(vd + r * RB + swz_v<T, CPR>(ch, rr) * 16, vp + (size ? e * LANES * 16 : 0), size);
+        }
+      }
+    }
+  };
+  // hands over the last tiles in flight: all but the newest `k` are there, and so on
+  auto drain = [&](int tiles, int k) {
+    for (; k >= 0; --k) {
+      if (tiles - 1 - k < 0) continue;
+      if (k == 0) cp_wait<0>();
+      else if (k == 1) cp_wait<1>();
+      else cp_wait<2>();
+      bar_arrive<AT_THREADS>(FULL + (tiles - 1 - k) % NST);
+    }
+  };
+
+  if (L::PRODUCERS > 1 && warp == AT_CONSUMERS / 32 + 1) {
+    // ======================================================== second producer
+    for (int tile = 0;; ++tile) {
+      if (tile >= NST - 1) {
+        cp_wait<NST - 2>();
+        bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
+      }
+      bar_sync<64>(AHEAD);  // the tile's offsets are there and its stage is free, or all is done
+      const int what = *(volatile int*)(sh + 2 + (tile & 1));
+      if (what != 1) {
+        if (what == 2) bar_arrive<AT_THREADS>(FULL);
+        drain(tile, NST - 3);
+        return;
+      }
+      copy(tile, 1);
+      cp_commit();
+    }
+  }
   if (warp == AT_CONSUMERS / 32) {
-    // ================================================================ producer
+    // ========================================================= first producer
     int b = (int)sh[0];  // cursor: sequence, segment of it (head, row tile), tile of that
     SeqPlan sp;
     sp.load(P, b, TP, ROWS);
@@ -366,15 +445,15 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
       return true;
     };
 
-    constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
-    constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
-    constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
-    const int my_row = lane / LANES, my_chunk = lane % LANES;
     int tile = 0;
     bool have = next();
     if (!have) {  // only if lengths change under the kernel: a tile of nothing ends the consumers
       if (lane == 0) *(TileDesc*)desc = TileDesc{0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
       bar_arrive<AT_THREADS>(FULL);
+      if constexpr (L::PRODUCERS > 1) {
+        if (lane == 0) *(volatile int*)(sh + 2) = 2;
+        bar_arrive<64>(AHEAD);
+      }
       return;
     }
     while (have) {
@@ -384,43 +463,24 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
         bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
       }
       const int slot = tile % NST;
-      if (tile >= NST) bar_sync<AT_THREADS>(EMPTY + slot);
-      __syncwarp();  // offs of the tile before are read
+      if (tile >= NST) bar_sync<EMPTY_THREADS>(EMPTY + slot);
 #pragma unroll
       for (int i = 0; i < TP / 32; ++i) {
         const bool ok = (unsigned)page[i] < (unsigned)c.num_pages;
         longlong2 o;
         o.x = ok ? page[i] * c.k_page + nd.head * c.k_head + in_page[i] * c.k_row : -1;
         o.y = ok ? page[i] * c.v_page + nd.head * c.v_head + in_page[i] * c.v_row : -1;
-        offs[i * 32 + lane] = o;
+        offs[(tile & 1) * TP + i * 32 + lane] = o;
         nd.mask[i] = __ballot_sync(0xffffffffu, ok);
       }
       if (lane == 0) *(TileDesc*)((char*)desc + slot * 64) = nd;
-      __syncwarp();
-      const uint32_t kd = smem_u32(ring + slot * L::STAGE), vd = kd + L::KB;
-      // eight rows' offsets are fetched before their copies are issued: the warp's
-      // time goes to issue, not to the latency of each row's address
-      constexpr int BATCH = 8;
-      static_assert(TP % (BATCH * RPI) == 0, "whole batches");
-#pragma unroll 1
-      for (int r0 = 0; r0 < TP; r0 += BATCH * RPI) {
-        longlong2 o[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) o[i] = offs[r0 + i * RPI + my_row];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int r = r0 + i * RPI + my_row, rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
-          const int size = o[i].x >= 0 ? 16 : 0;
-          const char* kp = (size ? c.k + o[i].x : P.q) + my_chunk * 16;
-          const char* vp = (size ? c.v + o[i].y : P.q) + my_chunk * 16;
-#pragma unroll
-          for (int e = 0; e < CPL; ++e) {
-            const int ch = my_chunk + e * LANES;
-            cp16(kd + r * RB + swz<CPR>(ch, rr) * 16, kp + (size ? e * LANES * 16 : 0), size);
-            cp16(vd + r * RB + swz_v<T, CPR>(ch, rr) * 16, vp + (size ? e * LANES * 16 : 0), size);
-          }
-        }
+      if constexpr (L::PRODUCERS > 1) {
+        if (lane == 0) *(volatile int*)(sh + 2 + (tile & 1)) = 1;
+        bar_sync<64>(AHEAD);
+      } else {
+        __syncwarp();
       }
+      copy(tile, 0);
       if (nd.flags & T_FIRST) {
         const uint32_t qd = smem_u32(ring + qslot * L::STAGE + 2 * L::KB);
         for (int r0 = 0; r0 < ROWS; r0 += RPI) {
@@ -442,324 +502,334 @@ __global__ void __launch_bounds__(AT_THREADS, Tile<T, HD, MT>::CTAS)
       if (!have && lane == 0) ((TileDesc*)((char*)desc + slot * 64))->flags |= T_END;
       ++tile;
     }
-    // the tiles still in flight
-#pragma unroll
-    for (int k = NST - 2; k >= 0; --k) {
-      if (tile - 1 - k < 0) continue;
-      if (k == 0) cp_wait<0>();
-      else if (k == 1) cp_wait<1>();
-      else cp_wait<2>();
-      bar_arrive<AT_THREADS>(FULL + (tile - 1 - k) % NST);
+    if constexpr (L::PRODUCERS > 1) {
+      if (lane == 0) *(volatile int*)(sh + 2 + (tile & 1)) = 0;
+      if (tile >= NST - 1) {  // as the second producer does before it looks
+        cp_wait<NST - 2>();
+        bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
+      }
+      bar_arrive<64>(AHEAD);
+      drain(tile, NST - 3);
+    } else {
+      drain(tile, NST - 2);
     }
-    for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<AT_THREADS>(EMPTY + k % NST);  // no arrival is left over
+    for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<EMPTY_THREADS>(EMPTY + k % NST);  // no arrival is left over
     return;
   }
 
   // ================================================================ consumers
-  float acc[MT][NT][4], m[MT][2], l[MT][2];
-  const int g = lane >> 2, t4 = lane & 3;
+  constexpr int SCORERS = TP / 16;                  // warps that score 16 positions each
+  constexpr int CW = HD >= 64 ? HD / 4 : 16;        // columns of P.V of a warp
+  constexpr int MT = CW / 16, ADDERS = HD / CW;     // their 16-column tiles; warps that have some
+  constexpr int PROW = TP * (L::ES == 2 ? 2 : 4);   // bytes of a row of weights
+  constexpr int QK = HD / 32;                       // steps of 32 of head_dim
+  float acc[MT][NR][4], m[NR][2], l[NR][2];
+  uint32_t qf[NR == 1 && L::ES == 2 ? QK : 1][4];   // the queries, where they fit registers
+  const int g = lane >> 2, t4 = lane & 3;           // this thread's positions and columns: g, g + 8; its rows: 2 t4, 2 t4 + 1
   for (int tile = 0;; ++tile) {
     const int slot = tile % NST;
     bar_sync<AT_THREADS>(FULL + slot);
     const TileDesc d = *(const TileDesc*)((char*)desc + slot * 64);
     unsigned char* const stage = ring + slot * L::STAGE;
-    const uint32_t ks = smem_u32(stage), vs = ks + L::KB, qs = smem_u32(ring + d.qslot * L::STAGE + 2 * L::KB);
+    unsigned char* const queries = ring + d.qslot * L::STAGE + 2 * L::KB;
+    const uint32_t ks = smem_u32(stage), vs = ks + L::KB, qs = smem_u32(queries);
     unsigned char* const pw = L::P_IN_K ? stage : p_own;
     const uint64_t vis = TP == 64 ? (uint64_t)d.mask[1] << 32 | d.mask[0] : d.mask[0];
     const bool plain = (d.flags & T_FULL) && vis == (TP == 64 ? ~0ull : 0xffffffffull);
+    // 8 query rows x 32 of head_dim: the second operands of two steps
+    const uint32_t qa = qs + (lane & 7) * RB + swz<CPR>(lane >> 3, lane & 7) * 16;
     if (d.flags & T_FIRST) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        m[i][0] = m[i][1] = -INFINITY;
-        l[i][0] = l[i][1] = 0.f;
+      for (int n = 0; n < NR; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
+        for (int i = 0; i < MT; ++i) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
+      }
+      if constexpr (NR == 1 && L::ES == 2) {
+#pragma unroll
+        for (int j = 0; j < QK; ++j) ldsm4(qa ^ (j * 64), qf[j]);
       }
     }
 
-    // ---- scores of this warp's WP positions
-    constexpr int SN = WP / 8;
-    float s[MT][SN][4];
+    // ---- scores: s[n][e] is of position g + 8 (e / 2) of the warp's 16 and row 8 n + 2 t4 + e % 2
+    float s[NR][4];
+    if (SCORERS == 4 || warp < SCORERS) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      if constexpr (L::ES == 2) {
+        // chunk 2 k + (0 or 1) of a row: its swizzled address differs from chunk
+        // 0 or 1's by an exclusive or with 32 k
+        const int kr = warp * 16 + (lane & 15);
+        const uint32_t ka = ks + kr * RB + swz<CPR>(lane >> 4, kr) * 16;
+        float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one row tile: every other step apart, to halve the chain of dependent products
 #pragma unroll
-      for (int n = 0; n < SN; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
-    if constexpr (L::ES == 2) {
-      // chunk 2 k + (0 or 1) of a row: its swizzled address differs from chunk
-      // 0 or 1's by an exclusive or with 32 k
-      const int kr = warp * WP + (lane >> 4) * 8 + (lane & 7), qr = lane & 15;
-      const uint32_t ka = ks + kr * RB + swz<CPR>((lane >> 3) & 1, kr) * 16;
-      const uint32_t qa = qs + qr * RB + swz<CPR>(lane >> 4, qr) * 16;
-      float s2[SN][4];  // one row tile: even and odd steps apart, to halve the chain of dependent products
-      if constexpr (MT == 1) {
+        for (int j = 0; j < QK; ++j) {
+          uint32_t k0[4], k1[4];
+          ldsm4(ka ^ (j * 64), k0);
+          ldsm4(ka ^ (j * 64 + 32), k1);
 #pragma unroll
-        for (int n = 0; n < SN; ++n) s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        uint32_t kb[4];
-        ldsm4(ka ^ (k * 32), kb);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint32_t a[4];
-          ldsm4((qa ^ (k * 32)) + i * 16 * RB, a);
-          float(*t)[4] = MT == 1 && (k & 1) ? s2 : s[i];
-          mma16<T>(t[0], a, kb[0], kb[1]);
-          mma16<T>(t[SN - 1], a, kb[2], kb[3]);
+          for (int n = 0; n < NR; ++n) {
+            uint32_t q[4];
+            if constexpr (NR == 1) {
+              q[0] = qf[j][0]; q[1] = qf[j][1]; q[2] = qf[j][2]; q[3] = qf[j][3];
+            } else {
+              ldsm4((qa ^ (j * 64)) + n * 8 * RB, q);
+            }
+            mma16<T>(s[n], k0, q[0], q[1]);
+            mma16<T>(NR == 1 ? s2 : s[n], k1, q[2], q[3]);
+          }
         }
-      }
-      if constexpr (MT == 1) {
+        if constexpr (NR == 1) {
 #pragma unroll
-        for (int n = 0; n < SN; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[0][n][e] += s2[n][e];
-      }
-    } else {
-      const int kr = warp * WP + g;
-      const float* kp = (const float*)(stage + kr * RB);
-      const float* qp = (const float*)(ring + d.qslot * L::STAGE + 2 * L::KB);
+          for (int e = 0; e < 4; ++e) s[0][e] += s2[e];
+        }
+      } else {
+        const int kr = warp * 16 + g;  // and kr + 8: the same swizzle
+        const float* const kp = (const float*)(stage + kr * RB);
+        const float* const qp = (const float*)(queries + g * RB);
 #pragma unroll 4
-      for (int k = 0; k < HD / 8; ++k) {
-        const float b0 = kp[swz<CPR>(2 * k, kr) * 4 + t4], b1 = kp[swz<CPR>(2 * k + 1, kr) * 4 + t4];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
+        for (int k = 0; k < HD / 8; ++k) {
+          const int c0 = swz<CPR>(2 * k, g) * 4 + t4, c1 = swz<CPR>(2 * k + 1, g) * 4 + t4;
           uint32_t ah[4], al[4];
+          split_tf32(kp[c0], ah[0], al[0]);
+          split_tf32(kp[c0 + 8 * HD], ah[1], al[1]);
+          split_tf32(kp[c1], ah[2], al[2]);
+          split_tf32(kp[c1 + 8 * HD], ah[3], al[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = i * 16 + g + (e & 1) * 8;
-            split_tf32(qp[r * HD + swz<CPR>(2 * k + (e >> 1), r) * 4 + t4], ah[e], al[e]);
-          }
-          mma_f32(s[i][0], ah, al, b0, b1);
-        }
-      }
-    }
-    // base-2 scores; positions a row does not see: -inf
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int n = 0; n < SN; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = s[i][n][e] * P.mul;
-          if (P.softcap > 0.f) x = P.cap2 * tanh_f(x);
-          s[i][n][e] = x;
-        }
-    int jhi[MT][2], jlo[MT][2];  // positions of this tile each of the thread's rows sees
-    if (!plain) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = d.row0 + i * 16 + g + r * 8;
-          const int q = d.p0 + row / P.group;  // this row's position
-          jhi[i][r] = row < d.count * P.group ? q - d.pos0 : -1;
-          jlo[i][r] = P.window < 0 ? 0 : (int)max((int64_t)q - P.window - d.pos0, (int64_t)0);
-        }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int n = 0; n < SN; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = warp * WP + n * 8 + t4 * 2 + (e & 1);
-            if (!(j <= jhi[i][e >> 1] && j >= jlo[i][e >> 1] && (vis >> j & 1u))) s[i][n][e] = -INFINITY;
-          }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x = fmaxf(s[i][0][2 * r], s[i][0][2 * r + 1]);
-        if (SN > 1) x = fmaxf(x, fmaxf(s[i][SN - 1][2 * r], s[i][SN - 1][2 * r + 1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        if (t4 == 0) wmax[warp * ROWS + i * 16 + r * 8 + g] = x;
-      }
-    bar_sync<AT_CONSUMERS>(INNER);  // maxima are there, and K is read: its rows may take the weights
-
-    float alpha[MT][2];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = i * 16 + r * 8 + g;
-        float x = m[i][r];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) x = fmaxf(x, wmax[w * ROWS + row]);
-        const float base = x == -INFINITY ? 0.f : x;
-        alpha[i][r] = ex2(m[i][r] - base);
-        m[i][r] = x;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < SN; ++n) {
-          const float p0 = ex2(s[i][n][2 * r] - base), p1 = ex2(s[i][n][2 * r + 1] - base);
-          sum += p0 + p1;
-          if constexpr (L::ES == 2) {
-            // hi + lo keep 16 bits (f16: 22) of a weight, so the product with V
-            // is good for an f32 output
-            const uint32_t hi = pack2<T>(p0, p1);
-            const float2 h = unpack2<T>(hi);
-            const uint32_t lo = pack2<T>(p0 - h.x, p1 - h.y);
-            unsigned char* at16 = pw + row * (TP * 2) + (((warp * SN + n) ^ (row & 7)) * 16) + t4 * 4;
-            *(uint32_t*)at16 = hi;
-            *(uint32_t*)(at16 + ROWS * TP * 2) = lo;
-          } else {
-            unsigned char* at32 = pw + row * (TP * 4) + (((warp * 2 + (t4 >> 1)) ^ (row & 7)) * 16) + (t4 & 1) * 8;
-            *(float2*)at32 = make_float2(p0, p1);
+          for (int n = 0; n < NR; ++n) {
+            uint32_t bh[2], bl[2];
+            split_tf32(qp[c0 + n * 8 * HD], bh[0], bl[0]);
+            split_tf32(qp[c1 + n * 8 * HD], bh[1], bl[1]);
+            mma_f32(s[n], ah, al, bh, bl);
           }
         }
-        l[i][r] = l[i][r] * alpha[i][r] + sum;
       }
-    bar_sync<AT_CONSUMERS>(INNER);  // weights are there
-
-    // ---- P.V for this warp's quarter of head_dim
+      // base-2 scores
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        acc[i][n][0] *= alpha[i][0];
-        acc[i][n][1] *= alpha[i][0];
-        acc[i][n][2] *= alpha[i][1];
-        acc[i][n][3] *= alpha[i][1];
+        for (int e = 0; e < 4; ++e) s[n][e] *= P.mul;
+      if (P.softcap > 0.f) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = P.cap2 * tanh_f(s[n][e]);
       }
-    // A position that some rows see and others do not may hold an infinity or
-    // NaN, which a weight of zero does not keep out of a matrix product.  Tiles
-    // with row-dependent masks look for such values first; with one of them in
-    // this warp's columns the products are made one by one, for the rows that
-    // do see the position.
-    bool odd = false;
-    if (!plain && d.count > 1) {
-      constexpr int W = RB / 64;  // 16-byte chunks of a row in a quarter of it
-#pragma unroll 1
-      for (int i = lane; i < TP * W; i += 32) {
-        const int j = i / W;
-        const uint4 v = *(const uint4*)(stage + L::KB + j * RB + swz_v<T, CPR>(warp * W + i % W, j) * 16);
-        odd = odd || odd_chunk<T>(v);
-      }
-      odd = __any_sync(0xffffffffu, odd);
-    }
-    if (odd) {
-#pragma unroll 1
-      for (int j = 0; j < TP; ++j) {
-        if (!(vis >> j & 1u)) continue;
-        float p[MT][2];
+      if (!plain) {  // positions a row does not see: -inf
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int row = i * 16 + r * 8 + g;
-            if constexpr (L::ES == 2) {
-              const unsigned char* at16 = pw + row * (TP * 2) + (((j >> 3) ^ (row & 7)) * 16) + (j & 7) * 2;
-              p[i][r] = (float)*(const T*)at16 + (float)*(const T*)(at16 + ROWS * TP * 2);
-            } else {
-              p[i][r] = *(const float*)(pw + row * (TP * 4) + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4);
+            int jlo, jhi;
+            row_view(P, d, n * 8 + 2 * t4 + r, jlo, jhi);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int j = warp * 16 + g + h * 8;
+              if (j < jlo || j > jhi || !(vis >> j & 1u)) s[n][h * 2 + r] = -INFINITY;
             }
           }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = warp * (HD / 4) + n * 8 + t4 * 2 + e;
-            constexpr int PC = 16 / L::ES;  // elements of a chunk
-            const float v = (float)((const T*)(stage + L::KB + j * RB + swz_v<T, CPR>(col / PC, j) * 16))[col % PC];
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-                if (j <= jhi[i][r] && j >= jlo[i][r]) acc[i][n][2 * r + e] += p[i][r] * v;
-          }
       }
-    } else if constexpr (L::ES == 2) {
-      const int pr = lane & 15;
-      const uint32_t pa = smem_u32(pw) + pr * (TP * 2) + (((lane >> 4) ^ (pr & 7)) * 16);
-      const uint32_t va = vs + pr * RB + swz_v<T, CPR>(warp * NT + (NT > 1 ? lane >> 4 : 0), pr) * 16;
 #pragma unroll
-      for (int k = 0; k < TP / 16; ++k) {
-        uint32_t ph[MT][4], pl[MT][4];
+      for (int n = 0; n < NR; ++n) {
+        float2 x = make_float2(fmaxf(s[n][0], s[n][2]), fmaxf(s[n][1], s[n][3]));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          ldsm4((pa ^ (k * 32)) + i * 16 * TP * 2, ph[i]);
-          ldsm4((pa ^ (k * 32)) + (ROWS + i * 16) * TP * 2, pl[i]);
+        for (int o = 4; o < 32; o <<= 1) {
+          x.x = fmaxf(x.x, __shfl_xor_sync(0xffffffffu, x.x, o));
+          x.y = fmaxf(x.y, __shfl_xor_sync(0xffffffffu, x.y, o));
         }
-#pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-          uint32_t vb[4];
-          if constexpr (NT == 1) ldsm2t(va + k * 16 * RB, vb);
-          else ldsm4t((va ^ (n * 16)) + k * 16 * RB, vb);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            mma16<T>(acc[i][n], ph[i], vb[0], vb[1]);
-            if constexpr (NT > 1) mma16<T>(acc[i][n + 1], ph[i], vb[2], vb[3]);
-            mma16<T>(acc[i][n], pl[i], vb[0], vb[1]);
-            if constexpr (NT > 1) mma16<T>(acc[i][n + 1], pl[i], vb[2], vb[3]);
-          }
-        }
+        if (g == 0) *(float2*)(wmax + warp * ROWS + n * 8 + 2 * t4) = x;
       }
-    } else {
+    }
+    bar_sync<AT_CONSUMERS>(INNER);  // maxima are there, and K is read: its rows may take the weights
+
+    float alpha[NR][2];
 #pragma unroll
-      for (int k = 0; k < TP / 8; ++k) {
-        uint32_t ph[MT][4], pl[MT][4];
+    for (int n = 0; n < NR; ++n) {
+      float2 x = make_float2(m[n][0], m[n][1]);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+      for (int w = 0; w < SCORERS; ++w) {
+        const float2 y = *(const float2*)(wmax + w * ROWS + n * 8 + 2 * t4);
+        x.x = fmaxf(x.x, y.x);
+        x.y = fmaxf(x.y, y.y);
+      }
+      const float b0 = x.x == -INFINITY ? 0.f : x.x, b1 = x.y == -INFINITY ? 0.f : x.y;
+      alpha[n][0] = ex2(m[n][0] - b0);
+      alpha[n][1] = ex2(m[n][1] - b1);
+      m[n][0] = x.x;
+      m[n][1] = x.y;
+      if (SCORERS == 4 || warp < SCORERS) {
+        const float p0 = ex2(s[n][0] - b0), p1 = ex2(s[n][1] - b1), p2 = ex2(s[n][2] - b0), p3 = ex2(s[n][3] - b1);
+        l[n][0] = l[n][0] * alpha[n][0] + (p0 + p2);
+        l[n][1] = l[n][1] * alpha[n][1] + (p1 + p3);
+        if constexpr (L::ES == 2) {
+          // hi + lo keep 16 bits (f16: 22) of a weight, so the product with V is
+          // good for an f32 output
+          const uint32_t h0 = pack2<T>(p0, p1), h1 = pack2<T>(p2, p3);
+          const float2 f0 = unpack2<T>(h0), f1 = unpack2<T>(h1);
+          const int row = n * 8 + (lane & 7), ch = warp * 2 + (lane >> 3 & 1);
+          stsm4t(smem_u32(pw) + (lane >> 4) * (ROWS * PROW) + row * PROW + ((ch ^ (row & 7)) * 16), h0, h1,
+                 pack2<T>(p0 - f0.x, p1 - f0.y), pack2<T>(p2 - f1.x, p3 - f1.y));
+        } else {
+          const float p[4] = {p0, p1, p2, p3};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int r = i * 16 + g + (e & 1) * 8;
-            split_tf32(*(const float*)(pw + r * (TP * 4) + (((2 * k + (e >> 1)) ^ (r & 7)) * 16) + t4 * 4), ph[i][e], pl[i][e]);
+            const int row = n * 8 + 2 * t4 + (e & 1), j = warp * 16 + g + (e >> 1) * 8;
+            *(float*)(pw + row * PROW + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4) = p[e];
           }
-        const int r0 = k * 8 + t4, r1 = r0 + 4;
-        const float* v0p = (const float*)(stage + L::KB + r0 * RB);
-        const float* v1p = (const float*)(stage + L::KB + r1 * RB);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int col = warp * (HD / 4) + n * 8 + g;
-          const float b0 = v0p[swz_v<T, CPR>(col / 4, r0) * 4 + col % 4], b1 = v1p[swz_v<T, CPR>(col / 4, r1) * 4 + col % 4];
-#pragma unroll
-          for (int i = 0; i < MT; ++i) mma_f32(acc[i][n], ph[i], pl[i], b0, b1);
         }
       }
     }
-    if (!(d.flags & T_END)) bar_arrive<AT_THREADS>(EMPTY + slot);
+    bar_sync<AT_CONSUMERS>(INNER);  // weights are there
+
+    // ---- P.V: acc[i][n][e] is of column g + 8 (e / 2) of the warp's i-th 16 and row 8 n + 2 t4 + e % 2
+    if (ADDERS == 4 || warp < ADDERS) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][n][e] *= alpha[n][e & 1];
+      // A position that some rows see and others do not may hold an infinity or
+      // NaN, which a weight of zero does not keep out of a matrix product.  Tiles
+      // with row-dependent masks look for such values first; with one of them in
+      // this warp's columns the products are made one by one, for the rows that
+      // do see the position.
+      bool odd = false;
+      if (!plain && d.count > 1) {
+        constexpr int W = CW * L::ES / 16;  // 16-byte chunks of a row that are this warp's
+#pragma unroll 1
+        for (int i = lane; i < TP * W; i += 32) {
+          const int j = i / W;
+          const uint4 v = *(const uint4*)(stage + L::KB + j * RB + swz_v<T, CPR>(warp * W + i % W, j) * 16);
+          odd = odd || odd_chunk<T>(v);
+        }
+        odd = __any_sync(0xffffffffu, odd);
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int j = 0; j < TP; ++j) {
+          if (!(vis >> j & 1u)) continue;
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int row = n * 8 + 2 * t4 + r;
+              int jlo, jhi;
+              row_view(P, d, row, jlo, jhi);
+              if (j < jlo || j > jhi) continue;
+              float p;
+              if constexpr (L::ES == 2) {
+                const unsigned char* at16 = pw + row * PROW + (((j >> 3) ^ (row & 7)) * 16) + (j & 7) * 2;
+                p = (float)*(const T*)at16 + (float)*(const T*)(at16 + ROWS * PROW);
+              } else {
+                p = *(const float*)(pw + row * PROW + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4);
+              }
+#pragma unroll
+              for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  constexpr int PC = 16 / L::ES;  // elements of a chunk
+                  const int col = warp * CW + i * 16 + g + h * 8;
+                  acc[i][n][h * 2 + r] +=
+                      p * (float)((const T*)(stage + L::KB + j * RB + swz_v<T, CPR>(col / PC, j) * 16))[col % PC];
+                }
+            }
+        }
+      } else if constexpr (L::ES == 2) {
+        const uint32_t pa = smem_u32(pw) + (lane & 7) * PROW + (((lane >> 3) ^ (lane & 7)) * 16);
+        const int vr = (lane >> 4) * 8 + (lane & 7);
+        const uint32_t va = vs + vr * RB + swz_v<T, CPR>(warp * (CW / 8) + (lane >> 3 & 1), vr) * 16;
+#pragma unroll
+        for (int j = 0; j < TP / 32; ++j) {
+          uint32_t ph[NR][4], pl[NR][4];
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            ldsm4((pa ^ (j * 64)) + n * 8 * PROW, ph[n]);
+            ldsm4((pa ^ (j * 64)) + (ROWS + n * 8) * PROW, pl[n]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              uint32_t v[4];
+              ldsm4t((va ^ (i * 32)) + (j * 32 + h * 16) * RB, v);
+#pragma unroll
+              for (int n = 0; n < NR; ++n) mma16<T>(acc[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
+#pragma unroll
+              for (int n = 0; n < NR; ++n) mma16<T>(acc[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
+            }
+        }
+      } else {
+#pragma unroll 2
+        for (int k = 0; k < TP / 8; ++k) {
+          uint32_t bh[NR][2], bl[NR][2];
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              split_tf32(*(const float*)(pw + (n * 8 + g) * PROW + (((2 * k + h) ^ g) * 16) + t4 * 4), bh[n][h], bl[n][h]);
+          const int r0 = k * 8 + t4;  // and r0 + 4: the same swizzle
+          const float* const vp = (const float*)(stage + L::KB + r0 * RB);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const int col = warp * CW + i * 16 + g;
+            const int c0 = swz_v<T, CPR>(col / 4, r0) * 4 + col % 4, c1 = swz_v<T, CPR>(col / 4 + 2, r0) * 4 + col % 4;
+            uint32_t ah[4], al[4];
+            split_tf32(vp[c0], ah[0], al[0]);
+            split_tf32(vp[c1], ah[1], al[1]);
+            split_tf32(vp[c0 + 4 * HD], ah[2], al[2]);
+            split_tf32(vp[c1 + 4 * HD], ah[3], al[3]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) mma_f32(acc[i][n], ah, al, bh[n], bl[n]);
+          }
+        }
+      }
+    }
+    if (!(d.flags & T_END)) bar_arrive<EMPTY_THREADS>(EMPTY + slot);
 
     // ---- the piece ends: the rows, or partials of them
     if (d.flags & T_LAST) {
+      if (SCORERS == 4 || warp < SCORERS) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+        for (int n = 0; n < NR; ++n) {
+          float2 x = make_float2(l[n][0], l[n][1]);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float x = l[i][r];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          if (t4 == 0) wsum[warp * ROWS + i * 16 + r * 8 + g] = x;
+          for (int o = 4; o < 32; o <<= 1) {
+            x.x += __shfl_xor_sync(0xffffffffu, x.x, o);
+            x.y += __shfl_xor_sync(0xffffffffu, x.y, o);
+          }
+          if (g == 0) *(float2*)(wsum + warp * ROWS + n * 8 + 2 * t4) = x;
         }
+      }
       bar_sync<AT_CONSUMERS>(INNER);
       const bool from0 = d.flags & T_FROM0, whole = from0 && (d.flags & T_TOEND);
       float* const part = P.part + ((int64_t)blockIdx.x * 2 + (from0 ? 1 : 0)) * (ROWS * (HD + 2));
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int in_tile = i * 16 + r * 8 + g, row = d.row0 + in_tile;
+          const int in_tile = n * 8 + 2 * t4 + r, row = d.row0 + in_tile;
           if (row >= d.count * P.group) continue;
-          const float sum = wsum[in_tile] + wsum[ROWS + in_tile] + wsum[2 * ROWS + in_tile] + wsum[3 * ROWS + in_tile];
-          if (whole) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
-            const int qi = row / P.group;
-            char* o = P.out + (int64_t)(d.first + qi) * P.o_tok +
-                      (int64_t)(d.head * P.group + row - qi * P.group) * P.o_head;
+          float sum = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const int col = warp * (HD / 4) + n * 8 + t4 * 2;
-              const float x = acc[i][n][2 * r] * inv, y = acc[i][n][2 * r + 1] * inv;
-              if (L::ES == 4 || P.out_f32) *(float2*)(o + col * 4) = make_float2(x, y);
-              else if constexpr (L::ES == 2) *(uint32_t*)(o + col * 2) = pack2<T>(x, y);
+          for (int w = 0; w < SCORERS; ++w) sum += wsum[w * ROWS + in_tile];
+          if (warp == 0 && g == 0 && !whole) *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(m[n][r], sum);
+          if (ADDERS < 4 && warp >= ADDERS) continue;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
+          const int qi = row / P.group;
+          char* const o = P.out + (int64_t)(d.first + qi) * P.o_tok +
+                          (int64_t)(d.head * P.group + row - qi * P.group) * P.o_head;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int col = warp * CW + i * 16 + g + h * 8;
+              const float x = acc[i][n][h * 2 + r];
+              if (!whole) part[in_tile * HD + col] = x;
+              else if (L::ES == 4 || P.out_f32) ((float*)o)[col] = x * inv;
+              else if constexpr (L::ES == 2) ((T*)o)[col] = narrow<T>(x * inv);
             }
-          } else {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              *(float2*)(part + in_tile * HD + warp * (HD / 4) + n * 8 + t4 * 2) =
-                  make_float2(acc[i][n][2 * r], acc[i][n][2 * r + 1]);
-            if (warp == 0 && t4 == 0) *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(m[i][r], sum);
-          }
         }
     }
     if (d.flags & T_END) break;
@@ -836,45 +906,45 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
 }
 
 // ------------------------------------------------------------------- host
-// Row tiles of 16, 32 or 64 rows: the smallest that holds a sequence's rows for
-// one KV head (more rows than 64 take several tiles, each reading K and V
+// Row tiles of 8, 16, 32 or 64 rows: the smallest that holds a sequence's rows
+// for one KV head (more rows than 64 take several tiles, each reading K and V
 // again, from L2).  f32 rows of 256 stop at 32: two stages of more do not fit.
 template <typename T, int HD>
-constexpr int max_mt() {
-  return sizeof(T) == 4 && HD == 256 ? 2 : 4;
+constexpr int max_nr() {
+  return sizeof(T) == 4 && HD == 256 ? 4 : 8;
 }
 template <typename T, int HD>
-int pick_mt(const PagedAttnParams& p) {
+int pick_nr(const PagedAttnParams& p) {
   const int64_t rows = (int64_t)p.max_rows * p.group;
-  return rows <= 16 ? 1 : (rows <= 32 || max_mt<T, HD>() == 2 ? 2 : 4);
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 || max_nr<T, HD>() == 4 ? 4 : 8;
 }
 
 // One tile at most in any segment: none is cut, and nothing needs joining.
-template <typename T, int HD, int MT>
+template <typename T, int HD, int NR>
 bool uncut(const PagedAttnParams& p) {
   int64_t span = (int64_t)p.c.pages_per_seq * p.c.page_size;
   if (p.window >= 0) span = std::min(span, p.window + p.max_rows);
-  return span <= Tile<T, HD, MT>::TP;
+  return span <= Tile<T, HD, NR>::TP;
 }
 
-template <typename T, int HD, int MT>
-int64_t workspace_mt(const PagedAttnParams& p) {
-  if (uncut<T, HD, MT>(p)) return 0;
-  const int64_t ctas = (int64_t)device_sm_count() * Tile<T, HD, MT>::CTAS;
-  return ctas * (2 * MT * 16 * (HD + 2) * 4 + 16);
+template <typename T, int HD, int NR>
+int64_t workspace_nr(const PagedAttnParams& p) {
+  if (uncut<T, HD, NR>(p)) return 0;
+  const int64_t ctas = (int64_t)device_sm_count() * Tile<T, HD, NR>::CTAS;
+  return ctas * (2 * NR * 8 * (HD + 2) * 4 + 16);
 }
 
-template <typename T, int HD, int MT>
-void launch_mt(PagedAttnParams p, cudaStream_t s) {
-  using L = Tile<T, HD, MT>;
+template <typename T, int HD, int NR>
+void launch_nr(PagedAttnParams p, cudaStream_t s) {
+  using L = Tile<T, HD, NR>;
   const int ctas = device_sm_count() * L::CTAS;
   check(ctas <= kAttnMaxCtas, E_INTERNAL, "more SMs than the attention join holds");
-  const bool cut = !uncut<T, HD, MT>(p);
+  const bool cut = !uncut<T, HD, NR>(p);
   p.mul = p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f;
   p.cap2 = p.softcap * 1.4426950408889634f;
   p.meta = cut ? (int32_t*)(p.part + (int64_t)ctas * 2 * L::ROWS * (HD + 2)) : nullptr;
-  ensure_smem_optin((const void*)paged_attn_kernel<T, HD, MT>, L::SMEM);
-  launch_k(paged_attn_kernel<T, HD, MT>, dim3(ctas), AT_THREADS, L::SMEM, s, 1, p);
+  ensure_smem_optin((const void*)paged_attn_kernel<T, HD, NR>, L::SMEM);
+  launch_k(paged_attn_kernel<T, HD, NR>, dim3(ctas), L::THREADS, L::SMEM, s, 1, p);
   if (cut) {
     const int rows = (int)std::min<int64_t>((int64_t)p.max_rows * p.group, L::ROWS);
     launch_k(paged_attn_join_kernel<T, HD, L::ROWS>, dim3(ctas, rows), AT_JOIN_THREADS, 0, s, 1, p);
@@ -882,30 +952,31 @@ void launch_mt(PagedAttnParams p, cudaStream_t s) {
 }
 
 template <typename T, int HD, class F>
-auto with_mt(const PagedAttnParams& p, F f) {
-  switch (pick_mt<T, HD>(p)) {
+auto with_nr(const PagedAttnParams& p, F f) {
+  switch (pick_nr<T, HD>(p)) {
     case 1: return f(std::integral_constant<int, 1>());
     case 2: return f(std::integral_constant<int, 2>());
-    default: return f(std::integral_constant<int, max_mt<T, HD>()>());
+    case 4: return f(std::integral_constant<int, 4>());
+    default: return f(std::integral_constant<int, max_nr<T, HD>()>());
   }
 }
 template <typename T, class F>
 auto with_hd(const PagedAttnParams& p, F f) {
   switch (p.hd) {
-    case 32: return with_mt<T, 32>(p, [&](auto mt) { return f(std::integral_constant<int, 32>(), mt); });
-    case 64: return with_mt<T, 64>(p, [&](auto mt) { return f(std::integral_constant<int, 64>(), mt); });
-    case 128: return with_mt<T, 128>(p, [&](auto mt) { return f(std::integral_constant<int, 128>(), mt); });
-    default: return with_mt<T, 256>(p, [&](auto mt) { return f(std::integral_constant<int, 256>(), mt); });
+    case 32: return with_nr<T, 32>(p, [&](auto nr) { return f(std::integral_constant<int, 32>(), nr); });
+    case 64: return with_nr<T, 64>(p, [&](auto nr) { return f(std::integral_constant<int, 64>(), nr); });
+    case 128: return with_nr<T, 128>(p, [&](auto nr) { return f(std::integral_constant<int, 128>(), nr); });
+    default: return with_nr<T, 256>(p, [&](auto nr) { return f(std::integral_constant<int, 256>(), nr); });
   }
 }
 
 template <typename T>
 int64_t attention_workspace_of(const PagedAttnParams& p) {
-  return with_hd<T>(p, [&](auto hd, auto mt) { return workspace_mt<T, decltype(hd)::value, decltype(mt)::value>(p); });
+  return with_hd<T>(p, [&](auto hd, auto nr) { return workspace_nr<T, decltype(hd)::value, decltype(nr)::value>(p); });
 }
 template <typename T>
 void launch_attention_of(const PagedAttnParams& p, cudaStream_t s) {
-  with_hd<T>(p, [&](auto hd, auto mt) { launch_mt<T, decltype(hd)::value, decltype(mt)::value>(p, s); });
+  with_hd<T>(p, [&](auto hd, auto nr) { launch_nr<T, decltype(hd)::value, decltype(nr)::value>(p, s); });
 }
 
 }  // namespace

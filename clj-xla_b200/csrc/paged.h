@@ -17,7 +17,8 @@ struct PagedView {
   const int32_t* lens;
   const int32_t* starts;  // null: `each` rows per sequence
   int64_t table_stride;   // entries
-  int32_t num_pages, page_size, pages_per_seq, nkv, num_seqs, tokens, each, pad_;
+  int32_t num_pages, page_size, pages_per_seq, nkv, num_seqs, tokens, each;
+  int32_t page_shift;  // log2(page_size), or -1
 };
 
 struct PagedAppendParams {
@@ -42,7 +43,7 @@ struct PagedAttnParams {
   // of tanh), log2(e) * softcap
   float mul, cap2;
   float* part;    // per CTA: two slots of rows and their (max, sum)
-  int32_t* meta;  // per CTA: CTAs that share the segment starting there (0: none), sequence, head, first row
+  int32_t* meta;  // 8 per CTA: CTAs that share the segment starting there (0: none), head, row tile, first row, rows
 };
 
 struct VerifyParams {

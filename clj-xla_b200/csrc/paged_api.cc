@@ -117,6 +117,9 @@ PagedView view_of(const CLJXLA_PagedKV* kv, int64_t tokens, const int32_t* start
   c.num_pages = (int32_t)kv->num_pages;
   c.page_size = (int32_t)kv->page_size;
   c.pages_per_seq = (int32_t)kv->pages_per_seq;
+  c.page_shift = -1;
+  for (int i = 0; i <= 30; ++i)
+    if (kv->page_size == (int64_t)1 << i) c.page_shift = i;
   c.nkv = (int32_t)kv->kv_heads;
   c.num_seqs = (int32_t)kv->num_seqs;
   c.tokens = (int32_t)tokens;

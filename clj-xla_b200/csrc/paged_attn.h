@@ -19,10 +19,11 @@
 // range order: no atomics, the same bits every time.
 //
 // Tile.  64 positions (32 for f32 rows of 256) of K and V rows go through a ring
-// of stages.  The producer warps behind the four consumer warps walk the
-// schedule, look the pages of a tile up one tile ahead, and gather the rows
-// with 16-byte cp.async (any page size, any strides; positions nobody sees are
-// filled with zeros and not read).  Products run on mma.sync with the positions
+// of stages.  Behind the four consumer warps, a scheduler warp walks the
+// schedule and looks the pages of a tile up one tile ahead, and two copier
+// warps (one warp issues copies for about 3 TB/s over the GPU) gather its K and
+// V rows with 16-byte cp.async (any page size, any strides; positions nobody
+// sees are filled with zeros and not read).  Products run on mma.sync with the positions
 // (scores) and the columns (P.V) as its 16 rows and 8 query rows as its columns:
 // a decode step has few query rows, so this wastes the least.  Each consumer
 // warp scores 16 positions, row maxima and weights are shared through shared
@@ -59,23 +60,21 @@ struct Tile {
   // weights as two 16-bit parts or one f32: in the tile's K rows once they are scored, if they fit
   static constexpr int PB = ROWS * TP * 4;
   static constexpr bool P_IN_K = PB <= KB;
-  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 64 + 2 * TP * 16; }
+  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 64 + 4 * TP * 8; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
     int n = 0;
     while (n < 4 && fixed(n + 1) + (n + 1) * STAGE <= 233472 / ctas - 1024) ++n;
     return n;
   }
   static constexpr int pick() {
-    int ctas = KB > 16384 ? 1 : KB > 8192 ? 2 : 3;
+    int ctas = KB > 16384 ? 1 : 2;
     while (ctas > 1 && fit(ctas) < 3) --ctas;
     return ctas;
   }
   static constexpr int CTAS = pick();
   static constexpr int NST = fit(CTAS);
   static constexpr int SMEM = fixed(NST) + NST * STAGE;
-  // one warp issues the copies of about 3 TB/s over the GPU, so an SM needs two
-  static constexpr int PRODUCERS = CTAS == 1 ? 2 : 1;
-  static constexpr int THREADS = AT_CONSUMERS + 32 * PRODUCERS;
+  static constexpr int THREADS = AT_CONSUMERS + 96;  // and a scheduler, a copier of K and one of V
   static_assert(NST >= 2, "a ring needs two stages");
 };
 
@@ -246,7 +245,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   float* const wsum = wmax + 4 * ROWS;
   TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
   int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
-  longlong2* const offs = (longlong2*)(sh + 8);  // [2][TP] the producers' K and V row offsets
+  const char** const rows = (const char**)(sh + 8);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedView& c = P.c;
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     }
     ctas = min((int64_t)gridDim.x, total);
     if ((int64_t)blockIdx.x >= ctas) {
-      if (tid == 0 && P.meta) P.meta[blockIdx.x * 4] = 0;
+      if (tid == 0 && P.meta) P.meta[blockIdx.x * 8] = 0;
       return;
     }
     const int64_t beg = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
@@ -285,7 +284,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     __syncthreads();
     if (tid == 0) {
       sh[0] = sh[1] = 0;
-      if (P.meta) P.meta[blockIdx.x * 4] = 0;  // no segment that starts here is cut, so far
+      if (P.meta) P.meta[blockIdx.x * 8] = 0;  // no segment that starts here is cut, so far
     }
     __syncthreads();
     int64_t excl = incl - mine;
@@ -304,74 +303,84 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   }
 
   // Stage hand-over: full[s] (producers arrive, consumers wait), empty[s] (consumers
-  // arrive, the first producer waits); ahead: the producers among themselves.
+  // arrive, the scheduler waits); ahead: the producers among themselves.
   constexpr int INNER = 1, AHEAD = 2, FULL = 3, EMPTY = FULL + NST;
-  constexpr int EMPTY_THREADS = AT_CONSUMERS + 32;
-
+  constexpr int EMPTY_THREADS = AT_CONSUMERS + 32, AHEAD_THREADS = 96;
   constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
   constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
   constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
   const int my_row = lane / LANES, my_chunk = lane % LANES;
-  // a producer's part of a tile's rows
-  auto copy = [&](int tile, int part) {
-    const int slot = tile % NST;
-    const uint32_t kd = smem_u32(ring + slot * L::STAGE), vd = kd + L::KB;
-    const longlong2* const of = offs + (tile & 1) * TP;
-    // eight rows' offsets are fetched before their copies are issued: the warp's
-    // time goes to issue, not to the latency of each row's address
-    constexpr int BATCH = 8, MINE = TP / L::PRODUCERS;
-    static_assert(MINE % (BATCH * RPI) == 0, "whole batches");
-#pragma unroll 1
-    for (int r0 = part * MINE; r0 < (part + 1) * MINE; r0 += BATCH * RPI) {
-      longlong2 o[BATCH];
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) o[i] = of[r0 + i * RPI + my_row];
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int r = r0 + i * RPI + my_row, rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
-        const int size = o[i].x >= 0 ? 16 : 0;
-        const char* kp = (size ? c.k + o[i].x : P.q) + my_chunk * 16;
-        const char* vp = (size ? c.v + o[i].y : P.q) + my_chunk * 16;
-#pragma unroll
-        for (int e = 0; e < CPL; ++e) {
-          const int ch = my_chunk + e * LANES;
-          cp16(kd + r * RB + swz<CPR>(ch, rr) * 16, kp + (size ? e * LANES * 16 : 0), size);
-          cp16(vd + r * RB + swz_v<T, CPR>(ch, rr) * 16, vp + (size ? e * LANES * 16 : 0), size);
-        }
-      }
+  volatile int* const plan = (volatile int*)(sh + 2);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
+  constexpr int ALL_THERE = 256, DONE = -1, BROKEN = -2;
+  // Producers: before the next tile's stage is waited for, the oldest tile in
+  // flight is handed to the consumers.
+  auto hand_over = [&](int tile) {
+    if (tile >= NST - 1) {
+      cp_wait<NST - 2>();
+      bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
     }
   };
-  // hands over the last tiles in flight: all but the newest `k` are there, and so on
-  auto drain = [&](int tiles, int k) {
-    for (; k >= 0; --k) {
+  auto drain = [&](int tiles) {  // what is left of that after `tiles` tiles
+    for (int k = NST - 3; k >= 0; --k) {
       if (tiles - 1 - k < 0) continue;
       if (k == 0) cp_wait<0>();
-      else if (k == 1) cp_wait<1>();
-      else cp_wait<2>();
+      else cp_wait<1>();
       bar_arrive<AT_THREADS>(FULL + (tiles - 1 - k) % NST);
     }
   };
 
-  if (L::PRODUCERS > 1 && warp == AT_CONSUMERS / 32 + 1) {
-    // ======================================================== second producer
+  if (warp > AT_CONSUMERS / 32) {
+    // ================================================== copiers: K rows, V rows
+    const bool is_v = warp == AT_CONSUMERS / 32 + 2;
     for (int tile = 0;; ++tile) {
-      if (tile >= NST - 1) {
-        cp_wait<NST - 2>();
-        bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
-      }
-      bar_sync<64>(AHEAD);  // the tile's offsets are there and its stage is free, or all is done
-      const int what = *(volatile int*)(sh + 2 + (tile & 1));
-      if (what != 1) {
-        if (what == 2) bar_arrive<AT_THREADS>(FULL);
-        drain(tile, NST - 3);
+      hand_over(tile);
+      bar_sync<AHEAD_THREADS>(AHEAD);  // the tile's rows are listed and its stage is free, or all is done
+      const int what = plan[tile & 1];
+      if (what < 0) {
+        if (what == BROKEN) bar_arrive<AT_THREADS>(FULL);
+        drain(tile);
         return;
       }
-      copy(tile, 1);
+      const uint32_t dst = smem_u32(ring + (tile % NST) * L::STAGE) + (is_v ? L::KB : 0);
+      const char* const* const of = rows + ((tile & 1) * 2 + is_v) * TP;
+      // eight rows' addresses are fetched before their copies are issued: the
+      // warp's time goes to issue, not to the latency of each row's address
+      constexpr int BATCH = 8;
+      static_assert(TP % (BATCH * RPI) == 0, "whole batches");
+      auto copy = [&](auto all, auto swizzle) {
+        const int n = what & 255;
+#pragma unroll 1
+        for (int r0 = 0; r0 < n; r0 += BATCH * RPI) {
+          const char* o[BATCH];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) o[i] = of[r0 + i * RPI + my_row];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
+            const bool ok = decltype(all)::value || o[i] != nullptr;
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) {
+              const int ch = my_chunk + e * LANES;
+              cp16(dst + (r0 + rr) * RB + swizzle(ch, rr) * 16, ok ? o[i] + ch * 16 : P.q, ok ? 16 : 0);
+            }
+          }
+        }
+      };
+      auto k_swz = [](int ch, int r) { return swz<CPR>(ch, r); };
+      auto v_swz = [](int ch, int r) { return swz_v<T, CPR>(ch, r); };
+      if constexpr (L::ES == 2) {  // the same for both
+        if (what & ALL_THERE) copy(std::true_type(), k_swz);
+        else copy(std::false_type(), k_swz);
+      } else if (is_v) {
+        copy(std::false_type(), v_swz);
+      } else {
+        copy(std::false_type(), k_swz);
+      }
       cp_commit();
     }
   }
   if (warp == AT_CONSUMERS / 32) {
-    // ========================================================= first producer
+    // =============================================================== scheduler
     int b = (int)sh[0];  // cursor: sequence, segment of it (head, row tile), tile of that
     SeqPlan sp;
     sp.load(P, b, TP, ROWS);
@@ -420,11 +429,10 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
           // the range ends inside a segment that starts here: its last tile belongs to CTA `to`
           const int64_t end = total * (blockIdx.x + 1) / ctas;
           const int64_t to = ((end + (sp.units - at)) * ctas - 1) / total;
-          int32_t* meta = P.meta + blockIdx.x * 4;
-          meta[0] = (int32_t)(min(to, ctas - 1) - blockIdx.x + 1);
-          meta[1] = b;
-          meta[2] = nd.head;
-          meta[3] = nd.row0;
+          const int n = (int)(min(to, ctas - 1) - blockIdx.x + 1);
+          int4* const meta = (int4*)(P.meta + blockIdx.x * 8);
+          meta[0] = make_int4(n, nd.head, nd.row0, nd.first);
+          meta[1] = make_int4(nd.count * P.group, 0, 0, 0);
         }
       }
       // every row sees every position, were all pages there
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         page[i] = -1;
         in_page[i] = 0;
         if (i * 32 + lane < nd.npos) {
-          const int slot = j / c.page_size;
+          const int slot = c.page_shift >= 0 ? j >> c.page_shift : j / c.page_size;
           page[i] = c.table[(int64_t)b * c.table_stride + slot];
           in_page[i] = j - slot * c.page_size;
         }
@@ -448,39 +456,34 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     int tile = 0;
     bool have = next();
     if (!have) {  // only if lengths change under the kernel: a tile of nothing ends the consumers
-      if (lane == 0) *(TileDesc*)desc = TileDesc{0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
-      bar_arrive<AT_THREADS>(FULL);
-      if constexpr (L::PRODUCERS > 1) {
-        if (lane == 0) *(volatile int*)(sh + 2) = 2;
-        bar_arrive<64>(AHEAD);
+      if (lane == 0) {
+        *(TileDesc*)desc = TileDesc{0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
+        plan[0] = BROKEN;
       }
+      bar_arrive<AT_THREADS>(FULL);
+      bar_arrive<AHEAD_THREADS>(AHEAD);
       return;
     }
     while (have) {
-      // tell the consumers of the oldest tile in flight before waiting for a free stage
-      if (tile >= NST - 1) {
-        cp_wait<NST - 2>();
-        bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
-      }
+      hand_over(tile);
       const int slot = tile % NST;
-      if (tile >= NST) bar_sync<EMPTY_THREADS>(EMPTY + slot);
+      bool all = true;
 #pragma unroll
       for (int i = 0; i < TP / 32; ++i) {
         const bool ok = (unsigned)page[i] < (unsigned)c.num_pages;
-        longlong2 o;
-        o.x = ok ? page[i] * c.k_page + nd.head * c.k_head + in_page[i] * c.k_row : -1;
-        o.y = ok ? page[i] * c.v_page + nd.head * c.v_head + in_page[i] * c.v_row : -1;
-        offs[(tile & 1) * TP + i * 32 + lane] = o;
+        const char** const to = rows + (tile & 1) * 2 * TP + i * 32 + lane;
+        to[0] = ok ? c.k + page[i] * c.k_page + nd.head * c.k_head + in_page[i] * c.k_row : nullptr;
+        to[TP] = ok ? c.v + page[i] * c.v_page + nd.head * c.v_head + in_page[i] * c.v_row : nullptr;
         nd.mask[i] = __ballot_sync(0xffffffffu, ok);
+        all = all && nd.mask[i] == 0xffffffffu;
       }
-      if (lane == 0) *(TileDesc*)((char*)desc + slot * 64) = nd;
-      if constexpr (L::PRODUCERS > 1) {
-        if (lane == 0) *(volatile int*)(sh + 2 + (tile & 1)) = 1;
-        bar_sync<64>(AHEAD);
-      } else {
-        __syncwarp();
+      if (tile >= NST) bar_sync<EMPTY_THREADS>(EMPTY + slot);
+      if (lane == 0) {
+        *(TileDesc*)((char*)desc + slot * 64) = nd;
+        // whole halves of 32 rows: what the consumers look at
+        plan[tile & 1] = all ? TP | ALL_THERE : min((nd.npos + 31) & ~31, TP);
       }
-      copy(tile, 0);
+      bar_sync<AHEAD_THREADS>(AHEAD);
       if (nd.flags & T_FIRST) {
         const uint32_t qd = smem_u32(ring + qslot * L::STAGE + 2 * L::KB);
         for (int r0 = 0; r0 < ROWS; r0 += RPI) {
@@ -502,17 +505,10 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       if (!have && lane == 0) ((TileDesc*)((char*)desc + slot * 64))->flags |= T_END;
       ++tile;
     }
-    if constexpr (L::PRODUCERS > 1) {
-      if (lane == 0) *(volatile int*)(sh + 2 + (tile & 1)) = 0;
-      if (tile >= NST - 1) {  // as the second producer does before it looks
-        cp_wait<NST - 2>();
-        bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
-      }
-      bar_arrive<64>(AHEAD);
-      drain(tile, NST - 3);
-    } else {
-      drain(tile, NST - 2);
-    }
+    if (lane == 0) plan[tile & 1] = DONE;
+    hand_over(tile);
+    bar_arrive<AHEAD_THREADS>(AHEAD);
+    drain(tile);
     for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<EMPTY_THREADS>(EMPTY + k % NST);  // no arrival is left over
     return;
   }
@@ -557,7 +553,9 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     if (SCORERS == 4 || warp < SCORERS) {
 #pragma unroll
       for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      if constexpr (L::ES == 2) {
+      if (warp * 16 >= d.npos) {
+        // nothing of the tile reaches this warp's positions: all are masked below
+      } else if constexpr (L::ES == 2) {
         // chunk 2 k + (0 or 1) of a row: its swizzled address differs from chunk
         // 0 or 1's by an exclusive or with 32 k
         const int kr = warp * 16 + (lane & 15);
@@ -699,7 +697,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       if (!plain && d.count > 1) {
         constexpr int W = CW * L::ES / 16;  // 16-byte chunks of a row that are this warp's
 #pragma unroll 1
-        for (int i = lane; i < TP * W; i += 32) {
+        for (int i = lane; i < d.npos * W; i += 32) {
           const int j = i / W;
           const uint4 v = *(const uint4*)(stage + L::KB + j * RB + swz_v<T, CPR>(warp * W + i % W, j) * 16);
           odd = odd || odd_chunk<T>(v);
@@ -742,6 +740,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         const uint32_t va = vs + vr * RB + swz_v<T, CPR>(warp * (CW / 8) + (lane >> 3 & 1), vr) * 16;
 #pragma unroll
         for (int j = 0; j < TP / 32; ++j) {
+          if (j * 32 >= d.npos) break;  // rows from here on were not copied
           uint32_t ph[NR][4], pl[NR][4];
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
@@ -762,7 +761,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         }
       } else {
 #pragma unroll 2
-        for (int k = 0; k < TP / 8; ++k) {
+        for (int k = 0; k * 8 < d.npos; ++k) {
           uint32_t bh[NR][2], bl[NR][2];
 #pragma unroll
           for (int n = 0; n < NR; ++n)
@@ -837,54 +836,51 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
 }
 
 // Adds up the partials of the segment that starts in CTA blockIdx.x and is cut
-// by its end: one row of it per blockIdx.y.
+// by its end: one row of it per blockIdx.y.  Two round trips to memory: what to
+// add, then statistics and values together (the first PRE partials of a group of
+// lanes are fetched before their weights are known).
 template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams P) {
-  constexpr int LANES = HD / 4, GROUPS = AT_JOIN_THREADS / LANES;
-  __shared__ float weight[kAttnMaxCtas];
-  __shared__ float red[2][4];
+  constexpr int LANES = HD / 4, GROUPS = AT_JOIN_THREADS / LANES, PRE = 4;
+  __shared__ float2 stat[kAttnMaxCtas];
   __shared__ float4 sums[GROUPS][LANES];
   pdl_enter();
-  const int tid = threadIdx.x, r = blockIdx.y;
-  const int32_t* meta = P.meta + blockIdx.x * 4;
-  const int n = min(meta[0], (int)(gridDim.x - blockIdx.x));
-  if (n < 1) return;
-  int first, count;
-  seq_rows(P.c, meta[1], first, count);
-  const int row = meta[3] + r;
-  if (row >= min(count, P.max_rows) * P.group) return;
+  const int tid = threadIdx.x, r = blockIdx.y, lane = tid % LANES, grp = tid / LANES;
+  const int4* const meta = (const int4*)(P.meta + blockIdx.x * 8);
+  const int4 what = meta[0];
+  const int rows = meta[1].x;
+  const int n = min(what.x, (int)(gridDim.x - blockIdx.x)), row = what.z + r;
+  if (n < 1 || row >= rows) return;
   // partial i: slot 1 of this CTA, then slot 0 of the ones behind it
   auto part = [&](int i) { return P.part + ((int64_t)(blockIdx.x + i) * 2 + (i == 0)) * (ROWS * (HD + 2)); };
-  float m = -INFINITY;
-  for (int i = tid; i < n; i += AT_JOIN_THREADS) m = fmaxf(m, part(i)[ROWS * HD + r * 2]);
+  float4 pre[PRE];
+#pragma unroll
+  for (int k = 0; k < PRE; ++k)
+    if (grp + k * GROUPS < n) pre[k] = *(const float4*)(part(grp + k * GROUPS) + r * HD + lane * 4);
+  for (int i = tid; i < n; i += AT_JOIN_THREADS) stat[i] = *(const float2*)(part(i) + ROWS * HD + r * 2);
+  __syncthreads();
+  // every group of 32 lanes finds the same maximum and sum
+  float m = -INFINITY, l = 0.f;
+  for (int i = tid & 31; i < n; i += 32) m = fmaxf(m, stat[i].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((tid & 31) == 0) red[0][tid >> 5] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int i = tid; i < n; i += AT_JOIN_THREADS) {
-    const float2 ml = *(const float2*)(part(i) + ROWS * HD + r * 2);
-    const float w = ex2(ml.x - base);
-    weight[i] = w;
-    l += w * ml.y;
-  }
+  for (int i = tid & 31; i < n; i += 32) l += ex2(stat[i].x - base) * stat[i].y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if ((tid & 31) == 0) red[1][tid >> 5] = l;
-  __syncthreads();
-  l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  const int lane = tid % LANES, grp = tid / LANES;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = grp; i < n; i += GROUPS) {
-    const float4 v = *(const float4*)(part(i) + r * HD + lane * 4);
-    const float w = weight[i];
+  auto add = [&](int i, const float4& v) {
+    const float w = ex2(stat[i].x - base);
     a.x += w * v.x;
     a.y += w * v.y;
     a.z += w * v.z;
     a.w += w * v.w;
-  }
+  };
+#pragma unroll
+  for (int k = 0; k < PRE; ++k)
+    if (grp + k * GROUPS < n) add(grp + k * GROUPS, pre[k]);
+#pragma unroll 4
+  for (int i = grp + PRE * GROUPS; i < n; i += GROUPS) add(i, *(const float4*)(part(i) + r * HD + lane * 4));
   sums[grp][lane] = a;
   __syncthreads();
   if (grp) return;
@@ -897,7 +893,8 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
     a.w += v.w;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* o = P.out + (int64_t)(first + row / P.group) * P.o_tok + (int64_t)(meta[2] * P.group + row % P.group) * P.o_head;
+  const int qi = row / P.group;
+  char* o = P.out + (int64_t)(what.w + qi) * P.o_tok + (int64_t)(what.y * P.group + row - qi * P.group) * P.o_head;
   if (sizeof(T) == 4 || P.out_f32) {
     ((float4*)o)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   } else if constexpr (sizeof(T) == 2) {
@@ -931,7 +928,7 @@ template <typename T, int HD, int NR>
 int64_t workspace_nr(const PagedAttnParams& p) {
   if (uncut<T, HD, NR>(p)) return 0;
   const int64_t ctas = (int64_t)device_sm_count() * Tile<T, HD, NR>::CTAS;
-  return ctas * (2 * NR * 8 * (HD + 2) * 4 + 16);
+  return ctas * (2 * NR * 8 * (HD + 2) * 4 + 32);
 }
 
 template <typename T, int HD, int NR>

@@ -28,6 +28,7 @@ struct PagedAppendParams {
   int64_t ks_tok, ks_head, vs_tok, vs_head, qs_tok, qs_head, qo_tok, qo_head;  // bytes
   const float* inv_freq;
   int32_t nq, hd, rotary, interleaved, vec, dt;  // vec: whole 16-byte vectors
+  int32_t tok, lot_bits;  // set at the launch: rows of a CTA, log2 of the threads of a head
   float rope_scale;
 };
 

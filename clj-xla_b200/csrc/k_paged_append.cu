@@ -59,7 +59,7 @@ __device__ __forceinline__ void turn_pair(float x, float y, float cs, float sn, 
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendParams P) {
+__global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const __grid_constant__ PagedAppendParams P) {
   constexpr int V = Lot<T, VEC>::V;
   __shared__ int s_pos[PA_TOK];
   __shared__ char *s_k[PA_TOK], *s_v[PA_TOK];  // where the row goes; null: its page is not there
@@ -68,7 +68,34 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   const PagedView& c = P.c;
   const int tid = threadIdx.x, warp = tid >> 5, half = P.rotary / 2;
   const int t0 = blockIdx.x * P.tok, n = min(P.tok, c.tokens - t0);
+  // a head's lots: pairs of lots (interleaved: lots of pairs; by elements: pairs), then lots that are copied
+  const bool whole = P.interleaved && VEC;  // a lot holds both elements of its pairs
+  const int turning = whole ? P.rotary / V : half / V, lots = turning + (P.hd - P.rotary) / V;
+  const int lot = tid & ((1 << P.lot_bits) - 1), lane0 = tid >> P.lot_bits, lanes = PA_THREADS >> P.lot_bits;
+  const int heads = P.nq + c.nkv, step = lanes * gridDim.y;
+  const bool turn = lot < turning;
+  const int e1 = !turn ? P.rotary + (lot - turning) * V : whole ? lot * V : P.interleaved ? 2 * lot : lot * V;
+  const int e2 = P.interleaved ? 2 * lot + 1 : half + lot * V;
+  const bool two = turn && !whole;
+  const int angle = whole ? lot * (V / 2) : lot * V;
   pdl_enter();
+  // The next head of the CTA's rows: their loads are in flight together, the
+  // first ones while the rows' pages and angles are found.
+  Lot<T, VEC> a[PA_TOK], b[PA_TOK];
+  int h = blockIdx.y * lanes + lane0;
+  auto fetch = [&]() {
+    if (lot >= lots || h >= heads) return;
+    const bool is_q = h < P.nq;
+    const char* const src = is_q ? P.qs + t0 * P.qs_tok + h * P.qs_head : P.ks + t0 * P.ks_tok + (h - P.nq) * P.ks_head;
+    const int64_t src_tok = is_q ? P.qs_tok : P.ks_tok;
+#pragma unroll
+    for (int k = 0; k < PA_TOK; ++k) {
+      if (k >= n) break;
+      a[k].load((const T*)(src + k * src_tok) + e1);
+      if (two) b[k].load((const T*)(src + k * src_tok) + e2);
+    }
+  };
+  fetch();
   if (warp < n) {
     const int t = t0 + warp, b = seq_of_row(c.starts, c.num_seqs, c.each, t);
     int pos = 0, page = -1;
@@ -97,57 +124,34 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   }
   __syncthreads();
 
-  // a head's lots: pairs of lots (interleaved: lots of pairs; by elements: pairs), then lots that are copied
-  const bool whole = P.interleaved && VEC;  // a lot holds both elements of its pairs
-  const int turning = whole ? P.rotary / V : half / V, lots = turning + (P.hd - P.rotary) / V;
-  const int lot = tid & ((1 << P.lot_bits) - 1), lane0 = tid >> P.lot_bits, lanes = PA_THREADS >> P.lot_bits;
-  const int heads = P.nq + c.nkv, step = lanes * gridDim.y;
-  const bool turn = lot < turning;
-  const int e1 = !turn ? P.rotary + (lot - turning) * V : whole ? lot * V : P.interleaved ? 2 * lot : lot * V;
-  const int e2 = P.interleaved ? 2 * lot + 1 : half + lot * V;
-  const bool two = turn && !whole;
-  const int angle = whole ? lot * (V / 2) : lot * V;
-  if (lot < lots) {
-    for (int h = blockIdx.y * lanes + lane0; h < heads; h += step) {
-      const bool is_q = h < P.nq;
-      const char* const src = is_q ? P.qs + t0 * P.qs_tok + h * P.qs_head : P.ks + t0 * P.ks_tok + (h - P.nq) * P.ks_head;
-      const int64_t src_tok = is_q ? P.qs_tok : P.ks_tok;
-      // a head of PA_TOK rows at a time: their loads are in flight together
-      Lot<T, VEC> a[PA_TOK], b[PA_TOK];
-      T* dst[PA_TOK];
+  for (; lot < lots && h < heads;) {
+    const bool is_q = h < P.nq;
 #pragma unroll
-      for (int k = 0; k < PA_TOK; ++k) {
-        dst[k] = nullptr;
-        if (k < n && s_live[k]) dst[k] = (T*)(is_q ? P.qo + (t0 + k) * P.qo_tok + h * P.qo_head
-                                                   : s_k[k] ? s_k[k] + (h - P.nq) * c.k_head : nullptr);
-        if (!dst[k]) continue;
-        a[k].load((const T*)(src + k * src_tok) + e1);
-        if (two) b[k].load((const T*)(src + k * src_tok) + e2);
-      }
+    for (int k = 0; k < PA_TOK; ++k) {
+      if (k >= n || !s_live[k] || (!is_q && !s_k[k])) continue;
+      T* const dst = (T*)(is_q ? P.qo + (t0 + k) * P.qo_tok + h * P.qo_head : s_k[k] + (h - P.nq) * c.k_head);
+      if (two) {
 #pragma unroll
-      for (int k = 0; k < PA_TOK; ++k) {
-        if (!dst[k]) continue;
-        if (two) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float x, y;
-            turn_pair(a[k].get(i), b[k].get(i), s_cos[k * 128 + angle + i], s_sin[k * 128 + angle + i], x, y);
-            a[k].set(i, x);
-            b[k].set(i, y);
-          }
-          b[k].store(dst[k] + e2);
-        } else if (turn) {
-#pragma unroll
-          for (int i = 0; i + 1 < V; i += 2) {
-            float x, y;
-            turn_pair(a[k].get(i), a[k].get(i + 1), s_cos[k * 128 + angle + i / 2], s_sin[k * 128 + angle + i / 2], x, y);
-            a[k].set(i, x);
-            a[k].set(i + 1, y);
-          }
+        for (int i = 0; i < V; ++i) {
+          float x, y;
+          turn_pair(a[k].get(i), b[k].get(i), s_cos[k * 128 + angle + i], s_sin[k * 128 + angle + i], x, y);
+          a[k].set(i, x);
+          b[k].set(i, y);
         }
-        a[k].store(dst[k] + e1);
+        b[k].store(dst + e2);
+      } else if (turn) {
+#pragma unroll
+        for (int i = 0; i + 1 < V; i += 2) {
+          float x, y;
+          turn_pair(a[k].get(i), a[k].get(i + 1), s_cos[k * 128 + angle + i / 2], s_sin[k * 128 + angle + i / 2], x, y);
+          a[k].set(i, x);
+          a[k].set(i + 1, y);
+        }
       }
+      a[k].store(dst + e1);
     }
+    h += step;
+    fetch();
   }
   const int vlots = P.hd / V, all = c.nkv * vlots;
   for (int i = blockIdx.y * PA_THREADS + tid; i < all; i += PA_THREADS * gridDim.y) {

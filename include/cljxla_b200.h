@@ -162,7 +162,7 @@ CLJXLA_EXPORT int cljxla_b200_attention_decode_static(const void* q, const void*
  * included, so row starts[b] + i is position seq_lens[b] - count + i.  Position
  * j lives in row j % page_size of page page_table[b][j / page_size], for every
  * KV head.  Rows at or behind starts[num_seqs] belong to nobody: nothing is
- * read from or written to them, so a captured graph may carry padding.
+ * written for them, so a captured graph may carry padding.
  *
  * Every pointer below is a device pointer unless it says otherwise.  starts,
  * seq_lens and page_table are read by the kernels when they run, so a captured

@@ -30,7 +30,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int VD_THREADS = 256;
+constexpr int VD_THREADS = 256, VD_PICK_THREADS = 512;
 constexpr int VD_MAX_ROWS = 128;    // of a sequence
 constexpr int VD_MAX_SPLITS = 32;   // slices of a row: a warp joins them
 constexpr int VD_CLUSTER = 8;
@@ -64,17 +64,20 @@ __device__ __forceinline__ void vd_unpack(const uint4& v, float* x) {
   }
 }
 
-// Statistics of a set of logits: maximum, sum of 2^((x - max) c), and the lowest
-// index of the maximum.  Of nothing, or of -inf alone: (-inf, 0, -1).  A NaN
-// is no maximum and makes the sum one.
+// Statistics of a set of logits: the maximum m, the sum of 2^(x c - R) with the
+// reference R = m c as it rounds (the same R wherever m is the same, so its
+// rounding cancels in every quotient and one FMA gives each exponent), and the
+// lowest index of the maximum.  Of nothing, or of -inf alone: (-inf, 0, -1).  A
+// NaN is no maximum and makes the sum one.
 struct Stat {
   float m, s;
   int i;
 };
+__device__ __forceinline__ float vd_ref(float m, float c) { return m == -INFINITY ? 0.f : __fmul_rn(m, c); }
 __device__ __forceinline__ void vd_join(Stat& a, const Stat& b, float c) {
-  const float M = fmaxf(a.m, b.m), base = M == -INFINITY ? 0.f : M;
+  const float M = fmaxf(a.m, b.m), R = vd_ref(M, c);
   if (b.i >= 0 && (a.i < 0 || b.m > a.m || (b.m == a.m && b.i < a.i))) a.i = b.i;
-  a.s = a.s * vd_ex2((a.m - base) * c) + b.s * vd_ex2((b.m - base) * c);
+  a.s = a.s * vd_ex2(vd_ref(a.m, c) - R) + b.s * vd_ex2(vd_ref(b.m, c) - R);  // an empty part has sum 0
   a.m = M;
 }
 __device__ __forceinline__ void vd_join_warp(Stat& a, float c) {
@@ -85,6 +88,22 @@ __device__ __forceinline__ void vd_join_warp(Stat& a, float c) {
     b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
     b.i = __shfl_xor_sync(0xffffffffu, a.i, o);
     vd_join(a, b, c);
+  }
+}
+
+// the largest of a 16-byte vector's values (NaN aside)
+template <typename T>
+__device__ __forceinline__ float vd_top(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 t = __hmax2(__hmax2(*(const __half2*)&v.x, *(const __half2*)&v.y),
+                              __hmax2(*(const __half2*)&v.z, *(const __half2*)&v.w));
+    return __half2float(__hmax(__low2half(t), __high2half(t)));
+  } else {
+    const __nv_bfloat162 t = __hmax2(__hmax2(*(const __nv_bfloat162*)&v.x, *(const __nv_bfloat162*)&v.y),
+                                     __hmax2(*(const __nv_bfloat162*)&v.z, *(const __nv_bfloat162*)&v.w));
+    return __bfloat162float(__hmax(__low2bfloat16(t), __high2bfloat16(t)));
   }
 }
 
@@ -113,50 +132,60 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
   constexpr int V = 16 / sizeof(T), U = 4;
   pdl_enter();
   const int split = blockIdx.y, row = blockIdx.x, which = blockIdx.z, tid = threadIdx.x;
+  const T* const x = (const T*)((which ? P.draft : P.target) + row * (which ? P.draft_stride : P.target_stride));
+  const float c = (which ? P.inv_td : P.inv_t) * kLog2e;
+  // elements in front of the first 16-byte boundary, whole vectors, and the rest
+  const int64_t head = min((int64_t)((16 - ((uintptr_t)x & 15)) & 15) / (int64_t)sizeof(T), P.vocab);
+  const int64_t vecs = (P.vocab - head) / V;
+  const int64_t lo = vecs * split / P.splits, hi = vecs * (split + 1) / P.splits;
+  const uint4* const xv = (const uint4*)(x + head);
+  // U vectors ahead of the ones in work, the first while the row's sequence is looked up
+  uint4 ahead[U];
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at + u * VD_THREADS < hi) ahead[u] = xv[at + u * VD_THREADS];
+  };
+  fetch(lo + tid);
   const int b = seq_of_row(P.starts, P.num_seqs, P.each, row);
   if (b < 0) return;
   int first, count;
   vd_rows(P, b, first, count);
   if (row - first >= count - which) return;  // not looked at; the draft of a sequence's last row is none
-  const T* const x = (const T*)((which ? P.draft : P.target) + row * (which ? P.draft_stride : P.target_stride));
-  const float c = (which ? P.inv_td : P.inv_t) * kLog2e;
   Stat a{-INFINITY, 0.f, -1};
   auto take = [&](float f, int64_t v) {
     Stat one{f, f == -INFINITY ? 0.f : f == f ? 1.f : f, f > -INFINITY ? (int)v : -1};
     if (!(f == f)) one.m = -INFINITY;
     vd_join(a, one, c);
   };
-  // elements in front of the first 16-byte boundary, whole vectors, and the rest
-  const int64_t head = min((int64_t)((16 - ((uintptr_t)x & 15)) & 15) / (int64_t)sizeof(T), P.vocab);
-  const int64_t vecs = (P.vocab - head) / V;
   if (split == 0 && tid < head) take(vd_f(x[tid]), tid);
-  const int64_t lo = vecs * split / P.splits, hi = vecs * (split + 1) / P.splits;
-  const uint4* const xv = (const uint4*)(x + head);
+  float ref = vd_ref(a.m, c);
   for (int64_t at = lo + tid; at < hi; at += U * VD_THREADS) {
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (at + u * VD_THREADS < hi) raw[u] = xv[at + u * VD_THREADS];
+    for (int u = 0; u < U; ++u) raw[u] = ahead[u];
+    fetch(at + U * VD_THREADS);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (at + u * VD_THREADS >= hi) break;
+      const float top = vd_top<T>(raw[u]);
       float f[V];
       vd_unpack<T>(raw[u], f);
-      float top = f[0];
-#pragma unroll
-      for (int i = 1; i < V; ++i) top = fmaxf(top, f[i]);
       if (top > a.m) {
         if (GREEDY) {  // later vectors have higher indices: the first of the larger values stays
 #pragma unroll
           for (int i = V - 1; i >= 0; --i)
             if (f[i] == top) a.i = (int)(head + (at + u * VD_THREADS) * V + i);
         }
-        a.s *= vd_ex2((a.m - top) * c);
+        const float R = __fmul_rn(top, c);
+        a.s *= vd_ex2(ref - R);
         a.m = top;
+        ref = R;
       }
-      const float base = a.m == -INFINITY ? 0.f : a.m;
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) a.s += vd_ex2((f[i] - base) * c);
+      for (int i = 0; i < V; ++i) sum += vd_ex2(fmaf(f[i], c, -ref));
+      a.s += sum;
     }
   }
   if (split == P.splits - 1 && tid < P.vocab - head - vecs * V) take(vd_f(x[head + vecs * V + tid]), head + vecs * V + tid);
@@ -172,40 +201,66 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
   if (GREEDY) vd_index(P, row)[split] = a.i;
 }
 
-// a token with a positive weight: the larger key, or the lower index of equal ones
+// The race's best so far: the larger w / e, compared by cross products (a
+// reciprocal per token would cost a third of the exponentials again), or the
+// lower index of equal ones.  Nothing yet: (0, 1, -1).
 struct Best {
-  float key;
+  float w, e;
   int i;
 };
 __device__ __forceinline__ void vd_best(Best& a, const Best& b) {
-  if (b.i >= 0 && (a.i < 0 || b.key > a.key || (b.key == a.key && b.i < a.i))) a = b;
+  const float x = b.w * a.e, y = a.w * b.e;
+  if (b.i >= 0 && (a.i < 0 || x > y || (x == y && b.i < a.i))) a = b;
 }
 __device__ __forceinline__ void vd_best_warp(Best& a) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Best b;
-    b.key = __shfl_xor_sync(0xffffffffu, a.key, o);
+    b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
+    b.e = __shfl_xor_sync(0xffffffffu, a.e, o);
     b.i = __shfl_xor_sync(0xffffffffu, a.i, o);
     vd_best(a, b);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_constant__ VerifyParams P) {
-  constexpr int V = 4;  // elements a thread takes at a time
+__global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const __grid_constant__ VerifyParams P) {
+  constexpr int THREADS = VD_PICK_THREADS, WARPS = THREADS / 32;
+  constexpr int V = 16 / sizeof(T);  // elements a thread takes at a time
   __shared__ float s_max[2][VD_MAX_ROWS], s_sum[2][VD_MAX_ROWS];
   __shared__ int s_arg[VD_MAX_ROWS], s_taken;
-  __shared__ Best s_best[2][VD_THREADS / 32], s_mine[2];
+  __shared__ Best s_best[WARPS], s_mine[2];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t lots = (P.vocab + V - 1) / V, lo = lots * rank / ctas, hi = lots * (rank + 1) / ctas;
+  if (!P.greedy) {  // whatever row decides, this CTA's part of e is needed: into L2 while the rows are read
+    const char* const e = (const char*)(P.race + b * P.race_stride + lo * V);
+    const int64_t bytes = (min(hi * V, P.vocab) - lo * V) * 4;
+    for (int64_t at = tid * 128; at < bytes; at += THREADS * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(e + at));
+  }
   pdl_enter();
   int first, count;
   vd_rows(P, b, first, count);
   if (tid == 0) s_taken = max(count - 1, 0);
   const float c = P.inv_t * kLog2e, cd = P.inv_td * kLog2e;
+  auto target = [&](int r) { return (const T*)(P.target + (first + r) * P.target_stride); };
+  auto draft = [&](int r) { return (const T*)(P.draft + (first + r) * P.draft_stride); };
+  // thread r's draft, with its logits and random number: on their way while the slices are joined
+  int x = -1;
+  bool valid = false;
+  float lx = 0.f, dx = 0.f, ux = 0.f;
+  if (tid < count - 1) {
+    x = P.tokens_in[first + tid + 1];
+    valid = x >= 0 && x < P.vocab;
+    if (valid) {
+      lx = vd_f(target(tid)[x]);
+      if (P.draft) dx = vd_f(draft(tid)[x]);
+    }
+    if (!P.greedy) ux = P.uniform[first + tid];
+  }
   // the rows' slices, joined
-  for (int i = warp; i < 2 * count; i += VD_THREADS / 32) {
+  for (int i = warp; i < 2 * count; i += WARPS) {
     const int which = i >= count, r = which ? i - count : i;
     if (which && (!P.draft || r == count - 1)) continue;
     Stat a{-INFINITY, 0.f, -1};
@@ -223,18 +278,15 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
     }
   }
   __syncthreads();
-  auto target = [&](int r) { return (const T*)(P.target + (first + r) * P.target_stride); };
-  auto draft = [&](int r) { return (const T*)(P.draft + (first + r) * P.draft_stride); };
-  auto logp = [&](int r, int x) { return (vd_f(target(r)[x]) - s_max[0][r]) * P.inv_t - logf(s_sum[0][r]); };
+  auto logp = [&](float l, int r) { return (fmaf(l, c, -vd_ref(s_max[0][r], c)) - log2f(s_sum[0][r])) * 0.6931471805599453f; };
   if (tid < count - 1) {
-    const int x = P.tokens_in[first + tid + 1];
-    bool good = x >= 0 && x < P.vocab;
+    bool good = valid;
     if (good && P.greedy) good = x == s_arg[tid];
     if (good && !P.greedy) {
       // in logarithms: both sides may lie far below the smallest float
       float lq = 0.f;
-      if (P.draft) lq = (vd_f(draft(tid)[x]) - s_max[1][tid]) * P.inv_td - logf(s_sum[1][tid]);
-      good = logf(P.uniform[first + tid]) + lq < logp(tid, x);
+      if (P.draft) lq = fmaf(dx, cd, -vd_ref(s_max[1][tid], cd)) - log2f(s_sum[1][tid]);
+      good = log2f(ux) + lq < fmaf(lx, c, -vd_ref(s_max[0][tid], c)) - log2f(s_sum[0][tid]);
     }
     if (!good) atomicMin(&s_taken, tid);
   }
@@ -243,89 +295,88 @@ __global__ void __launch_bounds__(VD_THREADS) verify_pick_kernel(const __grid_co
   int token = -1;
   if (P.greedy) {
     if (count > 0) token = s_arg[taken];
-  } else {
-    if (count > 0) {
-      const bool rejected = taken < count - 1, residual = rejected && P.draft;
-      const int out = rejected && !P.draft ? P.tokens_in[first + taken + 1] : -1;
-      const T *const l = target(taken), *const d = residual ? draft(taken) : l;
-      const float* const e = P.race + b * P.race_stride;
-      const float m = s_max[0][taken], inv = 1.f / s_sum[0][taken];
-      const float md = s_max[1][taken], invd = 1.f / s_sum[1][taken];
-      Best best[2] = {{0.f, -1}, {0.f, -1}};  // of w, and of p for where w is nothing
+  } else if (count > 0) {
+    const bool rejected = taken < count - 1;
+    bool residual = rejected && P.draft;
+    int out = rejected && !P.draft ? P.tokens_in[first + taken + 1] : -1;
+    const T* const l = target(taken);
+    const T* const d = residual ? draft(taken) : l;
+    const float* const e = P.race + b * P.race_stride;
+    const float ref = vd_ref(s_max[0][taken], c), inv = 1.f / s_sum[0][taken];
+    const float refd = residual ? vd_ref(s_max[1][taken], cd) : 0.f, invd = residual ? 1.f / s_sum[1][taken] : 0.f;
+    const bool aligned = (((uintptr_t)e | (uintptr_t)l | (uintptr_t)d) & 15) == 0;
+    // the race for w; once more for p in the rare case that w is nothing
+    for (int pass = 0; pass < 2 && token < 0; ++pass) {
+      Best best{0.f, 1.f, -1};
       auto race = [&](float lv, float dv, float ev, int64_t v) {
-        const float p = vd_ex2((lv - m) * c) * inv;
-        const float w = residual ? p - vd_ex2((dv - md) * cd) * invd : v == out ? 0.f : p;
-        if (w > 0.f) vd_best(best[0], {w / ev, (int)v});
-        else if (best[0].i < 0 && p > 0.f) vd_best(best[1], {p / ev, (int)v});
+        float w = vd_ex2(fmaf(lv, c, -ref)) * inv;
+        if (residual) w -= vd_ex2(fmaf(dv, cd, -refd)) * invd;
+        if (w * best.e > best.w * ev && (int)v != out) best = {w, ev, (int)v};  // a thread's indices ascend
       };
-      const bool aligned = (((uintptr_t)e | (uintptr_t)l * (4 / sizeof(T)) | (uintptr_t)d * (4 / sizeof(T))) & 15) == 0;
-      const int64_t lots = (P.vocab + V - 1) / V, lo = lots * rank / ctas, hi = lots * (rank + 1) / ctas;
-#pragma unroll 2
-      for (int64_t at = lo + tid; at < hi; at += VD_THREADS) {
-        const int64_t v = at * V;
-        float lv[V], dv[V], ev[V];
-        if (aligned && v + V <= P.vocab) {
-          const float4 f = *(const float4*)(e + v);
-          ev[0] = f.x; ev[1] = f.y; ev[2] = f.z; ev[3] = f.w;
-          if constexpr (sizeof(T) == 4) {
-            vd_unpack<T>(*(const uint4*)(l + v), lv);
-            if (residual) vd_unpack<T>(*(const uint4*)(d + v), dv);
-          } else {
-            float t[8];
-            const uint2 w = *(const uint2*)(l + v);
-            uint2 w2 = w;
-            if (residual) w2 = *(const uint2*)(d + v);
-            vd_unpack<T>(make_uint4(w.x, w.y, w2.x, w2.y), t);
+      if (aligned) {
+        uint4 la, da = {}, ln, dn = {};
+        float4 ea[V / 4], en[V / 4];
+        auto fetch = [&](int64_t at) {  // one lot ahead of the one in work
+          const int64_t v = at * V;
+          if (at >= hi || v + V > P.vocab) return;
+          ln = *(const uint4*)(l + v);
+          if (residual) dn = *(const uint4*)(d + v);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              lv[i] = t[i];
-              dv[i] = t[V + i];
-            }
+          for (int i = 0; i < V / 4; ++i) en[i] = *(const float4*)(e + v + 4 * i);
+        };
+        fetch(lo + tid);
+        for (int64_t at = lo + tid; at < hi; at += THREADS) {
+          const int64_t v = at * V;
+          if (v + V > P.vocab) {  // the vocabulary's last elements
+            for (int64_t k = v; k < P.vocab; ++k) race(vd_f(l[k]), vd_f(d[k]), e[k], k);
+            break;
           }
-        } else {
+          la = ln;
+          da = dn;
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) ea[i] = en[i];
+          fetch(at + THREADS);
+          float lv[V], dv[V];
+          vd_unpack<T>(la, lv);
+          vd_unpack<T>(da, dv);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const bool in = v + i < P.vocab;
-            lv[i] = in ? vd_f(l[v + i]) : -INFINITY;
-            dv[i] = in && residual ? vd_f(d[v + i]) : -INFINITY;
-            ev[i] = in ? e[v + i] : 1.f;
+            const float4& f = ea[i / 4];
+            race(lv[i], dv[i], i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w, v + i);
           }
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) race(lv[i], dv[i], ev[i], v + i);
+      } else {
+        // rows that start anywhere: element by element, a warp's loads side by side
+        const int64_t end = min(hi * V, P.vocab);
+#pragma unroll 8
+        for (int64_t v = lo * V + tid; v < end; v += THREADS) race(vd_f(l[v]), residual ? vd_f(d[v]) : 0.f, e[v], v);
       }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        vd_best_warp(best[k]);
-        if (lane == 0) s_best[k][warp] = best[k];
-      }
+      vd_best_warp(best);
+      if (lane == 0) s_best[warp] = best;
       __syncthreads();
       if (warp == 0) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          Best a = lane < VD_THREADS / 32 ? s_best[k][lane] : Best{0.f, -1};
-          vd_best_warp(a);
-          if (lane == 0) s_mine[k] = a;
-        }
+        Best a = lane < WARPS ? s_best[lane] : Best{0.f, 1.f, -1};
+        vd_best_warp(a);
+        if (lane == 0) s_mine[pass] = a;
       }
+      cluster.sync();  // the CTAs' best are there
+      Best a{0.f, 1.f, -1};
+      if (lane < ctas) a = *cluster.map_shared_rank(&s_mine[pass], lane);
+      vd_best_warp(a);
+      token = a.i;  // the same in every thread of the cluster
+      residual = false;
+      out = -1;
     }
-    cluster.sync();  // the CTAs' best are there
-    if (rank == 0 && count > 0) {
-      Best a[2] = {{0.f, -1}, {0.f, -1}};
-      for (int r = 0; r < ctas; ++r) {
-        const Best* const other = cluster.map_shared_rank(s_mine, r);
-        vd_best(a[0], other[0]);
-        vd_best(a[1], other[1]);
-      }
-      token = a[0].i >= 0 ? a[0].i : a[1].i;
-    }
-    cluster.sync();  // and read
+    cluster.sync();  // no CTA leaves while its best is read
   }
   if (rank) return;
-  for (int i = tid; i < P.max_tokens; i += VD_THREADS) {
-    const int x = i < taken ? P.tokens_in[first + i + 1] : (i == taken && count > 0 ? token : -1);
-    P.tokens_out[(int64_t)b * P.max_tokens + i] = x;
-    if (P.logprobs) P.logprobs[(int64_t)b * P.max_tokens + i] = x < 0 ? 0.f : logp(i, x);
+  if (tid < P.max_tokens) {  // at most VD_MAX_ROWS
+    const int t = tid < taken ? x : tid == taken && count > 0 ? token : -1;
+    P.tokens_out[(int64_t)b * P.max_tokens + tid] = t;
+    if (P.logprobs) {
+      if (tid == taken && t >= 0) lx = vd_f(target(tid)[t]);
+      P.logprobs[(int64_t)b * P.max_tokens + tid] = t < 0 ? 0.f : logp(lx, tid);
+    }
   }
   if (tid == 0) {
     P.accepted[b] = taken;
@@ -342,17 +393,17 @@ void launch_t(const VerifyParams& p, cudaStream_t s) {
   }
   // a cluster races as wide as the vocabulary gives every thread a few vectors
   int ctas = 1;
-  while (!p.greedy && ctas < VD_CLUSTER && p.vocab > (int64_t)ctas * VD_THREADS * 16) ctas *= 2;
-  launch_k(verify_pick_kernel<T>, dim3((unsigned)(p.num_seqs * ctas)), VD_THREADS, 0, s, ctas, p);
+  while (!p.greedy && ctas < VD_CLUSTER && p.vocab > (int64_t)ctas * VD_PICK_THREADS * 8) ctas *= 2;
+  launch_k(verify_pick_kernel<T>, dim3((unsigned)(p.num_seqs * ctas)), VD_PICK_THREADS, 0, s, ctas, p);
 }
 
 }  // namespace
 
-// Slices of a row: four CTAs' worth per SM over all rows, none below two
-// vectors a thread.
+// Slices of a row: up to eight CTAs per SM over all rows, none below two vectors
+// a thread.
 int verify_splits(int64_t tokens, int64_t vocab, bool draft) {
   const int64_t rows = std::max<int64_t>(tokens * (draft ? 2 : 1), 1);
-  const int64_t want = (4 * (int64_t)device_sm_count() + rows - 1) / rows;
+  const int64_t want = std::max<int64_t>(8 * (int64_t)device_sm_count() / rows, 1);
   const int64_t most = std::max<int64_t>(vocab / (VD_THREADS * 8), 1);
   return (int)std::min<int64_t>(std::min(want, most), VD_MAX_SPLITS);
 }

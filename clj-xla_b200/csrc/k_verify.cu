@@ -234,11 +234,6 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t lots = (P.vocab + V - 1) / V, lo = lots * rank / ctas, hi = lots * (rank + 1) / ctas;
-  if (!P.greedy) {  // whatever row decides, this CTA's part of e is needed: into L2 while the rows are read
-    const char* const e = (const char*)(P.race + b * P.race_stride + lo * V);
-    const int64_t bytes = (min(hi * V, P.vocab) - lo * V) * 4;
-    for (int64_t at = tid * 128; at < bytes; at += THREADS * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(e + at));
-  }
   pdl_enter();
   int first, count;
   vd_rows(P, b, first, count);

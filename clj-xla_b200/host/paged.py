@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 import threading
 from typing import Optional
 
@@ -76,18 +77,26 @@ class _VerifyArgs(ctypes.Structure):
                 ("workspace_bytes", _I)]
 
 
+# The argument structures as one packing each, faster than filling a ctypes
+# structure.  Fresh bytes per call, so calls from several threads share nothing.
+_APPEND, _ATTENTION, _VERIFY = struct.Struct("=18q1i1f"), struct.Struct("=12q2f2i2q"), struct.Struct("=14q2f2i7q")
+_pack_append, _pack_attention, _pack_verify = _APPEND.pack, _ATTENTION.pack, _VERIFY.pack
+_append_size, _attention_size, _verify_size = _APPEND.size, _ATTENTION.size, _VERIFY.size
+
+
 class _Calls:
     """The library's entries, bound once."""
 
     def __init__(self, path: str):
         lib = ctypes.CDLL(path)
+        args = _P  # packed bytes, see above
         call = [_P, ctypes.c_char_p, ctypes.c_size_t]
         size = [ctypes.POINTER(_I), ctypes.c_char_p, ctypes.c_size_t]
-        self.append = self._bind(lib.cljxla_b200_paged_append, [_P, _P] + call)
-        self.attend = self._bind(lib.cljxla_b200_paged_attention, [_P, _P] + call)
-        self.attend_size = self._bind(lib.cljxla_b200_paged_attention_workspace, [_P, _P] + size)
-        self.verify = self._bind(lib.cljxla_b200_verify_draft, [_P] + call)
-        self.verify_size = self._bind(lib.cljxla_b200_verify_draft_workspace, [_P] + size)
+        self.append = self._bind(lib.cljxla_b200_paged_append, [_P, args] + call)
+        self.attend = self._bind(lib.cljxla_b200_paged_attention, [_P, args] + call)
+        self.attend_size = self._bind(lib.cljxla_b200_paged_attention_workspace, [_P, args] + size)
+        self.verify = self._bind(lib.cljxla_b200_verify_draft, [args] + call)
+        self.verify_size = self._bind(lib.cljxla_b200_verify_draft_workspace, [args] + size)
 
     @staticmethod
     def _bind(f, types):
@@ -118,11 +127,15 @@ def _raise(rc: int):
     raise PJRTError(_err().value.decode(), rc)
 
 
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()  # torch.cuda.current_device() less its initialisation check: a CUDA tensor exists
+
+
 def _enqueue(device: int, call, *args):
     """Calls a library entry with torch's current stream of `device`, which is
     made the current device for the call."""
     err = _err()
-    if torch.cuda.current_device() != device:
+    if _current_device() != device:
         with torch.cuda.device(device):
             rc = call(*args, torch.cuda.current_stream(device).cuda_stream, err, 512)
     else:
@@ -131,21 +144,43 @@ def _enqueue(device: int, call, *args):
         _raise(rc)
 
 
+class _Sizes(dict):
+    """Workspace bytes by (device, sizes): a property of the sizes alone."""
+
+    def of(self, key, call, *args) -> int:
+        if len(self) >= 4096:
+            self.clear()
+        got = _I()
+        with torch.cuda.device(key[0]):
+            rc = call(*args, ctypes.byref(got), _err(), 512)
+        if rc:
+            _raise(rc)
+        self[key] = got.value
+        return got.value
+
+
+def _expected(name: str, shape, dtype, device: int, t: torch.Tensor, what: str = ""):
+    raise ValueError(f"{name}: {list(shape)} {dtype} on cuda:{device}{what} expected, got {list(t.shape)} {t.dtype} on "
+                     f"{t.device} with strides {t.stride()}")
+
+
 def _rows(t: torch.Tensor, name: str, shape, dtype, device: int):
     """Strides of a [rows, heads, head_dim] tensor whose last axis is contiguous."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
-        raise ValueError(f"{name}: {tuple(shape)} {dtype} on cuda:{device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
     s = t.stride()
-    if s[2] != 1:
-        raise ValueError(f"{name}: head_dim must be contiguous, got strides {s}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or s[2] != 1:
+        _expected(name, shape, dtype, device, t, " with head_dim contiguous")
     return s
 
 
-def _vector(t: torch.Tensor, name: str, n: Optional[int], dtype, device: int):
-    if t.dtype is not dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.get_device() != device \
-            or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous [{'n' if n is None else n}] {dtype} on cuda:{device} expected, "
-                         f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _vector(t: torch.Tensor, name: str, n: int, dtype, device: int) -> int:
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+        _expected(name, (n,), dtype, device, t, ", contiguous,")
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, name: str, rows: int, cols: int, dtype, device: int) -> int:
+    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != device or (cols > 1 and t.stride(1) != 1):
+        _expected(name, (rows, cols), dtype, device, t, " with contiguous rows")
     return t.data_ptr()
 
 
@@ -191,6 +226,8 @@ class Rope:
                 or not inv_freq.is_cuda:
             raise ValueError("Rope: inv_freq must be a contiguous f32 vector on a CUDA device")
         self.inv_freq, self.interleaved, self.scale = inv_freq, bool(interleaved), float(scale)
+        self.device = inv_freq.get_device()
+        self._args = (inv_freq.data_ptr(), 2 * inv_freq.shape[0], self.interleaved, self.scale)
 
 
 class PagedKV:
@@ -222,10 +259,7 @@ class PagedKV:
                              page_table.shape[1], page_table.stride(0), _TYPES[self.dtype], 0)
         self._at = ctypes.addressof(self._cache)
         self._lib = _library()
-        self._sizes = {}
-
-    def _starts(self, starts):
-        return None if starts is None else _vector(starts, "starts", self.num_seqs + 1, torch.int32, self.device)
+        self._key = (self.num_seqs, page_table.shape[1], heads, size, dim, self.dtype)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, q: Optional[torch.Tensor] = None,
                q_out: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, rope: Optional[Rope] = None):
@@ -233,30 +267,36 @@ class PagedKV:
         their pages, ``k`` rotated by ``rope``, and the rotated ``q`` ``[rows,
         q_heads, head_dim]`` into ``q_out`` (``q`` itself by default).  Rows whose
         page the table does not name are left out.  Returns ``q_out``."""
-        n, heads, dim, dt, dev = k.shape[0], self.kv_heads, self.head_dim, self.dtype, self.device
-        ks = _rows(k, "k", (n, heads, dim), dt, dev)
-        vs = _rows(v, "v", (n, heads, dim), dt, dev)
-        a = _AppendArgs(ctypes.sizeof(_AppendArgs), k.data_ptr(), v.data_ptr(), None, None, n, 0, ks[0], ks[1], vs[0], vs[1])
+        dt, dev, dim = self.dtype, self.device, self.head_dim
+        n = k.shape[0]
+        shape = (n, self.kv_heads, dim)
+        ks = _rows(k, "k", shape, dt, dev)
+        vs = _rows(v, "v", shape, dt, dev)
         if q is not None:
             if q_out is None:
                 q_out = q
             if q.dim() != 3:
                 raise ValueError("q: [rows, q_heads, head_dim] expected")
             nq = q.shape[1]
-            qs = _rows(q, "q", (n, nq, dim), dt, dev)
-            os = _rows(q_out, "q_out", (n, nq, dim), dt, dev)
-            a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), nq
-            a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride = qs[0], qs[1], os[0], os[1]
+            shape = (n, nq, dim)
+            qs = _rows(q, "q", shape, dt, dev)
+            os = qs if q_out is q else _rows(q_out, "q_out", shape, dt, dev)
+            qp, op = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        if starts is not None:
-            a.starts = self._starts(starts)
-        if rope is not None:
-            if rope.inv_freq.get_device() != dev:
+        else:
+            nq = qp = op = 0
+            qs = os = (0, 0)
+        sp = 0 if starts is None else _vector(starts, "starts", self.num_seqs + 1, torch.int32, dev)
+        if rope is None:
+            fp, rotary, interleaved, scale = 0, 0, False, 1.0
+        else:
+            fp, rotary, interleaved, scale = rope._args
+            if rope.device != dev:
                 raise ValueError("rope: inv_freq must be on the pages' device")
-            a.inv_freq, a.rotary_dim = rope.inv_freq.data_ptr(), 2 * rope.inv_freq.shape[0]
-            a.interleaved, a.rope_scale = rope.interleaved, rope.scale
-        _enqueue(dev, self._lib.append, self._at, ctypes.addressof(a))
+        _enqueue(dev, self._lib.append, self._at,
+                 _pack_append(_append_size, k.data_ptr(), v.data_ptr(), qp, op, n, nq, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0],
+                              os[1], sp, fp, rotary, interleaved, scale))
         return q_out
 
     def attend(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
@@ -271,50 +311,35 @@ class PagedKV:
         dt, dev, dim = self.dtype, self.device, self.head_dim
         if q.dim() != 3:
             raise ValueError("q: [rows, q_heads, head_dim] expected")
-        n, nq = q.shape[0], q.shape[1]
-        qs = _rows(q, "q", (n, nq, dim), dt, dev)
+        n, nq, _ = q.shape
+        shape = (n, nq, dim)
+        qs = _rows(q, "q", shape, dt, dev)
         if out is None:
-            out = torch.empty((n, nq, dim), dtype=dt, device=q.device)
+            out = torch.empty(shape, dtype=dt, device=q.device)
         odt = out.dtype
         if odt is not dt and odt is not torch.float32:
             raise ValueError(f"out: {dt} or torch.float32 expected, got {odt}")
-        os = _rows(out, "out", (n, nq, dim), odt, dev)
+        os = _rows(out, "out", shape, odt, dev)
         if max_tokens is None:
             max_tokens = n
-        a = _AttentionArgs(ctypes.sizeof(_AttentionArgs), q.data_ptr(), out.data_ptr(), n, nq, qs[0], qs[1], os[0], os[1],
-                           self._starts(starts), max_tokens, window, dim ** -0.5 if scale is None else scale, softcap,
-                           _TYPES[odt])
-        at = ctypes.addressof(a)
-        key = (n, nq, max_tokens, starts is None, window)
-        need = self._sizes.get(key)
+        if scale is None:
+            scale = dim ** -0.5
+        sp = 0 if starts is None else _vector(starts, "starts", self.num_seqs + 1, torch.int32, dev)
+        key = (dev, n, nq, max_tokens, sp == 0, window)
+        need = _attend_sizes.get(key + self._key)
         if need is None:
-            need = self._sizes[key] = _size(dev, self._lib.attend_size, self._at, at)
-        if need:
-            # from torch's allocator on this call's stream: calls that overlap, and captured graphs, have one each
-            work = torch.empty(need, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspace_bytes = work.data_ptr(), need
-        _enqueue(dev, self._lib.attend, self._at, at)
+            need = _attend_sizes.of(key + self._key, self._lib.attend_size, self._at,
+                                    _pack_attention(_attention_size, 0, 0, n, nq, qs[0], qs[1], os[0], os[1], sp, max_tokens, window, scale,
+                                                    softcap, _TYPES[odt], 0, 0, 0))
+        # from torch's allocator on this call's stream: calls that overlap, and captured graphs, have one each
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _enqueue(dev, self._lib.attend, self._at,
+                 _pack_attention(_attention_size, q.data_ptr(), out.data_ptr(), n, nq, qs[0], qs[1], os[0], os[1], sp, max_tokens, window,
+                                 scale, softcap, _TYPES[odt], 0, work.data_ptr() if need else 0, need))
         return out
 
 
-def _size(device: int, call, *args) -> int:
-    """A workspace query, with `device` as the current one."""
-    got = _I()
-    with torch.cuda.device(device):
-        rc = call(*args, ctypes.byref(got), _err(), 512)
-    if rc:
-        _raise(rc)
-    return got.value
-
-
-_verify_sizes = {}
-
-
-def _matrix(t, name, rows, cols, dtype, device):
-    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != device or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: [{rows}, {cols}] {dtype} with contiguous rows on cuda:{device} expected, "
-                         f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.data_ptr()
+_attend_sizes, _verify_sizes = _Sizes(), _Sizes()
 
 
 def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
@@ -345,42 +370,42 @@ def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, starts: Opti
     if not target_logits.is_cuda or target_logits.dim() != 2 or target_logits.dtype not in _TYPES or out_tokens.dim() != 2:
         raise ValueError("target_logits: [rows, vocab] f32, f16 or bf16 on a CUDA device, out_tokens: [num_seqs, max_tokens] expected")
     dev, dt = target_logits.get_device(), target_logits.dtype
+    i32, f32 = torch.int32, torch.float32
     rows, vocab = target_logits.shape
     seqs, most = out_tokens.shape
-    a = _VerifyArgs(ctypes.sizeof(_VerifyArgs), _matrix(target_logits, "target_logits", rows, vocab, dt, dev), None,
-                    _vector(tokens, "tokens", rows, torch.int32, dev))
-    if starts is not None:
-        a.starts = _vector(starts, "starts", seqs + 1, torch.int32, dev)
-    a.tokens, a.num_seqs, a.vocab, a.max_tokens = rows, seqs, vocab, most
-    a.target_stride = target_logits.stride(0)
-    a.temperature, a.dtype, a.greedy = temperature, _TYPES[dt], greedy
+    tp = _matrix(target_logits, "target_logits", rows, vocab, dt, dev)
+    ip = _vector(tokens, "tokens", rows, i32, dev)
+    sp = 0 if starts is None else _vector(starts, "starts", seqs + 1, i32, dev)
+    up = rp = dp = rs = ds = 0
+    if draft_temperature is None:
+        draft_temperature = temperature
     if not greedy:
         if uniform is None or race is None:
             raise ValueError("uniform and race are needed unless greedy")
-        a.uniform = _vector(uniform, "uniform", rows, torch.float32, dev)
-        a.race, a.race_stride = _matrix(race, "race", seqs, vocab, torch.float32, dev), race.stride(0)
+        up = _vector(uniform, "uniform", rows, f32, dev)
+        rp, rs = _matrix(race, "race", seqs, vocab, f32, dev), race.stride(0)
         if draft_logits is not None:
-            a.draft, a.draft_stride = _matrix(draft_logits, "draft_logits", rows, vocab, dt, dev), draft_logits.stride(0)
-            a.draft_temperature = temperature if draft_temperature is None else draft_temperature
-    if not out_tokens.is_contiguous():
-        raise ValueError("out_tokens must be contiguous")
-    a.tokens_out = _matrix(out_tokens, "out_tokens", seqs, most, torch.int32, dev)
-    a.accepted = _vector(accepted, "accepted", seqs, torch.int32, dev)
-    if logprobs is not None:
-        if not logprobs.is_contiguous():
-            raise ValueError("logprobs must be contiguous")
-        a.logprobs = _matrix(logprobs, "logprobs", seqs, most, torch.float32, dev)
+            dp, ds = _matrix(draft_logits, "draft_logits", rows, vocab, dt, dev), draft_logits.stride(0)
+    op = _matrix(out_tokens, "out_tokens", seqs, most, i32, dev)
+    ap = _vector(accepted, "accepted", seqs, i32, dev)
+    lp = 0 if logprobs is None else _matrix(logprobs, "logprobs", seqs, most, f32, dev)
+    if not out_tokens.is_contiguous() or (logprobs is not None and not logprobs.is_contiguous()):
+        raise ValueError("out_tokens and logprobs must be contiguous")
+    np = nn = 0
     if new_lens is not None:
         if seq_lens is None:
             raise ValueError("new_lens needs seq_lens")
-        a.seq_lens = _vector(seq_lens, "seq_lens", seqs, torch.int32, dev)
-        a.new_lens = _vector(new_lens, "new_lens", seqs, torch.int32, dev)
-    lib, at = _library(), ctypes.addressof(a)
-    key = (dev, rows, seqs, vocab, most, starts is None, a.draft is None)
+        np = _vector(seq_lens, "seq_lens", seqs, i32, dev)
+        nn = _vector(new_lens, "new_lens", seqs, i32, dev)
+    lib = _library()
+    key = (dev, rows, seqs, vocab, most, dp == 0, sp == 0)
+
+    def packed(work, size):
+        return _pack_verify(_verify_size, tp, dp, ip, sp, up, rp, rows, seqs, vocab, most, target_logits.stride(0), ds, rs, temperature,
+                            draft_temperature, _TYPES[dt], bool(greedy), op, ap, lp, np, nn, work, size)
+
     need = _verify_sizes.get(key)
     if need is None:
-        need = _verify_sizes[key] = _size(dev, lib.verify_size, at)
-    if need:
-        work = torch.empty(need, dtype=torch.uint8, device=target_logits.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-    _enqueue(dev, lib.verify, at)
+        need = _verify_sizes.of(key, lib.verify_size, packed(0, 0))
+    work = torch.empty(need, dtype=torch.uint8, device=target_logits.device) if need else None
+    _enqueue(dev, lib.verify, packed(work.data_ptr() if need else 0, need))

@@ -161,6 +161,8 @@ def test_struct_layouts_match_the_header(paged, tmp_path):
             want.append(getattr(t, f).offset)
     (tmp_path / "l.c").write_text(src + "return 0; }\n")
     subprocess.run(["gcc", "-I" + os.path.join(ROOT, "include"), str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    assert [s.size for s in (paged._APPEND, paged._ATTENTION, paged._VERIFY)] == \
+        [ctypes.sizeof(t) for t in (paged._AppendArgs, paged._AttentionArgs, paged._VerifyArgs)]
     got = subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == want
 

@@ -43,8 +43,8 @@ struct PagedAttnParams {
   // set at the launch: the factor from q.k to the argument of 2^x (with a cap:
   // of tanh), log2(e) * softcap
   float mul, cap2;
-  float* part;    // per CTA: two slots of rows and their (max, sum)
-  int32_t* meta;  // 8 per CTA: CTAs that share the segment starting there (0: none), head, row tile, first row, rows
+  float* part;  // per CTA: two slots of rows and their (max, sum)
+  uint32_t group_mul;  // 2^32 / group rounded up (0: group 1), set at the launch
 };
 
 struct VerifyParams {

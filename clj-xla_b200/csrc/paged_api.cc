@@ -152,6 +152,7 @@ PagedAttnParams attention_params(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAtt
   need(a->q_heads >= 1 && a->q_heads <= 65535 && a->q_heads % kv->kv_heads == 0,
        "q_heads must be a multiple of kv_heads");
   p.group = (int32_t)(a->q_heads / kv->kv_heads);
+  need(p.group <= 32768, "q_heads is more than 32768 times kv_heads");
   const int out_dt = element_type(a->out_dtype);
   need(out_dt == p.dt || out_dt == KDT_F32, "out_dtype must be the pages' type or F32");
   p.out_f32 = out_dt == KDT_F32;

@@ -44,7 +44,6 @@ namespace cljxla {
 namespace {
 
 constexpr int AT_CONSUMERS = 128, AT_JOIN_THREADS = 128;
-constexpr int kAttnMaxCtas = 1024;  // SMs times CTAs on one, at most
 
 // ------------------------------------------------------------------ layout
 template <typename T, int HD, int NR>
@@ -60,7 +59,7 @@ struct Tile {
   // weights as two 16-bit parts or one f32: in the tile's K rows once they are scored, if they fit
   static constexpr int PB = ROWS * TP * 4;
   static constexpr bool P_IN_K = PB <= KB;
-  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 64 + 4 * TP * 8; }
+  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 96 + 4 * TP * 8; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
     int n = 0;
     while (n < 4 && fixed(n + 1) + (n + 1) * STAGE <= 233472 / ctas - 1024) ++n;
@@ -202,34 +201,114 @@ __device__ __forceinline__ bool odd_chunk(const uint4& v) {
 
 // --------------------------------------------------------------- schedule
 // A tile: positions [pos0, pos0 + npos) of segment (b, head, rows row0 ..).
+// Its rows are `nrows` rows from head g0 of the group at the sequence's row q0 on.
 struct TileDesc {
-  int head, row0, pos0, npos, flags, qslot, first, count, p0;  // p0: position of the sequence's first row
+  int head, q0, g0, nrows, pos0, npos, flags, qslot, first, count, p0;  // p0: position of the sequence's first row
   uint32_t mask[2];  // positions whose page is there
 };
 enum { T_FIRST = 1, T_LAST = 2, T_FROM0 = 4, T_TOEND = 8, T_FULL = 16, T_END = 32 };  // T_END: the CTA's last tile
 
 // One sequence's share of the schedule.
 struct SeqPlan {
-  int first, count, rows, p0, lo, hi, units, tiles;  // rows: computed ones; tiles: row tiles
-  __device__ __forceinline__ void load(const PagedAttnParams& P, int b, int tile, int row_tile) {
-    int n;
-    seq_rows(P.c, b, first, n);
+  int first, count, rows, p0, lo, hi, units, tiles;  // rows: computed ones; units: position tiles; tiles: row tiles
+  __device__ __forceinline__ void make(const PagedAttnParams& P, int begin, int n, int len, int tile, int row_tile) {
+    first = begin;
     count = min(n, P.max_rows);
     rows = count * P.group;
     tiles = (rows + row_tile - 1) / row_tile;
-    p0 = seq_len(P.c, b) - n;
+    p0 = len - n;
     lo = P.window < 0 ? 0 : (int)max((int64_t)p0 - P.window, (int64_t)0);
     hi = min(p0 + count, capacity(P.c));
     units = max((hi - lo + tile - 1) / tile, 1);
   }
+  __device__ __forceinline__ void load(const PagedAttnParams& P, int b, int tile, int row_tile) {
+    int begin, n;
+    seq_rows(P.c, b, begin, n);
+    make(P, begin, n, seq_len(P.c, b), tile, row_tile);
+  }
   __device__ __forceinline__ int64_t cost(int nkv) const { return (int64_t)units * nkv * tiles; }
 };
 
-// The positions of tile `d` that query row `in_tile` of it sees: [jlo, jhi].
-__device__ __forceinline__ void row_view(const PagedAttnParams& P, const TileDesc& d, int in_tile, int& jlo, int& jhi) {
-  const int row = d.row0 + in_tile;
-  const int pos = d.p0 + row / P.group;  // the row's own position
-  jhi = row < d.count * P.group ? pos - d.pos0 : -1;
+__device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {  // a >= 0, b > 0
+  return (((uint64_t)a | (uint64_t)b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// How `total` tiles are cut: the first `more` CTAs have each + 1 of them, the others each.
+struct Cut {
+  int64_t total, each, more, ctas;
+  __device__ __forceinline__ void make(int64_t tiles) {
+    total = tiles;
+    ctas = min((int64_t)gridDim.x, total);
+    each = ctas ? div_small(total, ctas) : 0;
+    more = total - each * ctas;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t cta) const { return each * cta + min(cta, more); }
+  __device__ __forceinline__ int64_t owner(int64_t tile) const {
+    const int64_t edge = more * (each + 1);
+    return tile < edge ? div_small(tile, each + 1) : more + div_small(tile - edge, each);
+  }
+};
+
+// Cuts the call's tiles and finds the sequence that holds the one `pick` names
+// (of the cut), and its place there: sh[8], sh[9] (-1: none was found, which takes
+// lengths that change under the kernel).  By all THREADS threads of a CTA; the
+// results are for use after the next barrier.
+template <int THREADS, int TP, int ROWS, class F>
+__device__ __forceinline__ Cut locate(const PagedAttnParams& P, int64_t* sh, F pick) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const PagedView& c = P.c;
+  const int per = (c.num_seqs + THREADS - 1) / THREADS;
+  const int b0 = min(tid * per, c.num_seqs), b1 = min(b0 + per, c.num_seqs);
+  SeqPlan sp;
+  int64_t mine = 0;
+  for (int i = b0; i < b1; ++i) {
+    sp.load(P, i, TP, ROWS);
+    mine += sp.cost(c.nkv);
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh[warp] = incl;
+  if (tid == 0) {
+    sh[8] = 0;
+    sh[9] = -1;
+  }
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) incl += sh[w];
+    total += sh[w];
+  }
+  Cut cut;
+  cut.make(total);
+  const int64_t want = pick(cut);
+  int64_t excl = incl - mine;
+  if (want >= excl && want < incl) {
+    for (int i = b0; i < b1; ++i) {
+      if (per > 1) sp.load(P, i, TP, ROWS);
+      if (want < excl + sp.cost(c.nkv)) {
+        sh[8] = i;
+        sh[9] = want - excl;
+        break;
+      }
+      excl += sp.cost(c.nkv);
+    }
+  }
+  return cut;
+}
+
+// x / group for x below 64 + group
+__device__ __forceinline__ int div_group(const PagedAttnParams& P, int x) {
+  return P.group_mul ? (int)__umulhi((uint32_t)x, P.group_mul) : x;
+}
+
+// The positions of tile `d` that its query row `r` sees: [jlo, jhi].
+__device__ __forceinline__ void row_view(const PagedAttnParams& P, const TileDesc& d, int r, int& jlo, int& jhi) {
+  const int pos = d.p0 + d.q0 + div_group(P, r + d.g0);  // the row's own position
+  jhi = r < d.nrows ? pos - d.pos0 : -1;
   jlo = P.window < 0 ? 0 : (int)max((int64_t)pos - P.window - d.pos0, (int64_t)0);
 }
 
@@ -245,62 +324,17 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   float* const wsum = wmax + 4 * ROWS;
   TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
   int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
-  const char** const rows = (const char**)(sh + 8);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
+  const char** const rows = (const char**)(sh + 12);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedView& c = P.c;
   pdl_enter();
 
   // ---- this CTA's range of tiles
-  int64_t left, total = 0, ctas;
-  {
-    SeqPlan sp;
-    const int per = (c.num_seqs + AT_THREADS - 1) / AT_THREADS;
-    const int b0 = min(tid * per, c.num_seqs), b1 = min(b0 + per, c.num_seqs);
-    int64_t mine = 0;
-    for (int i = b0; i < b1; ++i) {
-      sp.load(P, i, TP, ROWS);
-      mine += sp.cost(c.nkv);
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) sh[warp] = incl;
-    __syncthreads();
-    for (int w = 0; w < AT_THREADS / 32; ++w) {
-      if (w < warp) incl += sh[w];
-      total += sh[w];
-    }
-    ctas = min((int64_t)gridDim.x, total);
-    if ((int64_t)blockIdx.x >= ctas) {
-      if (tid == 0 && P.meta) P.meta[blockIdx.x * 8] = 0;
-      return;
-    }
-    const int64_t beg = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-    left = end - beg;
-    __syncthreads();
-    if (tid == 0) {
-      sh[0] = sh[1] = 0;
-      if (P.meta) P.meta[blockIdx.x * 8] = 0;  // no segment that starts here is cut, so far
-    }
-    __syncthreads();
-    int64_t excl = incl - mine;
-    if (beg >= excl && beg < incl) {
-      for (int i = b0; i < b1; ++i) {
-        sp.load(P, i, TP, ROWS);
-        if (beg < excl + sp.cost(c.nkv)) {
-          sh[0] = i;
-          sh[1] = beg - excl;
-          break;
-        }
-        excl += sp.cost(c.nkv);
-      }
-    }
-    __syncthreads();
-  }
+  const Cut cut = locate<AT_THREADS, TP, ROWS>(P, sh, [](const Cut& k) { return k.begin(blockIdx.x); });
+  if ((int64_t)blockIdx.x >= cut.ctas) return;
+  int64_t left = cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
+  __syncthreads();
 
   // Stage hand-over: full[s] (producers arrive, consumers wait), empty[s] (consumers
   // arrive, the scheduler waits); ahead: the producers among themselves.
@@ -310,7 +344,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
   constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
   const int my_row = lane / LANES, my_chunk = lane % LANES;
-  volatile int* const plan = (volatile int*)(sh + 2);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
+  volatile int* const plan = (volatile int*)(sh + 10);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
   constexpr int ALL_THERE = 256, DONE = -1, BROKEN = -2;
   // Producers: before the next tile's stage is waited for, the oldest tile in
   // flight is handed to the consumers.
@@ -381,83 +415,93 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   }
   if (warp == AT_CONSUMERS / 32) {
     // =============================================================== scheduler
-    int b = (int)sh[0];  // cursor: sequence, segment of it (head, row tile), tile of that
+    // Two tiles are on their way: one whose pages are known by now, one whose page
+    // numbers have just been asked for; and the sequence behind the cursor's.
+    struct Look {
+      TileDesc d;
+      int page[TP / 32], in_page[TP / 32];
+    };
+    int b = (int)sh[8];  // cursor: sequence, segment of it (head, row tile), tile of that
     SeqPlan sp;
     sp.load(P, b, TP, ROWS);
-    const int64_t off = sh[1];
-    if (off >= sp.cost(c.nkv)) left = 0;  // lengths that change under the kernel: stay in bounds
-    int seg = (int)(off / sp.units), at = (int)(off % sp.units), qslot = -1;
-    bool fresh = true;  // the next tile is the first of its piece
+    const int64_t off = sh[9];
+    if (off < 0 || off >= sp.cost(c.nkv)) left = 0;  // lengths that change under the kernel: stay in bounds
+    int seg = left ? (int)div_small(off, sp.units) : 0, at = left ? (int)(off - (int64_t)seg * sp.units) : 0, qslot = -1;
+    int head = sp.tiles ? seg / sp.tiles : 0, row_tile = seg - head * sp.tiles;
+    bool fresh = true;    // the next tile is the first of its piece
     bool piece0 = false;  // whether the piece starts its segment
-    TileDesc nd;
-    int page[TP / 32], in_page[TP / 32];
-    auto next = [&]() -> bool {  // the cursor's next tile into nd; starts its page lookup
+    int then_first, then_n, then_len;
+    auto peek = [&]() {  // the sequence after b, asked for early
+      if (b + 1 >= c.num_seqs) return;
+      seq_rows(c, b + 1, then_first, then_n);
+      then_len = seq_len(c, b + 1);
+    };
+    peek();
+    auto next = [&](Look& k) -> bool {  // the cursor's next tile; starts its page lookup
       if (left == 0) return false;
       if (at >= sp.units) {
         at = 0;
-        if (++seg >= c.nkv * sp.tiles) {
-          seg = 0;
-          do {
-            if (++b >= c.num_seqs) {
-              left = 0;
-              return false;
-            }
-            sp.load(P, b, TP, ROWS);
-          } while (sp.tiles == 0);
-        }
         fresh = true;
+        if (++row_tile >= sp.tiles) {
+          row_tile = 0;
+          if (++head >= c.nkv) {
+            head = 0;
+            do {
+              if (++b >= c.num_seqs) {
+                left = 0;
+                return false;
+              }
+              sp.make(P, then_first, then_n, then_len, TP, ROWS);
+              peek();
+            } while (sp.tiles == 0);
+          }
+        }
       }
       if (fresh) {
         qslot = qslot + 1 == NST ? 0 : qslot + 1;
         piece0 = at == 0;
       }
-      nd.head = sp.tiles == 1 ? seg : seg / sp.tiles;
-      nd.row0 = (seg - nd.head * sp.tiles) * ROWS;
-      nd.pos0 = sp.lo + at * TP;
-      nd.npos = max(min(TP, sp.hi - nd.pos0), 0);
-      nd.qslot = qslot;
-      nd.first = sp.first;
-      nd.count = sp.count;
-      nd.p0 = sp.p0;
-      nd.flags = (fresh ? T_FIRST : 0) | (piece0 ? T_FROM0 : 0);
+      TileDesc& d = k.d;
+      const int row0 = row_tile * ROWS;
+      d.head = head;
+      d.q0 = row0 ? row0 / P.group : 0;
+      d.g0 = row0 - d.q0 * P.group;
+      d.nrows = min(sp.rows - row0, ROWS);
+      d.pos0 = sp.lo + at * TP;
+      d.npos = max(min(TP, sp.hi - d.pos0), 0);
+      d.qslot = qslot;
+      d.first = sp.first;
+      d.count = sp.count;
+      d.p0 = sp.p0;
+      d.flags = (fresh ? T_FIRST : 0) | (piece0 ? T_FROM0 : 0);
       ++at;
       --left;
-      if (at == sp.units) nd.flags |= T_LAST | T_TOEND;
-      if (left == 0) {
-        nd.flags |= T_LAST;
-        if (piece0 && at < sp.units && lane == 0) {
-          // the range ends inside a segment that starts here: its last tile belongs to CTA `to`
-          const int64_t end = total * (blockIdx.x + 1) / ctas;
-          const int64_t to = ((end + (sp.units - at)) * ctas - 1) / total;
-          const int n = (int)(min(to, ctas - 1) - blockIdx.x + 1);
-          int4* const meta = (int4*)(P.meta + blockIdx.x * 8);
-          meta[0] = make_int4(n, nd.head, nd.row0, nd.first);
-          meta[1] = make_int4(nd.count * P.group, 0, 0, 0);
-        }
-      }
+      if (at == sp.units) d.flags |= T_LAST | T_TOEND;
+      if (left == 0) d.flags |= T_LAST;
       // every row sees every position, were all pages there
-      if (nd.npos == TP && nd.pos0 + TP - 1 <= nd.p0 && (P.window < 0 || nd.pos0 >= nd.p0 + nd.count - 1 - P.window))
-        nd.flags |= T_FULL;
+      if (d.npos == TP && d.pos0 + TP - 1 <= d.p0 && (P.window < 0 || d.pos0 >= d.p0 + d.count - 1 - P.window))
+        d.flags |= T_FULL;
       fresh = false;
 #pragma unroll
       for (int i = 0; i < TP / 32; ++i) {
-        const int j = nd.pos0 + i * 32 + lane;
-        page[i] = -1;
-        in_page[i] = 0;
-        if (i * 32 + lane < nd.npos) {
+        const int j = d.pos0 + i * 32 + lane;
+        k.page[i] = -1;
+        k.in_page[i] = 0;
+        if (i * 32 + lane < d.npos) {
           const int slot = c.page_shift >= 0 ? j >> c.page_shift : j / c.page_size;
-          page[i] = c.table[(int64_t)b * c.table_stride + slot];
-          in_page[i] = j - slot * c.page_size;
+          k.page[i] = c.table[(int64_t)b * c.table_stride + slot];
+          k.in_page[i] = j - slot * c.page_size;
         }
       }
       return true;
     };
 
     int tile = 0;
-    bool have = next();
+    Look now, then;
+    bool have = next(now);
     if (!have) {  // only if lengths change under the kernel: a tile of nothing ends the consumers
       if (lane == 0) {
-        *(TileDesc*)desc = TileDesc{0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
+        *(TileDesc*)desc = TileDesc{0, 0, 0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
         plan[0] = BROKEN;
       }
       bar_arrive<AT_THREADS>(FULL);
@@ -465,15 +509,18 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       return;
     }
     while (have) {
+      have = next(then);
       hand_over(tile);
       const int slot = tile % NST;
+      TileDesc& nd = now.d;
+      if (!have) nd.flags |= T_END;
       bool all = true;
 #pragma unroll
       for (int i = 0; i < TP / 32; ++i) {
-        const bool ok = (unsigned)page[i] < (unsigned)c.num_pages;
+        const bool ok = (unsigned)now.page[i] < (unsigned)c.num_pages;
         const char** const to = rows + (tile & 1) * 2 * TP + i * 32 + lane;
-        to[0] = ok ? c.k + page[i] * c.k_page + nd.head * c.k_head + in_page[i] * c.k_row : nullptr;
-        to[TP] = ok ? c.v + page[i] * c.v_page + nd.head * c.v_head + in_page[i] * c.v_row : nullptr;
+        to[0] = ok ? c.k + now.page[i] * c.k_page + nd.head * c.k_head + now.in_page[i] * c.k_row : nullptr;
+        to[TP] = ok ? c.v + now.page[i] * c.v_page + nd.head * c.v_head + now.in_page[i] * c.v_row : nullptr;
         nd.mask[i] = __ballot_sync(0xffffffffu, ok);
         all = all && nd.mask[i] == 0xffffffffu;
       }
@@ -485,13 +532,13 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       }
       bar_sync<AHEAD_THREADS>(AHEAD);
       if (nd.flags & T_FIRST) {
-        const uint32_t qd = smem_u32(ring + qslot * L::STAGE + 2 * L::KB);
+        const uint32_t qd = smem_u32(ring + nd.qslot * L::STAGE + 2 * L::KB);
         for (int r0 = 0; r0 < ROWS; r0 += RPI) {
-          const int r = r0 + my_row, row = nd.row0 + r;
-          const bool ok = row < nd.count * P.group;
-          const int qi = row / P.group;
-          const char* src = ok ? P.q + (int64_t)(nd.first + qi) * P.q_tok +
-                                     (int64_t)(nd.head * P.group + row - qi * P.group) * P.q_head
+          const int r = r0 + my_row;
+          const bool ok = r < nd.nrows;
+          const int dq = div_group(P, r + nd.g0);
+          const char* src = ok ? P.q + (int64_t)(nd.first + nd.q0 + dq) * P.q_tok +
+                                     (int64_t)(nd.head * P.group + r + nd.g0 - dq * P.group) * P.q_head
                                : P.q;
 #pragma unroll
           for (int e = 0; e < CPL; ++e) {
@@ -501,8 +548,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         }
       }
       cp_commit();
-      have = next();
-      if (!have && lane == 0) ((TileDesc*)((char*)desc + slot * 64))->flags |= T_END;
+      now = then;
       ++tile;
     }
     if (lane == 0) plan[tile & 1] = DONE;
@@ -808,17 +854,17 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int in_tile = n * 8 + 2 * t4 + r, row = d.row0 + in_tile;
-          if (row >= d.count * P.group) continue;
+          const int in_tile = n * 8 + 2 * t4 + r;
+          if (in_tile >= d.nrows) continue;
           float sum = 0.f;
 #pragma unroll
           for (int w = 0; w < SCORERS; ++w) sum += wsum[w * ROWS + in_tile];
           if (warp == 0 && g == 0 && !whole) *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(m[n][r], sum);
           if (ADDERS < 4 && warp >= ADDERS) continue;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
-          const int qi = row / P.group;
-          char* const o = P.out + (int64_t)(d.first + qi) * P.o_tok +
-                          (int64_t)(d.head * P.group + row - qi * P.group) * P.o_head;
+          const int dq = div_group(P, in_tile + d.g0);
+          char* const o = P.out + (int64_t)(d.first + d.q0 + dq) * P.o_tok +
+                          (int64_t)(d.head * P.group + in_tile + d.g0 - dq * P.group) * P.o_head;
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -836,41 +882,61 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
 }
 
 // Adds up the partials of the segment that starts in CTA blockIdx.x and is cut
-// by its end: one row of it per blockIdx.y.  Two round trips to memory: what to
-// add, then statistics and values together (the first PRE partials of a group of
-// lanes are fetched before their weights are known).
-template <typename T, int HD, int ROWS>
+// by its end: one row of it per blockIdx.y.  Which that is follows from the
+// lengths, as in the kernel before, and is found while that one runs; then one
+// round trip to memory brings statistics and values together (the first PRE
+// partials of a group of lanes are fetched before their weights are known).
+template <typename T, int HD, int ROWS, int TP>
 __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams P) {
   constexpr int LANES = HD / 4, GROUPS = AT_JOIN_THREADS / LANES, PRE = 4;
-  __shared__ float2 stat[kAttnMaxCtas];
   __shared__ float4 sums[GROUPS][LANES];
-  pdl_enter();
+  __shared__ int64_t sh[12];
   const int tid = threadIdx.x, r = blockIdx.y, lane = tid % LANES, grp = tid / LANES;
-  const int4* const meta = (const int4*)(P.meta + blockIdx.x * 8);
-  const int4 what = meta[0];
-  const int rows = meta[1].x;
-  const int n = min(what.x, (int)(gridDim.x - blockIdx.x)), row = what.z + r;
-  if (n < 1 || row >= rows) return;
+  // the kernel before waited for everything that these lengths come from
+  const Cut cut = locate<AT_JOIN_THREADS, TP, ROWS>(P, sh, [](const Cut& k) { return k.begin(blockIdx.x + 1) - 1; });
+  __syncthreads();
+  SeqPlan sp;
+  int n = 0, head = 0, row = 0;
+  if ((int64_t)blockIdx.x < cut.ctas && sh[9] >= 0) {
+    const int64_t end = cut.begin(blockIdx.x + 1), off = sh[9];  // the range's last tile
+    sp.load(P, (int)sh[8], TP, ROWS);
+    const int64_t seg = div_small(off, sp.units), from = end - 1 - (off - seg * sp.units);  // its segment's first
+    const int64_t to = from + sp.units - 1;
+    if (from >= cut.begin(blockIdx.x) && to >= end) n = (int)(min(cut.owner(to), cut.ctas - 1) - blockIdx.x + 1);
+    head = (int)div_small(seg, max(sp.tiles, 1));
+    row = (int)(seg - (int64_t)head * sp.tiles) * ROWS + r;
+  }
+  pdl_enter();
+  if (n < 1 || row >= sp.rows || head >= P.c.nkv) return;
   // partial i: slot 1 of this CTA, then slot 0 of the ones behind it
   auto part = [&](int i) { return P.part + ((int64_t)(blockIdx.x + i) * 2 + (i == 0)) * (ROWS * (HD + 2)); };
+  auto stat = [&](int i) { return *(const float2*)(part(i) + ROWS * HD + r * 2); };
   float4 pre[PRE];
+  float pre_m[PRE];
 #pragma unroll
   for (int k = 0; k < PRE; ++k)
-    if (grp + k * GROUPS < n) pre[k] = *(const float4*)(part(grp + k * GROUPS) + r * HD + lane * 4);
-  for (int i = tid; i < n; i += AT_JOIN_THREADS) stat[i] = *(const float2*)(part(i) + ROWS * HD + r * 2);
-  __syncthreads();
-  // every group of 32 lanes finds the same maximum and sum
+    if (grp + k * GROUPS < n) {
+      pre[k] = *(const float4*)(part(grp + k * GROUPS) + r * HD + lane * 4);
+      pre_m[k] = stat(grp + k * GROUPS).x;
+    }
+  // every warp finds the same maximum and sum
   float m = -INFINITY, l = 0.f;
-  for (int i = tid & 31; i < n; i += 32) m = fmaxf(m, stat[i].x);
+  auto join = [&](float m2, float l2) {
+    const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
+    l = l * ex2(m - base) + l2 * ex2(m2 - base);
+    m = M;
+  };
+#pragma unroll 4
+  for (int i = tid & 31; i < n; i += 32) {
+    const float2 s = stat(i);
+    join(s.x, s.y);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 16; o > 0; o >>= 1) join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
   const float base = m == -INFINITY ? 0.f : m;
-  for (int i = tid & 31; i < n; i += 32) l += ex2(stat[i].x - base) * stat[i].y;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](int i, const float4& v) {
-    const float w = ex2(stat[i].x - base);
+  auto add = [&](float m2, const float4& v) {
+    const float w = ex2(m2 - base);
     a.x += w * v.x;
     a.y += w * v.y;
     a.z += w * v.z;
@@ -878,9 +944,9 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
   };
 #pragma unroll
   for (int k = 0; k < PRE; ++k)
-    if (grp + k * GROUPS < n) add(grp + k * GROUPS, pre[k]);
+    if (grp + k * GROUPS < n) add(pre_m[k], pre[k]);
 #pragma unroll 4
-  for (int i = grp + PRE * GROUPS; i < n; i += GROUPS) add(i, *(const float4*)(part(i) + r * HD + lane * 4));
+  for (int i = grp + PRE * GROUPS; i < n; i += GROUPS) add(stat(i).x, *(const float4*)(part(i) + r * HD + lane * 4));
   sums[grp][lane] = a;
   __syncthreads();
   if (grp) return;
@@ -894,7 +960,7 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int qi = row / P.group;
-  char* o = P.out + (int64_t)(what.w + qi) * P.o_tok + (int64_t)(what.y * P.group + row - qi * P.group) * P.o_head;
+  char* o = P.out + (int64_t)(sp.first + qi) * P.o_tok + (int64_t)(head * P.group + row - qi * P.group) * P.o_head;
   if (sizeof(T) == 4 || P.out_f32) {
     ((float4*)o)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   } else if constexpr (sizeof(T) == 2) {
@@ -928,23 +994,22 @@ template <typename T, int HD, int NR>
 int64_t workspace_nr(const PagedAttnParams& p) {
   if (uncut<T, HD, NR>(p)) return 0;
   const int64_t ctas = (int64_t)device_sm_count() * Tile<T, HD, NR>::CTAS;
-  return ctas * (2 * NR * 8 * (HD + 2) * 4 + 32);
+  return ctas * (2 * NR * 8 * (HD + 2) * 4);
 }
 
 template <typename T, int HD, int NR>
 void launch_nr(PagedAttnParams p, cudaStream_t s) {
   using L = Tile<T, HD, NR>;
   const int ctas = device_sm_count() * L::CTAS;
-  check(ctas <= kAttnMaxCtas, E_INTERNAL, "more SMs than the attention join holds");
   const bool cut = !uncut<T, HD, NR>(p);
   p.mul = p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f;
   p.cap2 = p.softcap * 1.4426950408889634f;
-  p.meta = cut ? (int32_t*)(p.part + (int64_t)ctas * 2 * L::ROWS * (HD + 2)) : nullptr;
+  p.group_mul = p.group > 1 ? (uint32_t)((((uint64_t)1 << 32) + p.group - 1) / p.group) : 0;
   ensure_smem_optin((const void*)paged_attn_kernel<T, HD, NR>, L::SMEM);
   launch_k(paged_attn_kernel<T, HD, NR>, dim3(ctas), L::THREADS, L::SMEM, s, 1, p);
   if (cut) {
     const int rows = (int)std::min<int64_t>((int64_t)p.max_rows * p.group, L::ROWS);
-    launch_k(paged_attn_join_kernel<T, HD, L::ROWS>, dim3(ctas, rows), AT_JOIN_THREADS, 0, s, 1, p);
+    launch_k(paged_attn_join_kernel<T, HD, L::ROWS, L::TP>, dim3(ctas, rows), AT_JOIN_THREADS, 0, s, 1, p);
   }
 }
 

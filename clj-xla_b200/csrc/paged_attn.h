@@ -59,14 +59,14 @@ struct Tile {
   // weights as two 16-bit parts or one f32: in the tile's K rows once they are scored, if they fit
   static constexpr int PB = ROWS * TP * 4;
   static constexpr bool P_IN_K = PB <= KB;
-  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 96 + 4 * TP * 8; }
+  static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 160 + 4 * TP * 8; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
     int n = 0;
     while (n < 4 && fixed(n + 1) + (n + 1) * STAGE <= 233472 / ctas - 1024) ++n;
     return n;
   }
   static constexpr int pick() {
-    int ctas = KB > 16384 ? 1 : 2;
+    int ctas = KB > 16384 || NR == 8 ? 1 : 2;  // 64 rows need all registers
     while (ctas > 1 && fit(ctas) < 3) --ctas;
     return ctas;
   }
@@ -165,11 +165,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 template <typename T>
-__device__ __forceinline__ T narrow(float x) {
-  if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
-  else return __float2bfloat16_rn(x);
-}
-template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*(const __half2*)&v);
   else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -226,30 +221,36 @@ struct SeqPlan {
     seq_rows(P.c, b, begin, n);
     make(P, begin, n, seq_len(P.c, b), tile, row_tile);
   }
-  __device__ __forceinline__ int64_t cost(int nkv) const { return (int64_t)units * nkv * tiles; }
+  __device__ __forceinline__ int64_t segments(int nkv) const { return (int64_t)nkv * tiles; }
 };
 
 __device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {  // a >= 0, b > 0
   return (((uint64_t)a | (uint64_t)b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// How `total` tiles are cut: the first `more` CTAs have each + 1 of them, the others each.
+// How the call's `total` slots are cut: the first `more` CTAs have each + 1 of
+// them, the others each.  A slot is a tile; where CTAs have several tiles each,
+// every segment has one slot more in front (extra = 1), for what its beginning and
+// end cost (about a tile: queries in, rows out), or CTAs with many short segments
+// would be the last.
 struct Cut {
   int64_t total, each, more, ctas;
-  __device__ __forceinline__ void make(int64_t tiles) {
-    total = tiles;
+  int extra;
+  __device__ __forceinline__ void make(int64_t tiles, int64_t segments) {
+    extra = tiles > 2 * (int64_t)gridDim.x ? 1 : 0;
+    total = tiles + extra * segments;
     ctas = min((int64_t)gridDim.x, total);
     each = ctas ? div_small(total, ctas) : 0;
     more = total - each * ctas;
   }
   __device__ __forceinline__ int64_t begin(int64_t cta) const { return each * cta + min(cta, more); }
-  __device__ __forceinline__ int64_t owner(int64_t tile) const {
+  __device__ __forceinline__ int64_t owner(int64_t slot) const {
     const int64_t edge = more * (each + 1);
-    return tile < edge ? div_small(tile, each + 1) : more + div_small(tile - edge, each);
+    return slot < edge ? div_small(slot, each + 1) : more + div_small(slot - edge, each);
   }
 };
 
-// Cuts the call's tiles and finds the sequence that holds the one `pick` names
+// Cuts the call's slots and finds the sequence that holds the one `pick` names
 // (of the cut), and its place there: sh[8], sh[9] (-1: none was found, which takes
 // lengths that change under the kernel).  By all THREADS threads of a CTA; the
 // results are for use after the next barrier.
@@ -260,41 +261,54 @@ __device__ __forceinline__ Cut locate(const PagedAttnParams& P, int64_t* sh, F p
   const int per = (c.num_seqs + THREADS - 1) / THREADS;
   const int b0 = min(tid * per, c.num_seqs), b1 = min(b0 + per, c.num_seqs);
   SeqPlan sp;
-  int64_t mine = 0;
+  int64_t tiles = 0, segments = 0;  // of this thread's sequences
   for (int i = b0; i < b1; ++i) {
     sp.load(P, i, TP, ROWS);
-    mine += sp.cost(c.nkv);
+    segments += sp.segments(c.nkv);
+    tiles += sp.segments(c.nkv) * sp.units;
   }
-  int64_t incl = mine;
+  int64_t tiles_to = tiles, segments_to = segments;  // up to and with them
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    const int64_t t = __shfl_up_sync(0xffffffffu, tiles_to, o), s = __shfl_up_sync(0xffffffffu, segments_to, o);
+    if (lane >= o) {
+      tiles_to += t;
+      segments_to += s;
+    }
   }
-  if (lane == 31) sh[warp] = incl;
+  if (lane == 31) {
+    sh[warp] = tiles_to;
+    sh[10 + warp] = segments_to;
+  }
   if (tid == 0) {
     sh[8] = 0;
     sh[9] = -1;
   }
   __syncthreads();
-  int64_t total = 0;
+  int64_t all_tiles = 0, all_segments = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) incl += sh[w];
-    total += sh[w];
+    if (w < warp) {
+      tiles_to += sh[w];
+      segments_to += sh[10 + w];
+    }
+    all_tiles += sh[w];
+    all_segments += sh[10 + w];
   }
   Cut cut;
-  cut.make(total);
+  cut.make(all_tiles, all_segments);
   const int64_t want = pick(cut);
-  int64_t excl = incl - mine;
+  const int64_t incl = tiles_to + cut.extra * segments_to;
+  int64_t excl = incl - tiles - cut.extra * segments;
   if (want >= excl && want < incl) {
     for (int i = b0; i < b1; ++i) {
       if (per > 1) sp.load(P, i, TP, ROWS);
-      if (want < excl + sp.cost(c.nkv)) {
+      const int64_t slots = sp.segments(c.nkv) * (sp.units + cut.extra);
+      if (want < excl + slots) {
         sh[8] = i;
         sh[9] = want - excl;
         break;
       }
-      excl += sp.cost(c.nkv);
+      excl += slots;
     }
   }
   return cut;
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   float* const wsum = wmax + 4 * ROWS;
   TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
   int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
-  const char** const rows = (const char**)(sh + 12);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
+  const char** const rows = (const char**)(sh + 20);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedView& c = P.c;
@@ -344,8 +358,8 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
   constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
   const int my_row = lane / LANES, my_chunk = lane % LANES;
-  volatile int* const plan = (volatile int*)(sh + 10);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
-  constexpr int ALL_THERE = 256, DONE = -1, BROKEN = -2;
+  volatile int* const plan = (volatile int*)(sh + 18);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
+  constexpr int ALL_THERE = 256, DONE = -1, NOTHING = -2;
   // Producers: before the next tile's stage is waited for, the oldest tile in
   // flight is handed to the consumers.
   auto hand_over = [&](int tile) {
@@ -371,7 +385,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       bar_sync<AHEAD_THREADS>(AHEAD);  // the tile's rows are listed and its stage is free, or all is done
       const int what = plan[tile & 1];
       if (what < 0) {
-        if (what == BROKEN) bar_arrive<AT_THREADS>(FULL);
+        if (what == NOTHING) bar_arrive<AT_THREADS>(FULL);
         drain(tile);
         return;
       }
@@ -425,8 +439,9 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     SeqPlan sp;
     sp.load(P, b, TP, ROWS);
     const int64_t off = sh[9];
-    if (off < 0 || off >= sp.cost(c.nkv)) left = 0;  // lengths that change under the kernel: stay in bounds
-    int seg = left ? (int)div_small(off, sp.units) : 0, at = left ? (int)(off - (int64_t)seg * sp.units) : 0, qslot = -1;
+    if (off < 0 || off >= sp.segments(c.nkv) * (sp.units + cut.extra)) left = 0;  // lengths that change under the kernel
+    const int seg = left ? (int)div_small(off, sp.units + cut.extra) : 0;
+    int at = left ? (int)(off - (int64_t)seg * (sp.units + cut.extra)) - cut.extra : 0, qslot = -1;  // -1: the slot in front
     int head = sp.tiles ? seg / sp.tiles : 0, row_tile = seg - head * sp.tiles;
     bool fresh = true;    // the next tile is the first of its piece
     bool piece0 = false;  // whether the piece starts its segment
@@ -440,7 +455,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     auto next = [&](Look& k) -> bool {  // the cursor's next tile; starts its page lookup
       if (left == 0) return false;
       if (at >= sp.units) {
-        at = 0;
+        at = -cut.extra;
         fresh = true;
         if (++row_tile >= sp.tiles) {
           row_tile = 0;
@@ -456,6 +471,10 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
             } while (sp.tiles == 0);
           }
         }
+      }
+      if (at < 0) {
+        at = 0;
+        if (--left == 0) return false;
       }
       if (fresh) {
         qslot = qslot + 1 == NST ? 0 : qslot + 1;
@@ -499,10 +518,10 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     int tile = 0;
     Look now, then;
     bool have = next(now);
-    if (!have) {  // only if lengths change under the kernel: a tile of nothing ends the consumers
+    if (!have) {  // a range of one slot in front of a segment: a tile of nothing ends the consumers
       if (lane == 0) {
         *(TileDesc*)desc = TileDesc{0, 0, 0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
-        plan[0] = BROKEN;
+        plan[0] = NOTHING;
       }
       bar_arrive<AT_THREADS>(FULL);
       bar_arrive<AHEAD_THREADS>(AHEAD);
@@ -566,7 +585,8 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   constexpr int PROW = TP * (L::ES == 2 ? 2 : 4);   // bytes of a row of weights
   constexpr int QK = HD / 32;                       // steps of 32 of head_dim
   float acc[MT][NR][4], m[NR][2], l[NR][2];
-  uint32_t qf[NR == 1 && L::ES == 2 ? QK : 1][4];   // the queries, where they fit registers
+  constexpr bool Q_REGS = L::ES == 2 && (NR == 1 || (NR == 2 && L::CTAS == 1));
+  uint32_t qf[Q_REGS ? QK : 1][Q_REGS ? NR : 1][4];  // the queries, where they fit registers
   const int g = lane >> 2, t4 = lane & 3;           // this thread's positions and columns: g, g + 8; its rows: 2 t4, 2 t4 + 1
   for (int tile = 0;; ++tile) {
     const int slot = tile % NST;
@@ -577,6 +597,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     const uint32_t ks = smem_u32(stage), vs = ks + L::KB, qs = smem_u32(queries);
     unsigned char* const pw = L::P_IN_K ? stage : p_own;
     const uint64_t vis = TP == 64 ? (uint64_t)d.mask[1] << 32 | d.mask[0] : d.mask[0];
+    const auto act = [&](int n) { return NR == 1 || NR == 8 || n * 8 < d.nrows; };  // whether any of 8 rows is there (8: no registers to ask)
     const bool plain = (d.flags & T_FULL) && vis == (TP == 64 ? ~0ull : 0xffffffffull);
     // 8 query rows x 32 of head_dim: the second operands of two steps
     const uint32_t qa = qs + (lane & 7) * RB + swz<CPR>(lane >> 3, lane & 7) * 16;
@@ -588,9 +609,11 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
       }
-      if constexpr (NR == 1 && L::ES == 2) {
+      if constexpr (Q_REGS) {
 #pragma unroll
-        for (int j = 0; j < QK; ++j) ldsm4(qa ^ (j * 64), qf[j]);
+        for (int j = 0; j < QK; ++j)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) ldsm4((qa ^ (j * 64)) + n * 8 * RB, qf[j][n]);
       }
     }
 
@@ -614,9 +637,11 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
           ldsm4(ka ^ (j * 64 + 32), k1);
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
+            if (!act(n)) break;
             uint32_t q[4];
-            if constexpr (NR == 1) {
-              q[0] = qf[j][0]; q[1] = qf[j][1]; q[2] = qf[j][2]; q[3] = qf[j][3];
+            if constexpr (Q_REGS) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[e] = qf[j][n][e];
             } else {
               ldsm4((qa ^ (j * 64)) + n * 8 * RB, q);
             }
@@ -642,6 +667,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
           split_tf32(kp[c1 + 8 * HD], ah[3], al[3]);
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
+            if (!act(n)) break;
             uint32_t bh[2], bl[2];
             split_tf32(qp[c0 + n * 8 * HD], bh[0], bl[0]);
             split_tf32(qp[c1 + n * 8 * HD], bh[1], bl[1]);
@@ -665,6 +691,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
+            if (!act(n)) break;
             int jlo, jhi;
             row_view(P, d, n * 8 + 2 * t4 + r, jlo, jhi);
 #pragma unroll
@@ -676,6 +703,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       }
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
+        if (!act(n)) break;
         float2 x = make_float2(fmaxf(s[n][0], s[n][2]), fmaxf(s[n][1], s[n][3]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
@@ -690,6 +718,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     float alpha[NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
+      if (!act(n)) break;
       float2 x = make_float2(m[n][0], m[n][1]);
 #pragma unroll
       for (int w = 0; w < SCORERS; ++w) {
@@ -742,12 +771,17 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       bool odd = false;
       if (!plain && d.count > 1) {
         constexpr int W = CW * L::ES / 16;  // 16-byte chunks of a row that are this warp's
+        auto look = [&](int from, int upto) {
 #pragma unroll 1
-        for (int i = lane; i < d.npos * W; i += 32) {
-          const int j = i / W;
-          const uint4 v = *(const uint4*)(stage + L::KB + j * RB + swz_v<T, CPR>(warp * W + i % W, j) * 16);
-          odd = odd || odd_chunk<T>(v);
-        }
+          for (int i = max(from, 0) * W + lane; i < min(upto, d.npos) * W; i += 32) {
+            const int j = i / W;
+            const uint4 v = *(const uint4*)(stage + L::KB + j * RB + swz_v<T, CPR>(warp * W + i % W, j) * 16);
+            odd = odd || odd_chunk<T>(v);
+          }
+        };
+        const int own = d.p0 - d.pos0;  // the first row's position; the later ones see further, and less far back
+        if (P.window >= 0) look(0, (int)max((int64_t)own + d.count - 1 - P.window, (int64_t)0));
+        look(own + 1, own + d.count);
         odd = __any_sync(0xffffffffu, odd);
       }
       if (odd) {
@@ -790,6 +824,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
           uint32_t ph[NR][4], pl[NR][4];
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
+            if (!act(n)) break;
             ldsm4((pa ^ (j * 64)) + n * 8 * PROW, ph[n]);
             ldsm4((pa ^ (j * 64)) + (ROWS + n * 8) * PROW, pl[n]);
           }
@@ -800,9 +835,11 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
               uint32_t v[4];
               ldsm4t((va ^ (i * 32)) + (j * 32 + h * 16) * RB, v);
 #pragma unroll
-              for (int n = 0; n < NR; ++n) mma16<T>(acc[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
+              for (int n = 0; n < NR; ++n)
+                if (act(n)) mma16<T>(acc[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
 #pragma unroll
-              for (int n = 0; n < NR; ++n) mma16<T>(acc[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
+              for (int n = 0; n < NR; ++n)
+                if (act(n)) mma16<T>(acc[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
             }
         }
       } else {
@@ -826,7 +863,8 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
             split_tf32(vp[c0 + 4 * HD], ah[2], al[2]);
             split_tf32(vp[c1 + 4 * HD], ah[3], al[3]);
 #pragma unroll
-            for (int n = 0; n < NR; ++n) mma_f32(acc[i][n], ah, al, bh[n], bl[n]);
+            for (int n = 0; n < NR; ++n)
+              if (act(n)) mma_f32(acc[i][n], ah, al, bh[n], bl[n]);
           }
         }
       }
@@ -838,6 +876,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       if (SCORERS == 4 || warp < SCORERS) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
+          if (!act(n)) break;
           float2 x = make_float2(l[n][0], l[n][1]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
@@ -850,32 +889,40 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       bar_sync<AT_CONSUMERS>(INNER);
       const bool from0 = d.flags & T_FROM0, whole = from0 && (d.flags & T_TOEND);
       float* const part = P.part + ((int64_t)blockIdx.x * 2 + (from0 ? 1 : 0)) * (ROWS * (HD + 2));
+      // neighbours in g swap a row, so that a thread has two columns of one row to
+      // store: row 8 n + 2 t4 + g % 2, columns g - g % 2 and the next
+      const int odd_g = g & 1;
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
+      for (int n = 0; n < NR; ++n) {
+        if (!act(n)) break;
+        const int in_tile = n * 8 + 2 * t4 + odd_g;
+        const bool mine = in_tile < d.nrows;
+        float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int in_tile = n * 8 + 2 * t4 + r;
-          if (in_tile >= d.nrows) continue;
-          float sum = 0.f;
+        for (int w = 0; w < SCORERS; ++w) sum += wsum[w * ROWS + in_tile];
+        if (mine && !whole && warp == 0 && g < 2)
+          *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(odd_g ? m[n][1] : m[n][0], sum);
+        if (ADDERS < 4 && warp >= ADDERS) continue;
+        const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
+        const int dq = div_group(P, in_tile + d.g0);
+        const bool wide = !whole || L::ES == 4 || P.out_f32;
+        char* const o = whole ? P.out + (int64_t)(d.first + d.q0 + dq) * P.o_tok +
+                                    (int64_t)(d.head * P.group + in_tile + d.g0 - dq * P.group) * P.o_head
+                              : (char*)(part + in_tile * HD);
 #pragma unroll
-          for (int w = 0; w < SCORERS; ++w) sum += wsum[w * ROWS + in_tile];
-          if (warp == 0 && g == 0 && !whole) *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(m[n][r], sum);
-          if (ADDERS < 4 && warp >= ADDERS) continue;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
-          const int dq = div_group(P, in_tile + d.g0);
-          char* const o = P.out + (int64_t)(d.first + d.q0 + dq) * P.o_tok +
-                          (int64_t)(d.head * P.group + in_tile + d.g0 - dq * P.group) * P.o_head;
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int col = warp * CW + i * 16 + g + h * 8;
-              const float x = acc[i][n][h * 2 + r];
-              if (!whole) part[in_tile * HD + col] = x;
-              else if (L::ES == 4 || P.out_f32) ((float*)o)[col] = x * inv;
-              else if constexpr (L::ES == 2) ((T*)o)[col] = narrow<T>(x * inv);
-            }
-        }
+          for (int h = 0; h < 2; ++h) {
+            const float a0 = acc[i][n][h * 2], a1 = acc[i][n][h * 2 + 1];
+            const float keep = odd_g ? a1 : a0, give = odd_g ? a0 : a1;
+            const float got = __shfl_xor_sync(0xffffffffu, give, 4);
+            const float x = (odd_g ? got : keep) * scale, y = (odd_g ? keep : got) * scale;
+            const int col = warp * CW + i * 16 + h * 8 + g - odd_g;
+            if (!mine) continue;
+            if (wide) *(float2*)(o + col * 4) = make_float2(x, y);
+            else if constexpr (L::ES == 2) *(uint32_t*)(o + col * 2) = pack2<T>(x, y);
+          }
+      }
     }
     if (d.flags & T_END) break;
   }
@@ -890,7 +937,7 @@ template <typename T, int HD, int ROWS, int TP>
 __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams P) {
   constexpr int LANES = HD / 4, GROUPS = AT_JOIN_THREADS / LANES, PRE = 4;
   __shared__ float4 sums[GROUPS][LANES];
-  __shared__ int64_t sh[12];
+  __shared__ int64_t sh[20];
   const int tid = threadIdx.x, r = blockIdx.y, lane = tid % LANES, grp = tid / LANES;
   // the kernel before waited for everything that these lengths come from
   const Cut cut = locate<AT_JOIN_THREADS, TP, ROWS>(P, sh, [](const Cut& k) { return k.begin(blockIdx.x + 1) - 1; });
@@ -898,11 +945,13 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
   SeqPlan sp;
   int n = 0, head = 0, row = 0;
   if ((int64_t)blockIdx.x < cut.ctas && sh[9] >= 0) {
-    const int64_t end = cut.begin(blockIdx.x + 1), off = sh[9];  // the range's last tile
+    const int64_t end = cut.begin(blockIdx.x + 1), off = sh[9];  // the range's last slot
     sp.load(P, (int)sh[8], TP, ROWS);
-    const int64_t seg = div_small(off, sp.units), from = end - 1 - (off - seg * sp.units);  // its segment's first
-    const int64_t to = from + sp.units - 1;
-    if (from >= cut.begin(blockIdx.x) && to >= end) n = (int)(min(cut.owner(to), cut.ctas - 1) - blockIdx.x + 1);
+    const int slots = sp.units + cut.extra;
+    const int64_t seg = div_small(off, slots), base = end - 1 - (off - seg * slots);  // its segment's first
+    const int64_t from = base + cut.extra, to = base + slots - 1;                   // its first and last tile's
+    if (from >= cut.begin(blockIdx.x) && from < end && to >= end)
+      n = (int)(min(cut.owner(to), cut.ctas - 1) - blockIdx.x + 1);
     head = (int)div_small(seg, max(sp.tiles, 1));
     row = (int)(seg - (int64_t)head * sp.tiles) * ROWS + r;
   }

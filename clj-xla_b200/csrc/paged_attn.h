@@ -20,9 +20,8 @@
 //
 // Tile.  64 positions (32 for f32 rows of 256) of K and V rows go through a ring
 // of stages.  Behind the four consumer warps, a scheduler warp walks the
-// schedule and looks the pages of a tile up one tile ahead, and two copier
-// warps (one warp issues copies for about 3 TB/s over the GPU) gather its K and
-// V rows with 16-byte cp.async (any page size, any strides; positions nobody
+// schedule and looks the pages of a tile up ahead, and two copier warps (one
+// warp issues copies for about 3 TB/s over the GPU) gather its K and V rows with 16-byte cp.async (any page size, any strides; positions nobody
 // sees are filled with zeros and not read).  Products run on mma.sync with the positions
 // (scores) and the columns (P.V) as its 16 rows and 8 query rows as its columns:
 // a decode step has few query rows, so this wastes the least.  Each consumer
@@ -350,22 +349,22 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   int64_t left = cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
   __syncthreads();
 
-  // Stage hand-over: full[s] (producers arrive, consumers wait), empty[s] (consumers
-  // arrive, the scheduler waits); ahead: the producers among themselves.
+  // Stage hand-over: full[s] (copiers arrive, consumers wait), empty[s] (consumers
+  // arrive, the scheduler waits); ahead: scheduler and copiers among themselves.
   constexpr int INNER = 1, AHEAD = 2, FULL = 3, EMPTY = FULL + NST;
-  constexpr int EMPTY_THREADS = AT_CONSUMERS + 32, AHEAD_THREADS = 96;
+  constexpr int FULL_THREADS = AT_CONSUMERS + 64, EMPTY_THREADS = AT_CONSUMERS + 32, AHEAD_THREADS = 96;
   constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
   constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
   constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
   const int my_row = lane / LANES, my_chunk = lane % LANES;
   volatile int* const plan = (volatile int*)(sh + 18);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
   constexpr int ALL_THERE = 256, DONE = -1, NOTHING = -2;
-  // Producers: before the next tile's stage is waited for, the oldest tile in
-  // flight is handed to the consumers.
+  // Copiers: before the next tile is waited for, the oldest one in flight is handed
+  // to the consumers.
   auto hand_over = [&](int tile) {
     if (tile >= NST - 1) {
       cp_wait<NST - 2>();
-      bar_arrive<AT_THREADS>(FULL + (tile + 1) % NST);
+      bar_arrive<FULL_THREADS>(FULL + (tile + 1) % NST);
     }
   };
   auto drain = [&](int tiles) {  // what is left of that after `tiles` tiles
@@ -373,19 +372,19 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       if (tiles - 1 - k < 0) continue;
       if (k == 0) cp_wait<0>();
       else cp_wait<1>();
-      bar_arrive<AT_THREADS>(FULL + (tiles - 1 - k) % NST);
+      bar_arrive<FULL_THREADS>(FULL + (tiles - 1 - k) % NST);
     }
   };
 
   if (warp > AT_CONSUMERS / 32) {
-    // ================================================== copiers: K rows, V rows
+    // ========================================== copiers: K rows; V rows and queries
     const bool is_v = warp == AT_CONSUMERS / 32 + 2;
     for (int tile = 0;; ++tile) {
       hand_over(tile);
       bar_sync<AHEAD_THREADS>(AHEAD);  // the tile's rows are listed and its stage is free, or all is done
       const int what = plan[tile & 1];
       if (what < 0) {
-        if (what == NOTHING) bar_arrive<AT_THREADS>(FULL);
+        if (what == NOTHING) bar_arrive<FULL_THREADS>(FULL);
         drain(tile);
         return;
       }
@@ -423,6 +422,22 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         copy(std::false_type(), v_swz);
       } else {
         copy(std::false_type(), k_swz);
+      }
+      if (is_v) {
+        const TileDesc& d = *(const TileDesc*)((char*)desc + (tile % NST) * 64);
+        if (d.flags & T_FIRST) {  // rows past nrows stay what they are: nothing of them is kept
+          const uint32_t qd = smem_u32(ring + d.qslot * L::STAGE + 2 * L::KB);
+          const char* const base = P.q + (int64_t)(d.first + d.q0) * P.q_tok + (int64_t)(d.head * P.group) * P.q_head;
+          for (int r = my_row; r < d.nrows; r += RPI) {
+            const int dq = div_group(P, r + d.g0);
+            const char* const src = base + dq * P.q_tok + (r + d.g0 - dq * P.group) * P.q_head;
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) {
+              const int ch = my_chunk + e * LANES;
+              cp16(qd + r * RB + swz<CPR>(ch, r) * 16, src + ch * 16, 16);
+            }
+          }
+        }
       }
       cp_commit();
     }
@@ -523,23 +538,22 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         *(TileDesc*)desc = TileDesc{0, 0, 0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
         plan[0] = NOTHING;
       }
-      bar_arrive<AT_THREADS>(FULL);
       bar_arrive<AHEAD_THREADS>(AHEAD);
       return;
     }
     while (have) {
       have = next(then);
-      hand_over(tile);
       const int slot = tile % NST;
       TileDesc& nd = now.d;
       if (!have) nd.flags |= T_END;
       bool all = true;
+      const char *const kh = c.k + nd.head * c.k_head, *const vh = c.v + nd.head * c.v_head;
 #pragma unroll
       for (int i = 0; i < TP / 32; ++i) {
         const bool ok = (unsigned)now.page[i] < (unsigned)c.num_pages;
         const char** const to = rows + (tile & 1) * 2 * TP + i * 32 + lane;
-        to[0] = ok ? c.k + now.page[i] * c.k_page + nd.head * c.k_head + now.in_page[i] * c.k_row : nullptr;
-        to[TP] = ok ? c.v + now.page[i] * c.v_page + nd.head * c.v_head + now.in_page[i] * c.v_row : nullptr;
+        to[0] = ok ? kh + now.page[i] * c.k_page + now.in_page[i] * c.k_row : nullptr;
+        to[TP] = ok ? vh + now.page[i] * c.v_page + now.in_page[i] * c.v_row : nullptr;
         nd.mask[i] = __ballot_sync(0xffffffffu, ok);
         all = all && nd.mask[i] == 0xffffffffu;
       }
@@ -550,30 +564,11 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         plan[tile & 1] = all ? TP | ALL_THERE : min((nd.npos + 31) & ~31, TP);
       }
       bar_sync<AHEAD_THREADS>(AHEAD);
-      if (nd.flags & T_FIRST) {
-        const uint32_t qd = smem_u32(ring + nd.qslot * L::STAGE + 2 * L::KB);
-        for (int r0 = 0; r0 < ROWS; r0 += RPI) {
-          const int r = r0 + my_row;
-          const bool ok = r < nd.nrows;
-          const int dq = div_group(P, r + nd.g0);
-          const char* src = ok ? P.q + (int64_t)(nd.first + nd.q0 + dq) * P.q_tok +
-                                     (int64_t)(nd.head * P.group + r + nd.g0 - dq * P.group) * P.q_head
-                               : P.q;
-#pragma unroll
-          for (int e = 0; e < CPL; ++e) {
-            const int ch = my_chunk + e * LANES;
-            cp16(qd + r * RB + swz<CPR>(ch, r) * 16, src + (ok ? ch * 16 : 0), ok ? 16 : 0);
-          }
-        }
-      }
-      cp_commit();
       now = then;
       ++tile;
     }
     if (lane == 0) plan[tile & 1] = DONE;
-    hand_over(tile);
     bar_arrive<AHEAD_THREADS>(AHEAD);
-    drain(tile);
     for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<EMPTY_THREADS>(EMPTY + k % NST);  // no arrival is left over
     return;
   }
@@ -590,7 +585,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   const int g = lane >> 2, t4 = lane & 3;           // this thread's positions and columns: g, g + 8; its rows: 2 t4, 2 t4 + 1
   for (int tile = 0;; ++tile) {
     const int slot = tile % NST;
-    bar_sync<AT_THREADS>(FULL + slot);
+    bar_sync<FULL_THREADS>(FULL + slot);
     const TileDesc d = *(const TileDesc*)((char*)desc + slot * 64);
     unsigned char* const stage = ring + slot * L::STAGE;
     unsigned char* const queries = ring + d.qslot * L::STAGE + 2 * L::KB;

@@ -228,16 +228,18 @@ __device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {  // a >= 0,
 }
 
 // How the call's `total` slots are cut: the first `more` CTAs have each + 1 of
-// them, the others each.  A slot is a tile; where CTAs have several tiles each,
-// every segment has one slot more in front (extra = 1), for what its beginning and
-// end cost (about a tile: queries in, rows out), or CTAs with many short segments
-// would be the last.
+// them, the others each.  Where CTAs have several tiles each, a tile is two slots
+// (`scale`) and every segment has one more in front (`extra`) for what its
+// beginning and end cost (queries in, rows out: 0.5 to 0.7 us, a tile 1 to 1.4), or
+// CTAs with many short segments would be the last; else a tile is one slot.  A tile
+// belongs to the CTA that has its first slot.
 struct Cut {
   int64_t total, each, more, ctas;
-  int extra;
+  int extra, scale;
   __device__ __forceinline__ void make(int64_t tiles, int64_t segments) {
     extra = tiles > 2 * (int64_t)gridDim.x ? 1 : 0;
-    total = tiles + extra * segments;
+    scale = 1 + extra;
+    total = scale * tiles + extra * segments;
     ctas = min((int64_t)gridDim.x, total);
     each = ctas ? div_small(total, ctas) : 0;
     more = total - each * ctas;
@@ -247,6 +249,7 @@ struct Cut {
     const int64_t edge = more * (each + 1);
     return slot < edge ? div_small(slot, each + 1) : more + div_small(slot - edge, each);
   }
+  __device__ __forceinline__ int64_t slots(int64_t units) const { return scale * units + extra; }  // of a segment
 };
 
 // Cuts the call's slots and finds the sequence that holds the one `pick` names
@@ -296,12 +299,12 @@ __device__ __forceinline__ Cut locate(const PagedAttnParams& P, int64_t* sh, F p
   Cut cut;
   cut.make(all_tiles, all_segments);
   const int64_t want = pick(cut);
-  const int64_t incl = tiles_to + cut.extra * segments_to;
-  int64_t excl = incl - tiles - cut.extra * segments;
+  const int64_t incl = cut.scale * tiles_to + cut.extra * segments_to;
+  int64_t excl = incl - cut.scale * tiles - cut.extra * segments;
   if (want >= excl && want < incl) {
     for (int i = b0; i < b1; ++i) {
       if (per > 1) sp.load(P, i, TP, ROWS);
-      const int64_t slots = sp.segments(c.nkv) * (sp.units + cut.extra);
+      const int64_t slots = sp.segments(c.nkv) * cut.slots(sp.units);
       if (want < excl + slots) {
         sh[8] = i;
         sh[9] = want - excl;
@@ -454,9 +457,17 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     SeqPlan sp;
     sp.load(P, b, TP, ROWS);
     const int64_t off = sh[9];
-    if (off < 0 || off >= sp.segments(c.nkv) * (sp.units + cut.extra)) left = 0;  // lengths that change under the kernel
-    const int seg = left ? (int)div_small(off, sp.units + cut.extra) : 0;
-    int at = left ? (int)(off - (int64_t)seg * (sp.units + cut.extra)) - cut.extra : 0, qslot = -1;  // -1: the slot in front
+    if (off < 0 || off >= sp.segments(c.nkv) * cut.slots(sp.units)) left = 0;  // lengths that change under the kernel
+    int seg = 0, at = 0, qslot = -1;
+    if (left) {
+      seg = (int)div_small(off, cut.slots(sp.units));
+      const int64_t in = off - seg * cut.slots(sp.units) - cut.extra;  // -1: the slot in front
+      at = in < 0 ? -1 : (int)in / cut.scale;
+      if (in > 0 && in % cut.scale) {  // the middle of a tile that the CTA before has
+        ++at;
+        --left;
+      }
+    }
     int head = sp.tiles ? seg / sp.tiles : 0, row_tile = seg - head * sp.tiles;
     bool fresh = true;    // the next tile is the first of its piece
     bool piece0 = false;  // whether the piece starts its segment
@@ -468,7 +479,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     };
     peek();
     auto next = [&](Look& k) -> bool {  // the cursor's next tile; starts its page lookup
-      if (left == 0) return false;
+      if (left <= 0) return false;
       if (at >= sp.units) {
         at = -cut.extra;
         fresh = true;
@@ -489,7 +500,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       }
       if (at < 0) {
         at = 0;
-        if (--left == 0) return false;
+        if (--left <= 0) return false;
       }
       if (fresh) {
         qslot = qslot + 1 == NST ? 0 : qslot + 1;
@@ -509,9 +520,9 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       d.p0 = sp.p0;
       d.flags = (fresh ? T_FIRST : 0) | (piece0 ? T_FROM0 : 0);
       ++at;
-      --left;
+      left -= cut.scale;
       if (at == sp.units) d.flags |= T_LAST | T_TOEND;
-      if (left == 0) d.flags |= T_LAST;
+      if (left <= 0) d.flags |= T_LAST;
       // every row sees every position, were all pages there
       if (d.npos == TP && d.pos0 + TP - 1 <= d.p0 && (P.window < 0 || d.pos0 >= d.p0 + d.count - 1 - P.window))
         d.flags |= T_FULL;
@@ -533,7 +544,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
     int tile = 0;
     Look now, then;
     bool have = next(now);
-    if (!have) {  // a range of one slot in front of a segment: a tile of nothing ends the consumers
+    if (!have) {  // no tile's first slot is in the range: a tile of nothing ends the consumers
       if (lane == 0) {
         *(TileDesc*)desc = TileDesc{0, 0, 0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
         plan[0] = NOTHING;
@@ -898,7 +909,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
         if (mine && !whole && warp == 0 && g < 2)
           *(float2*)(part + ROWS * HD + in_tile * 2) = make_float2(odd_g ? m[n][1] : m[n][0], sum);
         if (ADDERS < 4 && warp >= ADDERS) continue;
-        const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // no position seen: zeros; a NaN stays one
+        const float scale = !whole ? 1.f : sum == 0.f ? 0.f : __fdividef(1.f, sum);  // no position seen: zeros; a NaN stays one
         const int dq = div_group(P, in_tile + d.g0);
         const bool wide = !whole || L::ES == 4 || P.out_f32;
         char* const o = whole ? P.out + (int64_t)(d.first + d.q0 + dq) * P.o_tok +
@@ -942,9 +953,8 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
   if ((int64_t)blockIdx.x < cut.ctas && sh[9] >= 0) {
     const int64_t end = cut.begin(blockIdx.x + 1), off = sh[9];  // the range's last slot
     sp.load(P, (int)sh[8], TP, ROWS);
-    const int slots = sp.units + cut.extra;
-    const int64_t seg = div_small(off, slots), base = end - 1 - (off - seg * slots);  // its segment's first
-    const int64_t from = base + cut.extra, to = base + slots - 1;                   // its first and last tile's
+    const int64_t slots = cut.slots(sp.units), seg = div_small(off, slots), base = end - 1 - (off - seg * slots);
+    const int64_t from = base + cut.extra, to = base + slots - cut.scale;  // its first and last tile's first slots
     if (from >= cut.begin(blockIdx.x) && from < end && to >= end)
       n = (int)(min(cut.owner(to), cut.ctas - 1) - blockIdx.x + 1);
     head = (int)div_small(seg, max(sp.tiles, 1));
@@ -1002,7 +1012,7 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
     a.z += v.z;
     a.w += v.w;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
   const int qi = row / P.group;
   char* o = P.out + (int64_t)(sp.first + qi) * P.o_tok + (int64_t)(head * P.group + row - qi * P.group) * P.o_head;
   if (sizeof(T) == 4 || P.out_f32) {

@@ -203,9 +203,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
 
 // The race's best so far: the larger w / e, compared by cross products (a
 // reciprocal per token would cost a third of the exponentials again), or the
-// lower index of equal ones.  Nothing yet: (0, 1, -1).
+// lower index of equal ones.  Nothing yet: (0, 1, 0, -1).
 struct Best {
-  float w, e;
+  float w, e, l;  // l: the token's logit
   int i;
 };
 __device__ __forceinline__ void vd_best(Best& a, const Best& b) {
@@ -218,6 +218,7 @@ __device__ __forceinline__ void vd_best_warp(Best& a) {
     Best b;
     b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
     b.e = __shfl_xor_sync(0xffffffffu, a.e, o);
+    b.l = __shfl_xor_sync(0xffffffffu, a.l, o);
     b.i = __shfl_xor_sync(0xffffffffu, a.i, o);
     vd_best(a, b);
   }
@@ -234,14 +235,15 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t lots = (P.vocab + V - 1) / V, lo = lots * rank / ctas, hi = lots * (rank + 1) / ctas;
-  pdl_enter();
+  // what comes from the caller's tensors is fetched before the wait: the kernel
+  // that this one overlaps has itself waited for whatever wrote them
   int first, count;
   vd_rows(P, b, first, count);
   if (tid == 0) s_taken = max(count - 1, 0);
   const float c = P.inv_t * kLog2e, cd = P.inv_td * kLog2e;
   auto target = [&](int r) { return (const T*)(P.target + (first + r) * P.target_stride); };
   auto draft = [&](int r) { return (const T*)(P.draft + (first + r) * P.draft_stride); };
-  // thread r's draft, with its logits and random number: on their way while the slices are joined
+  // thread r's draft, with its logits and random number
   int x = -1;
   bool valid = false;
   float lx = 0.f, dx = 0.f, ux = 0.f;
@@ -254,6 +256,7 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
     }
     if (!P.greedy) ux = P.uniform[first + tid];
   }
+  pdl_enter();
   // the rows' slices, joined
   for (int i = warp; i < 2 * count; i += WARPS) {
     const int which = i >= count, r = which ? i - count : i;
@@ -288,6 +291,7 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   __syncthreads();
   const int taken = s_taken;
   int token = -1;
+  float token_l = 0.f;
   if (P.greedy) {
     if (count > 0) token = s_arg[taken];
   } else if (count > 0) {
@@ -302,11 +306,11 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
     const bool aligned = (((uintptr_t)e | (uintptr_t)l | (uintptr_t)d) & 15) == 0;
     // the race for w; once more for p in the rare case that w is nothing
     for (int pass = 0; pass < 2 && token < 0; ++pass) {
-      Best best{0.f, 1.f, -1};
+      Best best{0.f, 1.f, 0.f, -1};
       auto race = [&](float lv, float dv, float ev, int64_t v) {
         float w = vd_ex2(fmaf(lv, c, -ref)) * inv;
         if (residual) w -= vd_ex2(fmaf(dv, cd, -refd)) * invd;
-        if (w * best.e > best.w * ev && (int)v != out) best = {w, ev, (int)v};  // a thread's indices ascend
+        if (w * best.e > best.w * ev && (int)v != out) best = {w, ev, lv, (int)v};  // a thread's indices ascend
       };
       if (aligned) {
         uint4 la, da = {}, ln, dn = {};
@@ -350,33 +354,36 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
       if (lane == 0) s_best[warp] = best;
       __syncthreads();
       if (warp == 0) {
-        Best a = lane < WARPS ? s_best[lane] : Best{0.f, 1.f, -1};
+        Best a = lane < WARPS ? s_best[lane] : Best{0.f, 1.f, 0.f, -1};
         vd_best_warp(a);
         if (lane == 0) s_mine[pass] = a;
       }
       cluster.sync();  // the CTAs' best are there
-      Best a{0.f, 1.f, -1};
+      Best a{0.f, 1.f, 0.f, -1};
       if (lane < ctas) a = *cluster.map_shared_rank(&s_mine[pass], lane);
       vd_best_warp(a);
       token = a.i;  // the same in every thread of the cluster
+      token_l = a.l;
       residual = false;
       out = -1;
     }
-    cluster.sync();  // no CTA leaves while its best is read
+    cluster.barrier_arrive();
   }
-  if (rank) return;
-  if (tid < P.max_tokens) {  // at most VD_MAX_ROWS
-    const int t = tid < taken ? x : tid == taken && count > 0 ? token : -1;
-    P.tokens_out[(int64_t)b * P.max_tokens + tid] = t;
-    if (P.logprobs) {
-      if (tid == taken && t >= 0) lx = vd_f(target(tid)[t]);
-      P.logprobs[(int64_t)b * P.max_tokens + tid] = t < 0 ? 0.f : logp(lx, tid);
+  if (rank == 0) {
+    if (tid < P.max_tokens) {  // at most VD_MAX_ROWS
+      const int t = tid < taken ? x : tid == taken && count > 0 ? token : -1;
+      P.tokens_out[(int64_t)b * P.max_tokens + tid] = t;
+      if (P.logprobs) {
+        if (tid == taken && t >= 0) lx = P.greedy ? s_max[0][taken] : token_l;
+        P.logprobs[(int64_t)b * P.max_tokens + tid] = t < 0 ? 0.f : logp(lx, tid);
+      }
+    }
+    if (tid == 0) {
+      P.accepted[b] = taken;
+      if (P.new_lens) P.new_lens[b] = P.seq_lens[b] - max(count - 1 - taken, 0);
     }
   }
-  if (tid == 0) {
-    P.accepted[b] = taken;
-    if (P.new_lens) P.new_lens[b] = P.seq_lens[b] - max(count - 1 - taken, 0);
-  }
+  if (!P.greedy && count > 0) cluster.barrier_wait();  // no CTA leaves while its best is read
 }
 
 template <typename T>

@@ -45,19 +45,24 @@ namespace {
 constexpr int AT_CONSUMERS = 128, AT_JOIN_THREADS = 128;
 
 // ------------------------------------------------------------------ layout
+// floats of a slot of partials: rows, then their (max, sum), to whole 16 bytes
+constexpr int slot_floats(int rows, int hd) { return (rows * (hd + 2) + 3) & ~3; }
+
 template <typename T, int HD, int NR>
 struct Tile {
   static constexpr int ES = sizeof(T);
   static constexpr int RB = HD * ES;            // bytes of a row
   static constexpr int TP = RB > 512 ? 32 : 64; // positions of a tile
-  static constexpr int ROWS = NR * 8;           // query rows
+  static constexpr bool SIMT = NR < 0;          // f32 and up to 4 rows: products on the FMA units, -NR rows
+  static constexpr int ROWS = SIMT ? -NR : NR * 8;  // query rows
   static constexpr int CPR = RB / 16;           // 16-byte chunks of a row
   static constexpr int KB = TP * RB;
   static constexpr int QB = ROWS * RB;
   static constexpr int STAGE = 2 * KB + QB;     // K, V, and the queries of a segment that starts here
-  // weights as two 16-bit parts or one f32: in the tile's K rows once they are scored, if they fit
-  static constexpr int PB = ROWS * TP * 4;
-  static constexpr bool P_IN_K = PB <= KB;
+  // weights as two 16-bit parts or one f32: in the tile's K rows once they are
+  // scored, if they fit (SIMT: they do, and this is the warps' rows at a piece's end)
+  static constexpr int PB = SIMT ? 4 * ROWS * HD * 4 : ROWS * TP * 4;
+  static constexpr bool P_IN_K = !SIMT && PB <= KB;
   static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 160 + 4 * TP * 8; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
     int n = 0;
@@ -74,6 +79,11 @@ struct Tile {
   static constexpr int SMEM = fixed(NST) + NST * STAGE;
   static constexpr int THREADS = AT_CONSUMERS + 96;  // and a scheduler, a copier of K and one of V
   static_assert(NST >= 2, "a ring needs two stages");
+  // Named barriers.  Stage hand-over: full[s] (copiers arrive, consumers wait),
+  // empty[s] (consumers arrive, the scheduler waits); ahead: scheduler and copiers
+  // among themselves; inner: the consumers.
+  static constexpr int INNER = 1, AHEAD = 2, FULL = 3, EMPTY = FULL + NST;
+  static constexpr int FULL_THREADS = AT_CONSUMERS + 64, EMPTY_THREADS = AT_CONSUMERS + 32, AHEAD_THREADS = 96;
 };
 
 // chunk c of row r sits at chunk swz(c, r): the eight rows that a matrix load
@@ -328,263 +338,15 @@ __device__ __forceinline__ void row_view(const PagedAttnParams& P, const TileDes
   jlo = P.window < 0 ? 0 : (int)max((int64_t)pos - P.window - d.pos0, (int64_t)0);
 }
 
+// The consumer warps on mma.sync.
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTAS)
-    paged_attn_kernel(const __grid_constant__ PagedAttnParams P) {
+__device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned char* const ring, unsigned char* const p_own,
+                                            float* const wmax, float* const wsum, const TileDesc* const desc,
+                                            const int warp, const int lane) {
   using L = Tile<T, HD, NR>;
-  constexpr int TP = L::TP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST, AT_THREADS = L::THREADS;
-  extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char* const ring = smem;
-  unsigned char* const p_own = smem + NST * L::STAGE;
-  float* const wmax = (float*)(p_own + (L::P_IN_K ? 0 : L::PB));  // [4][ROWS]
-  float* const wsum = wmax + 4 * ROWS;
-  TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
-  int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
-  const char** const rows = (const char**)(sh + 20);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
-
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const PagedView& c = P.c;
-  pdl_enter();
-
-  // ---- this CTA's range of tiles
-  const Cut cut = locate<AT_THREADS, TP, ROWS>(P, sh, [](const Cut& k) { return k.begin(blockIdx.x); });
-  if ((int64_t)blockIdx.x >= cut.ctas) return;
-  int64_t left = cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
-  __syncthreads();
-
-  // Stage hand-over: full[s] (copiers arrive, consumers wait), empty[s] (consumers
-  // arrive, the scheduler waits); ahead: scheduler and copiers among themselves.
-  constexpr int INNER = 1, AHEAD = 2, FULL = 3, EMPTY = FULL + NST;
-  constexpr int FULL_THREADS = AT_CONSUMERS + 64, EMPTY_THREADS = AT_CONSUMERS + 32, AHEAD_THREADS = 96;
-  constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
-  constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
-  constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
-  const int my_row = lane / LANES, my_chunk = lane % LANES;
-  volatile int* const plan = (volatile int*)(sh + 18);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
-  constexpr int ALL_THERE = 256, DONE = -1, NOTHING = -2;
-  // Copiers: before the next tile is waited for, the oldest one in flight is handed
-  // to the consumers.
-  auto hand_over = [&](int tile) {
-    if (tile >= NST - 1) {
-      cp_wait<NST - 2>();
-      bar_arrive<FULL_THREADS>(FULL + (tile + 1) % NST);
-    }
-  };
-  auto drain = [&](int tiles) {  // what is left of that after `tiles` tiles
-    for (int k = NST - 3; k >= 0; --k) {
-      if (tiles - 1 - k < 0) continue;
-      if (k == 0) cp_wait<0>();
-      else cp_wait<1>();
-      bar_arrive<FULL_THREADS>(FULL + (tiles - 1 - k) % NST);
-    }
-  };
-
-  if (warp > AT_CONSUMERS / 32) {
-    // ========================================== copiers: K rows; V rows and queries
-    const bool is_v = warp == AT_CONSUMERS / 32 + 2;
-    for (int tile = 0;; ++tile) {
-      hand_over(tile);
-      bar_sync<AHEAD_THREADS>(AHEAD);  // the tile's rows are listed and its stage is free, or all is done
-      const int what = plan[tile & 1];
-      if (what < 0) {
-        if (what == NOTHING) bar_arrive<FULL_THREADS>(FULL);
-        drain(tile);
-        return;
-      }
-      const uint32_t dst = smem_u32(ring + (tile % NST) * L::STAGE) + (is_v ? L::KB : 0);
-      const char* const* const of = rows + ((tile & 1) * 2 + is_v) * TP;
-      // eight rows' addresses are fetched before their copies are issued: the
-      // warp's time goes to issue, not to the latency of each row's address
-      constexpr int BATCH = 8;
-      static_assert(TP % (BATCH * RPI) == 0, "whole batches");
-      auto copy = [&](auto all, auto swizzle) {
-        const int n = what & 255;
-#pragma unroll 1
-        for (int r0 = 0; r0 < n; r0 += BATCH * RPI) {
-          const char* o[BATCH];
-#pragma unroll
-          for (int i = 0; i < BATCH; ++i) o[i] = of[r0 + i * RPI + my_row];
-#pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
-            const bool ok = decltype(all)::value || o[i] != nullptr;
-#pragma unroll
-            for (int e = 0; e < CPL; ++e) {
-              const int ch = my_chunk + e * LANES;
-              cp16(dst + (r0 + rr) * RB + swizzle(ch, rr) * 16, ok ? o[i] + ch * 16 : P.q, ok ? 16 : 0);
-            }
-          }
-        }
-      };
-      auto k_swz = [](int ch, int r) { return swz<CPR>(ch, r); };
-      auto v_swz = [](int ch, int r) { return swz_v<T, CPR>(ch, r); };
-      if constexpr (L::ES == 2) {  // the same for both
-        if (what & ALL_THERE) copy(std::true_type(), k_swz);
-        else copy(std::false_type(), k_swz);
-      } else if (is_v) {
-        copy(std::false_type(), v_swz);
-      } else {
-        copy(std::false_type(), k_swz);
-      }
-      if (is_v) {
-        const TileDesc& d = *(const TileDesc*)((char*)desc + (tile % NST) * 64);
-        if (d.flags & T_FIRST) {  // rows past nrows stay what they are: nothing of them is kept
-          const uint32_t qd = smem_u32(ring + d.qslot * L::STAGE + 2 * L::KB);
-          const char* const base = P.q + (int64_t)(d.first + d.q0) * P.q_tok + (int64_t)(d.head * P.group) * P.q_head;
-          for (int r = my_row; r < d.nrows; r += RPI) {
-            const int dq = div_group(P, r + d.g0);
-            const char* const src = base + dq * P.q_tok + (r + d.g0 - dq * P.group) * P.q_head;
-#pragma unroll
-            for (int e = 0; e < CPL; ++e) {
-              const int ch = my_chunk + e * LANES;
-              cp16(qd + r * RB + swz<CPR>(ch, r) * 16, src + ch * 16, 16);
-            }
-          }
-        }
-      }
-      cp_commit();
-    }
-  }
-  if (warp == AT_CONSUMERS / 32) {
-    // =============================================================== scheduler
-    // Two tiles are on their way: one whose pages are known by now, one whose page
-    // numbers have just been asked for; and the sequence behind the cursor's.
-    struct Look {
-      TileDesc d;
-      int page[TP / 32], in_page[TP / 32];
-    };
-    int b = (int)sh[8];  // cursor: sequence, segment of it (head, row tile), tile of that
-    SeqPlan sp;
-    sp.load(P, b, TP, ROWS);
-    const int64_t off = sh[9];
-    if (off < 0 || off >= sp.segments(c.nkv) * cut.slots(sp.units)) left = 0;  // lengths that change under the kernel
-    int seg = 0, at = 0, qslot = -1;
-    if (left) {
-      seg = (int)div_small(off, cut.slots(sp.units));
-      const int64_t in = off - seg * cut.slots(sp.units) - cut.extra;  // -1: the slot in front
-      at = in < 0 ? -1 : (int)in / cut.scale;
-      if (in > 0 && in % cut.scale) {  // the middle of a tile that the CTA before has
-        ++at;
-        --left;
-      }
-    }
-    int head = sp.tiles ? seg / sp.tiles : 0, row_tile = seg - head * sp.tiles;
-    bool fresh = true;    // the next tile is the first of its piece
-    bool piece0 = false;  // whether the piece starts its segment
-    int then_first, then_n, then_len;
-    auto peek = [&]() {  // the sequence after b, asked for early
-      if (b + 1 >= c.num_seqs) return;
-      seq_rows(c, b + 1, then_first, then_n);
-      then_len = seq_len(c, b + 1);
-    };
-    peek();
-    auto next = [&](Look& k) -> bool {  // the cursor's next tile; starts its page lookup
-      if (left <= 0) return false;
-      if (at >= sp.units) {
-        at = -cut.extra;
-        fresh = true;
-        if (++row_tile >= sp.tiles) {
-          row_tile = 0;
-          if (++head >= c.nkv) {
-            head = 0;
-            do {
-              if (++b >= c.num_seqs) {
-                left = 0;
-                return false;
-              }
-              sp.make(P, then_first, then_n, then_len, TP, ROWS);
-              peek();
-            } while (sp.tiles == 0);
-          }
-        }
-      }
-      if (at < 0) {
-        at = 0;
-        if (--left <= 0) return false;
-      }
-      if (fresh) {
-        qslot = qslot + 1 == NST ? 0 : qslot + 1;
-        piece0 = at == 0;
-      }
-      TileDesc& d = k.d;
-      const int row0 = row_tile * ROWS;
-      d.head = head;
-      d.q0 = row0 ? row0 / P.group : 0;
-      d.g0 = row0 - d.q0 * P.group;
-      d.nrows = min(sp.rows - row0, ROWS);
-      d.pos0 = sp.lo + at * TP;
-      d.npos = max(min(TP, sp.hi - d.pos0), 0);
-      d.qslot = qslot;
-      d.first = sp.first;
-      d.count = sp.count;
-      d.p0 = sp.p0;
-      d.flags = (fresh ? T_FIRST : 0) | (piece0 ? T_FROM0 : 0);
-      ++at;
-      left -= cut.scale;
-      if (at == sp.units) d.flags |= T_LAST | T_TOEND;
-      if (left <= 0) d.flags |= T_LAST;
-      // every row sees every position, were all pages there
-      if (d.npos == TP && d.pos0 + TP - 1 <= d.p0 && (P.window < 0 || d.pos0 >= d.p0 + d.count - 1 - P.window))
-        d.flags |= T_FULL;
-      fresh = false;
-#pragma unroll
-      for (int i = 0; i < TP / 32; ++i) {
-        const int j = d.pos0 + i * 32 + lane;
-        k.page[i] = -1;
-        k.in_page[i] = 0;
-        if (i * 32 + lane < d.npos) {
-          const int slot = c.page_shift >= 0 ? j >> c.page_shift : j / c.page_size;
-          k.page[i] = c.table[(int64_t)b * c.table_stride + slot];
-          k.in_page[i] = j - slot * c.page_size;
-        }
-      }
-      return true;
-    };
-
-    int tile = 0;
-    Look now, then;
-    bool have = next(now);
-    if (!have) {  // no tile's first slot is in the range: a tile of nothing ends the consumers
-      if (lane == 0) {
-        *(TileDesc*)desc = TileDesc{0, 0, 0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
-        plan[0] = NOTHING;
-      }
-      bar_arrive<AHEAD_THREADS>(AHEAD);
-      return;
-    }
-    while (have) {
-      have = next(then);
-      const int slot = tile % NST;
-      TileDesc& nd = now.d;
-      if (!have) nd.flags |= T_END;
-      bool all = true;
-      const char *const kh = c.k + nd.head * c.k_head, *const vh = c.v + nd.head * c.v_head;
-#pragma unroll
-      for (int i = 0; i < TP / 32; ++i) {
-        const bool ok = (unsigned)now.page[i] < (unsigned)c.num_pages;
-        const char** const to = rows + (tile & 1) * 2 * TP + i * 32 + lane;
-        to[0] = ok ? kh + now.page[i] * c.k_page + now.in_page[i] * c.k_row : nullptr;
-        to[TP] = ok ? vh + now.page[i] * c.v_page + now.in_page[i] * c.v_row : nullptr;
-        nd.mask[i] = __ballot_sync(0xffffffffu, ok);
-        all = all && nd.mask[i] == 0xffffffffu;
-      }
-      if (tile >= NST) bar_sync<EMPTY_THREADS>(EMPTY + slot);
-      if (lane == 0) {
-        *(TileDesc*)((char*)desc + slot * 64) = nd;
-        // whole halves of 32 rows: what the consumers look at
-        plan[tile & 1] = all ? TP | ALL_THERE : min((nd.npos + 31) & ~31, TP);
-      }
-      bar_sync<AHEAD_THREADS>(AHEAD);
-      now = then;
-      ++tile;
-    }
-    if (lane == 0) plan[tile & 1] = DONE;
-    bar_arrive<AHEAD_THREADS>(AHEAD);
-    for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<EMPTY_THREADS>(EMPTY + k % NST);  // no arrival is left over
-    return;
-  }
-
-  // ================================================================ consumers
+  constexpr int TP = L::TP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST;
+  constexpr int INNER = L::INNER, FULL = L::FULL, EMPTY = L::EMPTY;
+  constexpr int FULL_THREADS = L::FULL_THREADS, EMPTY_THREADS = L::EMPTY_THREADS;
   constexpr int SCORERS = TP / 16;                  // warps that score 16 positions each
   constexpr int CW = HD >= 64 ? HD / 4 : 16;        // columns of P.V of a warp
   constexpr int MT = CW / 16, ADDERS = HD / CW;     // their 16-column tiles; warps that have some
@@ -894,7 +656,7 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
       }
       bar_sync<AT_CONSUMERS>(INNER);
       const bool from0 = d.flags & T_FROM0, whole = from0 && (d.flags & T_TOEND);
-      float* const part = P.part + ((int64_t)blockIdx.x * 2 + (from0 ? 1 : 0)) * (ROWS * (HD + 2));
+      float* const part = P.part + ((int64_t)blockIdx.x * 2 + (from0 ? 1 : 0)) * slot_floats(ROWS, HD);
       // neighbours in g swap a row, so that a thread has two columns of one row to
       // store: row 8 n + 2 t4 + g % 2, columns g - g % 2 and the next
       const int odd_g = g & 1;
@@ -934,6 +696,438 @@ __global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTA
   }
 }
 
+// The consumer warps for f32 and up to four query rows, on the FMA units: a warp
+// has a quarter of a tile's positions to itself, scores (a lane per position and
+// part of head_dim) and weighs them and adds its own P.V (a lane per four columns), and
+// the four warps meet only at the end of a piece.  tf32 products in three terms
+// cost about 1000 instructions a warp and tile whatever the rows, this about 130 per row
+// and 100.
+template <int HD, int NR>
+__device__ __forceinline__ void consume_simt(const PagedAttnParams& P, unsigned char* const ring, unsigned char* const p_own,
+                                             float* const wmax, float* const wsum, const TileDesc* const desc,
+                                             const int warp, const int lane) {
+  using L = Tile<float, HD, NR>;
+  constexpr int TP = L::TP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST;
+  constexpr int WP = TP / 4, HS = 32 / WP;                       // positions of a warp, lanes of a position
+  constexpr int VL = CPR < 32 ? CPR : 32, VG = 32 / VL, VC = CPR / VL;  // lanes of a V row, rows at a time, chunks of a lane
+  const int pos = lane % WP, part = lane / WP, vl = lane % VL, vg = lane / VL;
+  float4 acc[ROWS][VC];
+  float m[ROWS], l[ROWS];
+  for (int tile = 0;; ++tile) {
+    const int slot = tile % NST;
+    bar_sync<L::FULL_THREADS>(L::FULL + slot);
+    const TileDesc d = *(const TileDesc*)((char*)desc + slot * 64);
+    unsigned char* const stage = ring + slot * L::STAGE;
+    const unsigned char* const queries = ring + d.qslot * L::STAGE + 2 * L::KB;
+    const uint64_t vis = TP == 64 ? (uint64_t)d.mask[1] << 32 | d.mask[0] : d.mask[0];
+    const bool plain = (d.flags & T_FULL) && vis == (TP == 64 ? ~0ull : 0xffffffffull);
+    const int mine = min(max(d.npos - warp * WP, 0), WP);  // positions of this warp
+    const int j = warp * WP + pos;
+    if (d.flags & T_FIRST) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < VC; ++i) acc[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    if (mine > 0) {
+      float4 s4[ROWS];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) s4[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int ch = part; ch < CPR; ch += HS) {
+        const float4 k = *(const float4*)(stage + j * RB + swz<CPR>(ch, j) * 16);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const float4 q = *(const float4*)(queries + r * RB + swz<CPR>(ch, r) * 16);
+          s4[r].x += q.x * k.x;
+          s4[r].y += q.y * k.y;
+          s4[r].z += q.z * k.z;
+          s4[r].w += q.w * k.w;
+        }
+      }
+      __syncwarp();  // this warp's K rows are read: the first takes its weights
+      float* const pw = (float*)(stage + warp * WP * RB);
+      bool part_seen = false;  // whether some row sees a position that another does not
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        float s = (s4[r].x + s4[r].y) + (s4[r].z + s4[r].w);
+#pragma unroll
+        for (int o = WP; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        s *= P.mul;
+        if (P.softcap > 0.f) s = P.cap2 * tanh_f(s);
+        bool see = true;
+        if (!plain) {
+          int jlo, jhi;
+          row_view(P, d, r, jlo, jhi);
+          see = j >= jlo && j <= jhi && (vis >> j & 1u);
+          if (!see) s = -INFINITY;
+          part_seen = d.count > 1;
+        }
+        float top = fmaxf(m[r], s);
+#pragma unroll
+        for (int o = WP / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = top == -INFINITY ? 0.f : top;
+        const float alpha = ex2(m[r] - base), p = ex2(s - base);
+        m[r] = top;
+        l[r] = l[r] * alpha + (part == 0 ? p : 0.f);
+        if (part == 0) pw[r * WP + pos] = see ? p : part_seen ? -1.f : 0.f;
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+          acc[r][i].x *= alpha;
+          acc[r][i].y *= alpha;
+          acc[r][i].z *= alpha;
+          acc[r][i].w *= alpha;
+        }
+      }
+      __syncwarp();
+      auto add = [&](auto careful) {
+#pragma unroll 4
+        for (int i0 = 0; i0 < WP; i0 += VG) {
+          const int jj = i0 + vg, row = warp * WP + jj;
+          if (i0 >= mine) break;  // rows from here on may not have been copied
+          float w[ROWS];
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) w[r] = jj < mine ? pw[r * WP + jj] : 0.f;
+#pragma unroll
+          for (int i = 0; i < VC; ++i) {
+            float4 v = *(const float4*)(stage + L::KB + row * RB + swz_v<float, CPR>(vl + i * VL, row) * 16);
+            if (VG > 1 && jj >= mine) v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+              if (decltype(careful)::value && w[r] == -1.f) continue;  // not seen: whatever it holds stays out
+              acc[r][i].x += w[r] * v.x;
+              acc[r][i].y += w[r] * v.y;
+              acc[r][i].z += w[r] * v.z;
+              acc[r][i].w += w[r] * v.w;
+            }
+          }
+        }
+      };
+      if (part_seen) add(std::true_type());
+      else add(std::false_type());
+    }
+    if (!(d.flags & T_END)) bar_arrive<L::EMPTY_THREADS>(L::EMPTY + slot);
+
+    // ---- the piece ends: the warps' rows together, or partials of them
+    if (d.flags & T_LAST) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+        for (int o = WP / 2; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+        if (lane == 0) {
+          wmax[warp * ROWS + r] = m[r];
+          wsum[warp * ROWS + r] = l[r];
+        }
+      }
+      bar_sync<AT_CONSUMERS>(L::INNER);
+      float top[ROWS], sum[ROWS];
+      float4* const rows4 = (float4*)p_own;  // [warp][row][chunk]
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        top[r] = fmaxf(fmaxf(wmax[r], wmax[ROWS + r]), fmaxf(wmax[2 * ROWS + r], wmax[3 * ROWS + r]));
+        const float base = top[r] == -INFINITY ? 0.f : top[r];
+        sum[r] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum[r] += wsum[w * ROWS + r] * ex2(wmax[w * ROWS + r] - base);
+        const float f = ex2(m[r] - base);
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+          float4 a = acc[r][i];
+#pragma unroll
+          for (int o = VL; o < 32; o <<= 1) {
+            a.x += __shfl_xor_sync(0xffffffffu, a.x, o);
+            a.y += __shfl_xor_sync(0xffffffffu, a.y, o);
+            a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
+            a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+          }
+          if (vg == 0) rows4[(warp * ROWS + r) * CPR + vl + i * VL] = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+        }
+      }
+      bar_sync<AT_CONSUMERS>(L::INNER);
+      const bool from0 = d.flags & T_FROM0, whole = from0 && (d.flags & T_TOEND);
+      float* const part_out = P.part + ((int64_t)blockIdx.x * 2 + (from0 ? 1 : 0)) * slot_floats(ROWS, HD);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r >= d.nrows) break;
+        if (!whole && warp == 0 && lane == 0) *(float2*)(part_out + ROWS * HD + r * 2) = make_float2(top[r], sum[r]);
+        const float scale = !whole ? 1.f : sum[r] == 0.f ? 0.f : __fdividef(1.f, sum[r]);  // no position seen: zeros
+        const int dq = div_group(P, r + d.g0);
+        float4* const o = whole ? (float4*)(P.out + (int64_t)(d.first + d.q0 + dq) * P.o_tok +
+                                            (int64_t)(d.head * P.group + r + d.g0 - dq * P.group) * P.o_head)
+                                : (float4*)(part_out + r * HD);
+        for (int ch = warp * 32 + lane; ch < CPR; ch += AT_CONSUMERS) {
+          const float4 a = rows4[r * CPR + ch], b = rows4[(ROWS + r) * CPR + ch], c = rows4[(2 * ROWS + r) * CPR + ch],
+                       e = rows4[(3 * ROWS + r) * CPR + ch];
+          o[ch] = make_float4(((a.x + b.x) + (c.x + e.x)) * scale, ((a.y + b.y) + (c.y + e.y)) * scale,
+                              ((a.z + b.z) + (c.z + e.z)) * scale, ((a.w + b.w) + (c.w + e.w)) * scale);
+        }
+      }
+    }
+    if (d.flags & T_END) break;
+  }
+}
+
+template <typename T, int HD, int NR>
+__global__ void __launch_bounds__(Tile<T, HD, NR>::THREADS, Tile<T, HD, NR>::CTAS)
+    paged_attn_kernel(const __grid_constant__ PagedAttnParams P) {
+  using L = Tile<T, HD, NR>;
+  constexpr int TP = L::TP, ROWS = L::ROWS, RB = L::RB, CPR = L::CPR, NST = L::NST, AT_THREADS = L::THREADS;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char* const ring = smem;
+  unsigned char* const p_own = smem + NST * L::STAGE;
+  float* const wmax = (float*)(p_own + (L::P_IN_K ? 0 : L::PB));  // [4][ROWS]
+  float* const wsum = wmax + 4 * ROWS;
+  TileDesc* const desc = (TileDesc*)(wsum + 4 * ROWS);  // [NST], 64 bytes each
+  int64_t* const sh = (int64_t*)((unsigned char*)desc + NST * 64);
+  const char** const rows = (const char**)(sh + 20);  // [2][K, V][TP] addresses of a tile's rows (null: not there)
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const PagedView& c = P.c;
+  pdl_enter();
+
+  // ---- this CTA's range of tiles
+  const Cut cut = locate<AT_THREADS, TP, ROWS>(P, sh, [](const Cut& k) { return k.begin(blockIdx.x); });
+  if ((int64_t)blockIdx.x >= cut.ctas) return;
+  int64_t left = cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
+  __syncthreads();
+
+  constexpr int AHEAD = L::AHEAD, FULL = L::FULL, EMPTY = L::EMPTY;
+  constexpr int FULL_THREADS = L::FULL_THREADS, EMPTY_THREADS = L::EMPTY_THREADS, AHEAD_THREADS = L::AHEAD_THREADS;
+  constexpr int LANES = CPR < 32 ? CPR : 32;  // lanes of a row
+  constexpr int RPI = 32 / LANES;             // rows of one warp-wide copy
+  constexpr int CPL = CPR / LANES;            // chunks of a row for a lane
+  const int my_row = lane / LANES, my_chunk = lane % LANES;
+  volatile int* const plan = (volatile int*)(sh + 18);  // [2] rows to copy of a tile, + ALL_THERE, or DONE
+  constexpr int ALL_THERE = 256, DONE = -1, NOTHING = -2;
+  // Copiers: before the next tile is waited for, the oldest one in flight is handed
+  // to the consumers.
+  auto hand_over = [&](int tile) {
+    if (tile >= NST - 1) {
+      cp_wait<NST - 2>();
+      bar_arrive<FULL_THREADS>(FULL + (tile + 1) % NST);
+    }
+  };
+  auto drain = [&](int tiles) {  // what is left of that after `tiles` tiles
+    for (int k = NST - 3; k >= 0; --k) {
+      if (tiles - 1 - k < 0) continue;
+      if (k == 0) cp_wait<0>();
+      else cp_wait<1>();
+      bar_arrive<FULL_THREADS>(FULL + (tiles - 1 - k) % NST);
+    }
+  };
+
+  if (warp > AT_CONSUMERS / 32) {
+    // ========================================== copiers: K rows; V rows and queries
+    const bool is_v = warp == AT_CONSUMERS / 32 + 2;
+    for (int tile = 0;; ++tile) {
+      hand_over(tile);
+      bar_sync<AHEAD_THREADS>(AHEAD);  // the tile's rows are listed and its stage is free, or all is done
+      const int what = plan[tile & 1];
+      if (what < 0) {
+        if (what == NOTHING) bar_arrive<FULL_THREADS>(FULL);
+        drain(tile);
+        return;
+      }
+      const uint32_t dst = smem_u32(ring + (tile % NST) * L::STAGE) + (is_v ? L::KB : 0);
+      const char* const* const of = rows + ((tile & 1) * 2 + is_v) * TP;
+      // eight rows' addresses are fetched before their copies are issued: the
+      // warp's time goes to issue, not to the latency of each row's address
+      constexpr int BATCH = 8;
+      static_assert(TP % (BATCH * RPI) == 0, "whole batches");
+      auto copy = [&](auto all, auto swizzle) {
+        const int n = what & 255;
+#pragma unroll 1
+        for (int r0 = 0; r0 < n; r0 += BATCH * RPI) {
+          const char* o[BATCH];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) o[i] = of[r0 + i * RPI + my_row];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int rr = i * RPI + my_row;  // r0 is a multiple of 8: equal swizzles
+            const bool ok = decltype(all)::value || o[i] != nullptr;
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) {
+              const int ch = my_chunk + e * LANES;
+              cp16(dst + (r0 + rr) * RB + swizzle(ch, rr) * 16, ok ? o[i] + ch * 16 : P.q, ok ? 16 : 0);
+            }
+          }
+        }
+      };
+      auto k_swz = [](int ch, int r) { return swz<CPR>(ch, r); };
+      auto v_swz = [](int ch, int r) { return swz_v<T, CPR>(ch, r); };
+      if constexpr (L::ES == 2) {  // the same for both
+        if (what & ALL_THERE) copy(std::true_type(), k_swz);
+        else copy(std::false_type(), k_swz);
+      } else if (is_v) {
+        copy(std::false_type(), v_swz);
+      } else {
+        copy(std::false_type(), k_swz);
+      }
+      if (is_v) {
+        const TileDesc& d = *(const TileDesc*)((char*)desc + (tile % NST) * 64);
+        if (d.flags & T_FIRST) {  // rows past nrows stay what they are: nothing of them is kept
+          const uint32_t qd = smem_u32(ring + d.qslot * L::STAGE + 2 * L::KB);
+          const char* const base = P.q + (int64_t)(d.first + d.q0) * P.q_tok + (int64_t)(d.head * P.group) * P.q_head;
+          for (int r = my_row; r < d.nrows; r += RPI) {
+            const int dq = div_group(P, r + d.g0);
+            const char* const src = base + dq * P.q_tok + (r + d.g0 - dq * P.group) * P.q_head;
+#pragma unroll
+            for (int e = 0; e < CPL; ++e) {
+              const int ch = my_chunk + e * LANES;
+              cp16(qd + r * RB + swz<CPR>(ch, r) * 16, src + ch * 16, 16);
+            }
+          }
+        }
+      }
+      cp_commit();
+    }
+  }
+  if (warp == AT_CONSUMERS / 32) {
+    // =============================================================== scheduler
+    // Two tiles are on their way: one whose pages are known by now, one whose page
+    // numbers have just been asked for; and the sequence behind the cursor's.
+    struct Look {
+      TileDesc d;
+      int page[TP / 32], in_page[TP / 32];
+    };
+    int b = (int)sh[8];  // cursor: sequence, segment of it (head, row tile), tile of that
+    SeqPlan sp;
+    sp.load(P, b, TP, ROWS);
+    const int64_t off = sh[9];
+    if (off < 0 || off >= sp.segments(c.nkv) * cut.slots(sp.units)) left = 0;  // lengths that change under the kernel
+    int seg = 0, at = 0, qslot = -1;
+    if (left) {
+      seg = (int)div_small(off, cut.slots(sp.units));
+      const int64_t in = off - seg * cut.slots(sp.units) - cut.extra;  // -1: the slot in front
+      at = in < 0 ? -1 : (int)in / cut.scale;
+      if (in > 0 && in % cut.scale) {  // the middle of a tile that the CTA before has
+        ++at;
+        --left;
+      }
+    }
+    int head = sp.tiles ? seg / sp.tiles : 0, row_tile = seg - head * sp.tiles;
+    bool fresh = true;    // the next tile is the first of its piece
+    bool piece0 = false;  // whether the piece starts its segment
+    int then_first, then_n, then_len;
+    auto peek = [&]() {  // the sequence after b, asked for early
+      if (b + 1 >= c.num_seqs) return;
+      seq_rows(c, b + 1, then_first, then_n);
+      then_len = seq_len(c, b + 1);
+    };
+    peek();
+    auto next = [&](Look& k) -> bool {  // the cursor's next tile; starts its page lookup
+      if (left <= 0) return false;
+      if (at >= sp.units) {
+        at = -cut.extra;
+        fresh = true;
+        if (++row_tile >= sp.tiles) {
+          row_tile = 0;
+          if (++head >= c.nkv) {
+            head = 0;
+            do {
+              if (++b >= c.num_seqs) {
+                left = 0;
+                return false;
+              }
+              sp.make(P, then_first, then_n, then_len, TP, ROWS);
+              peek();
+            } while (sp.tiles == 0);
+          }
+        }
+      }
+      if (at < 0) {
+        at = 0;
+        if (--left <= 0) return false;
+      }
+      if (fresh) {
+        qslot = qslot + 1 == NST ? 0 : qslot + 1;
+        piece0 = at == 0;
+      }
+      TileDesc& d = k.d;
+      const int row0 = row_tile * ROWS;
+      d.head = head;
+      d.q0 = row0 ? row0 / P.group : 0;
+      d.g0 = row0 - d.q0 * P.group;
+      d.nrows = min(sp.rows - row0, ROWS);
+      d.pos0 = sp.lo + at * TP;
+      d.npos = max(min(TP, sp.hi - d.pos0), 0);
+      d.qslot = qslot;
+      d.first = sp.first;
+      d.count = sp.count;
+      d.p0 = sp.p0;
+      d.flags = (fresh ? T_FIRST : 0) | (piece0 ? T_FROM0 : 0);
+      ++at;
+      left -= cut.scale;
+      if (at == sp.units) d.flags |= T_LAST | T_TOEND;
+      if (left <= 0) d.flags |= T_LAST;
+      // every row sees every position, were all pages there
+      if (d.npos == TP && d.pos0 + TP - 1 <= d.p0 && (P.window < 0 || d.pos0 >= d.p0 + d.count - 1 - P.window))
+        d.flags |= T_FULL;
+      fresh = false;
+#pragma unroll
+      for (int i = 0; i < TP / 32; ++i) {
+        const int j = d.pos0 + i * 32 + lane;
+        k.page[i] = -1;
+        k.in_page[i] = 0;
+        if (i * 32 + lane < d.npos) {
+          const int slot = c.page_shift >= 0 ? j >> c.page_shift : j / c.page_size;
+          k.page[i] = c.table[(int64_t)b * c.table_stride + slot];
+          k.in_page[i] = j - slot * c.page_size;
+        }
+      }
+      return true;
+    };
+
+    int tile = 0;
+    Look now, then;
+    bool have = next(now);
+    if (!have) {  // no tile's first slot is in the range: a tile of nothing ends the consumers
+      if (lane == 0) {
+        *(TileDesc*)desc = TileDesc{0, 0, 0, 0, 0, 0, T_FIRST | T_END, 0, 0, 0, 0, {0u, 0u}};
+        plan[0] = NOTHING;
+      }
+      bar_arrive<AHEAD_THREADS>(AHEAD);
+      return;
+    }
+    while (have) {
+      have = next(then);
+      const int slot = tile % NST;
+      TileDesc& nd = now.d;
+      if (!have) nd.flags |= T_END;
+      bool all = true;
+      const char *const kh = c.k + nd.head * c.k_head, *const vh = c.v + nd.head * c.v_head;
+#pragma unroll
+      for (int i = 0; i < TP / 32; ++i) {
+        const bool ok = (unsigned)now.page[i] < (unsigned)c.num_pages;
+        const char** const to = rows + (tile & 1) * 2 * TP + i * 32 + lane;
+        to[0] = ok ? kh + now.page[i] * c.k_page + now.in_page[i] * c.k_row : nullptr;
+        to[TP] = ok ? vh + now.page[i] * c.v_page + now.in_page[i] * c.v_row : nullptr;
+        nd.mask[i] = __ballot_sync(0xffffffffu, ok);
+        all = all && nd.mask[i] == 0xffffffffu;
+      }
+      if (tile >= NST) bar_sync<EMPTY_THREADS>(EMPTY + slot);
+      if (lane == 0) {
+        *(TileDesc*)((char*)desc + slot * 64) = nd;
+        // whole halves of 32 rows: what the consumers look at
+        plan[tile & 1] = all ? TP | ALL_THERE : min((nd.npos + 31) & ~31, TP);
+      }
+      bar_sync<AHEAD_THREADS>(AHEAD);
+      now = then;
+      ++tile;
+    }
+    if (lane == 0) plan[tile & 1] = DONE;
+    bar_arrive<AHEAD_THREADS>(AHEAD);
+    for (int k = max(tile - NST, 0); k < tile - 1; ++k) bar_sync<EMPTY_THREADS>(EMPTY + k % NST);  // no arrival is left over
+    return;
+  }
+
+  if constexpr (L::SIMT) consume_simt<HD, NR>(P, ring, p_own, wmax, wsum, desc, warp, lane);
+  else consume_mma<T, HD, NR>(P, ring, p_own, wmax, wsum, desc, warp, lane);
+}
+
 // Adds up the partials of the segment that starts in CTA blockIdx.x and is cut
 // by its end: one row of it per blockIdx.y.  Which that is follows from the
 // lengths, as in the kernel before, and is found while that one runs; then one
@@ -963,7 +1157,7 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
   pdl_enter();
   if (n < 1 || row >= sp.rows || head >= P.c.nkv) return;
   // partial i: slot 1 of this CTA, then slot 0 of the ones behind it
-  auto part = [&](int i) { return P.part + ((int64_t)(blockIdx.x + i) * 2 + (i == 0)) * (ROWS * (HD + 2)); };
+  auto part = [&](int i) { return P.part + ((int64_t)(blockIdx.x + i) * 2 + (i == 0)) * slot_floats(ROWS, HD); };
   auto stat = [&](int i) { return *(const float2*)(part(i) + ROWS * HD + r * 2); };
   float4 pre[PRE];
   float pre_m[PRE];
@@ -1026,6 +1220,8 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
 // Row tiles of 8, 16, 32 or 64 rows: the smallest that holds a sequence's rows
 // for one KV head (more rows than 64 take several tiles, each reading K and V
 // again, from L2).  f32 rows of 256 stop at 32: two stages of more do not fit.
+// f32 with at most four rows: 1, 2 or 4 of them on the FMA units (a negative
+// count).
 template <typename T, int HD>
 constexpr int max_nr() {
   return sizeof(T) == 4 && HD == 256 ? 4 : 8;
@@ -1033,6 +1229,7 @@ constexpr int max_nr() {
 template <typename T, int HD>
 int pick_nr(const PagedAttnParams& p) {
   const int64_t rows = (int64_t)p.max_rows * p.group;
+  if (sizeof(T) == 4 && rows <= 4) return rows <= 1 ? -1 : rows <= 2 ? -2 : -4;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 || max_nr<T, HD>() == 4 ? 4 : 8;
 }
 
@@ -1048,7 +1245,7 @@ template <typename T, int HD, int NR>
 int64_t workspace_nr(const PagedAttnParams& p) {
   if (uncut<T, HD, NR>(p)) return 0;
   const int64_t ctas = (int64_t)device_sm_count() * Tile<T, HD, NR>::CTAS;
-  return ctas * (2 * NR * 8 * (HD + 2) * 4);
+  return ctas * 2 * slot_floats(Tile<T, HD, NR>::ROWS, HD) * 4;
 }
 
 template <typename T, int HD, int NR>
@@ -1069,7 +1266,13 @@ void launch_nr(PagedAttnParams p, cudaStream_t s) {
 
 template <typename T, int HD, class F>
 auto with_nr(const PagedAttnParams& p, F f) {
-  switch (pick_nr<T, HD>(p)) {
+  const int nr = pick_nr<T, HD>(p);
+  if constexpr (sizeof(T) == 4) {
+    if (nr == -1) return f(std::integral_constant<int, -1>());
+    if (nr == -2) return f(std::integral_constant<int, -2>());
+    if (nr == -4) return f(std::integral_constant<int, -4>());
+  }
+  switch (nr) {
     case 1: return f(std::integral_constant<int, 1>());
     case 2: return f(std::integral_constant<int, 2>());
     case 4: return f(std::integral_constant<int, 4>());

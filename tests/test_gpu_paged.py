@@ -157,6 +157,17 @@ ATTEND = {
     "f32_hd32_rows64": ([70, 10], [20, 10], 1, 3, 32, 16, "f32", "f32", -1, 0.0),
     "empty_sequences": ([0, 50, 0, 7], [0, 1, 0, 2], 2, 2, 64, 16, "bf16", "f32", -1, 0.0),
     "rows_before_position_0": ([2, 0, 30], [5, 3, 1], 2, 2, 128, 16, "bf16", "f32", -1, 0.0),
+    "f32_1row_hd128": ([300, 65, 1, 64], [1, 1, 1, 1], 2, 1, 128, 16, "f32", "f32", 100, 0.0),
+    "f32_1row_hd256": ([300, 33, 1, 32], [1, 1, 1, 1], 2, 1, 256, 7, "f32", "f32", -1, 30.0),
+    "f32_2rows_hd64": ([900, 65, 2, 64], [2, 1, 2, 2], 2, 1, 64, 16, "f32", "f32", 70, 0.0),
+    "f32_2rows_hd256": ([300, 65, 2, 64], [1, 1, 1, 1], 2, 2, 256, 16, "f32", "f32", -1, 0.0),
+    "f32_3rows_hd32": ([300, 65, 3, 64], [3, 2, 3, 1], 3, 1, 32, 1, "f32", "f32", 20, 0.0),
+    "f32_4rows_hd128": ([700, 65, 2, 64], [2, 1, 2, 2], 3, 2, 128, 16, "f32", "f32", 33, 25.0),
+    "f32_4rows_before_0": ([2, 0, 30, 0], [4, 3, 1, 0], 2, 1, 64, 16, "f32", "f32", -1, 0.0),
+    "long_f32": ([5000, 4097], [1, 2], 2, 2, 64, 16, "f32", "f32", -1, 0.0),
+    "many_pieces": ([1 + (37 * i) % 200 for i in range(90)], [1 + i % 3 if 1 + (37 * i) % 200 > 3 else 1 for i in range(90)],
+                    8, 2, 128, 16, "bf16", "f32", -1, 0.0),
+    "many_pieces_f32": ([1 + (37 * i) % 200 for i in range(90)], [1 for i in range(90)], 8, 2, 64, 16, "f32", "f32", 64, 0.0),
     "long": ([5000, 4097], [1, 2], 2, 2, 128, 16, "bf16", "f32", -1, 0.0),
 }
 
@@ -214,11 +225,14 @@ def test_attend_length_past_the_table(paged):
     check_rows(cache.attend(case.q.cuda(), starts=case.dstarts, max_tokens=1, window=3), want, tol)
 
 
-@pytest.mark.parametrize("hd,dtype", [(32, "bf16"), (64, "f32"), (128, "bf16"), (256, "f16"), (256, "f32")])
+@pytest.mark.parametrize("hd,dtype,group,count", [(32, "bf16", 2, 5), (64, "f32", 2, 5), (128, "bf16", 2, 5),
+                                                  (256, "f16", 2, 5), (256, "f32", 2, 5), (128, "bf16", 1, 2),
+                                                  (256, "bf16", 8, 5), (64, "f32", 1, 2), (128, "f32", 2, 2),
+                                                  (256, "f32", 1, 4), (32, "f32", 1, 3)])
 @pytest.mark.parametrize("bad", [INF, -INF, math.nan])
-def test_attend_unseen_positions_may_hold_anything(paged, hd, dtype, bad):
+def test_attend_unseen_positions_may_hold_anything(paged, hd, dtype, group, count, bad):
     """Page tails, evicted pages, positions before the window, and later drafts."""
-    case = Case([77, 40], [5, 3], 2, 2, hd, 16, dtype, seed=7)
+    case = Case([77, 40], [count, min(3, count)], 2, group, hd, 16, dtype, seed=7)
     case.table[0, 0] = -1
     window = 30
     want, tol = case.attend(hd ** -0.5, 0.0, window)
@@ -230,18 +244,18 @@ def test_attend_unseen_positions_may_hold_anything(paged, hd, dtype, bad):
                 k[p, :, o] = bad
                 v[p, :, o] = bad
     cache = case.cache(paged, k.cuda(), v.cuda())
-    check_rows(cache.attend(case.q.cuda(), starts=case.dstarts, max_tokens=5, window=window), want, tol)
-    # the newest draft of sequence 0 (row 4, position 76) is unseen by rows 0 to 3, and the oldest
-    # position that row 0 sees is unseen by rows 1 to 4
+    check_rows(cache.attend(case.q.cuda(), starts=case.dstarts, max_tokens=count, window=window), want, tol)
+    # the newest draft of sequence 0 (position 76) is unseen by its other rows, and the oldest
+    # position that row 0 sees by the rows behind it
     p, o = case.page_at(0, 76), 76 % 16
-    p2, o2 = case.page_at(0, 72 - 30), (72 - 30) % 16
+    p2, o2 = case.page_at(0, 77 - count - 30), (77 - count - 30) % 16
     k[p, :, o] = bad
     v[p, :, o, 1::2] = bad
     v[p2, :, o2, 3] = bad
     cache = case.cache(paged, k.cuda(), v.cuda())
-    got = cache.attend(case.q.cuda(), starts=case.dstarts, max_tokens=5, window=window)
+    got = cache.attend(case.q.cuda(), starts=case.dstarts, max_tokens=count, window=window)
     w2 = list(want)
-    w2[0] = w2[4] = None
+    w2[0] = w2[count - 1] = None
     check_rows(got, w2, tol)
     g0 = got[0].double().cpu()
     assert not torch.isfinite(g0[:, 3]).any()  # row 0 does see that value

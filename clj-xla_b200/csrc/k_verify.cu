@@ -107,7 +107,8 @@ __device__ __forceinline__ float vd_top(const uint4& v) {
   }
 }
 
-__device__ __forceinline__ void vd_rows(const VerifyParams& P, int b, int& first, int& count) {
+// First row, rows that are looked at and rows of sequence b.
+__device__ __forceinline__ void vd_rows(const VerifyParams& P, int b, int& first, int& count, int& all) {
   if (!P.starts) {
     first = b * P.each;
     count = P.each;
@@ -116,6 +117,7 @@ __device__ __forceinline__ void vd_rows(const VerifyParams& P, int b, int& first
     first = lo;
     count = max(hi - lo, 0);
   }
+  all = count;
   count = min(count, P.max_tokens);
 }
 
@@ -149,8 +151,8 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
   fetch(lo + tid);
   const int b = seq_of_row(P.starts, P.num_seqs, P.each, row);
   if (b < 0) return;
-  int first, count;
-  vd_rows(P, b, first, count);
+  int first, count, all;
+  vd_rows(P, b, first, count, all);
   if (row - first >= count - which) return;  // not looked at; the draft of a sequence's last row is none
   Stat a{-INFINITY, 0.f, -1};
   auto take = [&](float f, int64_t v) {
@@ -237,8 +239,8 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   const int64_t lots = (P.vocab + V - 1) / V, lo = lots * rank / ctas, hi = lots * (rank + 1) / ctas;
   // what comes from the caller's tensors is fetched before the wait: the kernel
   // that this one overlaps has itself waited for whatever wrote them
-  int first, count;
-  vd_rows(P, b, first, count);
+  int first, count, all;
+  vd_rows(P, b, first, count, all);
   if (tid == 0) s_taken = max(count - 1, 0);
   const float c = P.inv_t * kLog2e, cd = P.inv_td * kLog2e;
   auto target = [&](int r) { return (const T*)(P.target + (first + r) * P.target_stride); };
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
     }
     if (tid == 0) {
       P.accepted[b] = taken;
-      if (P.new_lens) P.new_lens[b] = P.seq_lens[b] - max(count - 1 - taken, 0);
+      if (P.new_lens) P.new_lens[b] = P.seq_lens[b] - max(all - 1 - taken, 0);
     }
   }
   if (!P.greedy && count > 0) cluster.barrier_wait();  // no CTA leaves while its best is read

@@ -166,6 +166,8 @@ PagedAttnParams attention_params(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAtt
        "scale must be finite, softcap finite and not negative");
   p.scale = a->scale;
   p.softcap = a->softcap;
+  const float per_cap = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
+  need(per_cap - per_cap == 0.f, "scale / softcap must be finite");
   p.window = a->window < 0 ? -1 : (a->window > kMaxCount ? kMaxCount : a->window);
   const int64_t es = element_size(p.dt), eo = element_size(out_dt);
   need_stride(a->q_token_stride, "q_token_stride out of range");

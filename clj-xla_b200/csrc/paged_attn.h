@@ -59,9 +59,11 @@ struct Tile {
   static constexpr int KB = TP * RB;
   static constexpr int QB = ROWS * RB;
   static constexpr int STAGE = 2 * KB + QB;     // K, V, and the queries of a segment that starts here
-  // weights as two 16-bit parts or one f32: in the tile's K rows once they are
-  // scored, if they fit (SIMT: they do, and this is the warps' rows at a piece's end)
-  static constexpr int PB = SIMT ? 4 * ROWS * HD * 4 : ROWS * TP * 4;
+  // weights as two (bf16: three) 16-bit parts or one f32: in the tile's K rows once
+  // they are scored, if they fit (SIMT: they do, and this is the warps' rows at a
+  // piece's end)
+  static constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+  static constexpr int PB = SIMT ? 4 * ROWS * HD * 4 : ROWS * TP * (ES == 2 ? 2 * PARTS : 4);
   static constexpr bool P_IN_K = !SIMT && PB <= KB;
   static constexpr int fixed(int nst) { return (P_IN_K ? 0 : PB) + 2 * 4 * ROWS * 4 + nst * 64 + 160 + 4 * TP * 8; }
   static constexpr int fit(int ctas) {  // stages that fit with this many CTAs on an SM (228 KB, 1 KB each reserved)
@@ -131,6 +133,9 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void stsm2t(uint32_t addr, uint32_t r0, uint32_t r1) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1,%2};" ::"r"(addr), "r"(r0), "r"(r1) : "memory");
+}
 __device__ __forceinline__ void stsm4t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1),
                "r"(r2), "r"(r3)
@@ -178,14 +183,17 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*(const __half2*)&v);
   else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
-// tanh: from 2^x where that is accurate (1 - 2 / (1 + e^2y) is off by about
-// 2^-23), from its series where that would cancel (|y| < 0.1: the next term is
-// below 2^-32 of the result)
+// tanh.  Below 1: Lambert's continued fraction y / (1 + y^2 / (3 + y^2 / (5 + ...)))
+// to its sixth level, as a quotient (the rest is below 2^-27 of it there); from
+// 1 on 1 - 2 / (1 + e^2y), which would cancel for small y: a capped score times the
+// cap must keep its relative precision.
 __device__ __forceinline__ float tanh_f(float y) {
-  const float big = 1.f - __fdividef(2.f, 1.f + ex2(y * 2.8853900817779268f));
   const float z = y * y;
-  const float small = y * fmaf(z, fmaf(z, fmaf(z, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
-  return fabsf(y) < 0.1f ? small : big;
+  const float num = fmaf(z, fmaf(z, 21.f, 1260.f), 10395.f);
+  const float den = fmaf(z, fmaf(z, z + 210.f, 4725.f), 10395.f);
+  const float low = y * __fdividef(num, den);
+  const float high = 1.f - __fdividef(2.f, 1.f + ex2(y * 2.8853900817779268f));
+  return fabsf(y) < 1.f ? low : high;
 }
 // whether either 16-bit value is an infinity or NaN
 template <typename T>
@@ -355,6 +363,7 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
   float acc[MT][NR][4], m[NR][2], l[NR][2];
   constexpr bool Q_REGS = L::ES == 2 && (NR == 1 || (NR == 2 && L::CTAS == 1));
   uint32_t qf[Q_REGS ? QK : 1][Q_REGS ? NR : 1][4];  // the queries, where they fit registers
+  const bool third = L::PARTS == 3 && P.out_f32;    // a third part of the weights
   const int g = lane >> 2, t4 = lane & 3;           // this thread's positions and columns: g, g + 8; its rows: 2 t4, 2 t4 + 1
   for (int tile = 0;; ++tile) {
     const int slot = tile % NST;
@@ -504,13 +513,19 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
         l[n][0] = l[n][0] * alpha[n][0] + (p0 + p2);
         l[n][1] = l[n][1] * alpha[n][1] + (p1 + p3);
         if constexpr (L::ES == 2) {
-          // hi + lo keep 16 bits (f16: 22) of a weight, so the product with V is
-          // good for an f32 output
+          // Parts of a weight, each what the ones before leave: two keep 22 bits in
+          // f16 and 16 in bf16, enough for its own outputs; an f32 one takes a third.
           const uint32_t h0 = pack2<T>(p0, p1), h1 = pack2<T>(p2, p3);
           const float2 f0 = unpack2<T>(h0), f1 = unpack2<T>(h1);
+          const float q0 = p0 - f0.x, q1 = p1 - f0.y, q2 = p2 - f1.x, q3 = p3 - f1.y;
+          const uint32_t l0 = pack2<T>(q0, q1), l1 = pack2<T>(q2, q3);
           const int row = n * 8 + (lane & 7), ch = warp * 2 + (lane >> 3 & 1);
-          stsm4t(smem_u32(pw) + (lane >> 4) * (ROWS * PROW) + row * PROW + ((ch ^ (row & 7)) * 16), h0, h1,
-                 pack2<T>(p0 - f0.x, p1 - f0.y), pack2<T>(p2 - f1.x, p3 - f1.y));
+          const uint32_t to = smem_u32(pw) + row * PROW + ((ch ^ (row & 7)) * 16);
+          stsm4t(to + (lane >> 4) * (ROWS * PROW), h0, h1, l0, l1);
+          if (third) {
+            const float2 g0 = unpack2<T>(l0), g1 = unpack2<T>(l1);
+            stsm2t(to + 2 * ROWS * PROW, pack2<T>(q0 - g0.x, q1 - g0.y), pack2<T>(q2 - g1.x, q3 - g1.y));
+          }
         } else {
           const float p[4] = {p0, p1, p2, p3};
 #pragma unroll
@@ -525,12 +540,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
 
     // ---- P.V: acc[i][n][e] is of column g + 8 (e / 2) of the warp's i-th 16 and row 8 n + 2 t4 + e % 2
     if (ADDERS == 4 || warp < ADDERS) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][n][e] *= alpha[n][e & 1];
       // A position that some rows see and others do not may hold an infinity or
       // NaN, which a weight of zero does not keep out of a matrix product.  Tiles
       // with row-dependent masks look for such values first; with one of them in
@@ -553,6 +562,12 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
         odd = __any_sync(0xffffffffu, odd);
       }
       if (odd) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][n][e] *= alpha[n][e & 1];
 #pragma unroll 1
         for (int j = 0; j < TP; ++j) {
           if (!(vis >> j & 1u)) continue;
@@ -568,6 +583,7 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
               if constexpr (L::ES == 2) {
                 const unsigned char* at16 = pw + row * PROW + (((j >> 3) ^ (row & 7)) * 16) + (j & 7) * 2;
                 p = (float)*(const T*)at16 + (float)*(const T*)(at16 + ROWS * PROW);
+                if (third) p += (float)*(const T*)(at16 + 2 * ROWS * PROW);
               } else {
                 p = *(const float*)(pw + row * PROW + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4);
               }
@@ -582,58 +598,86 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
                 }
             }
         }
-      } else if constexpr (L::ES == 2) {
+      } else {
+        // A tile's sum is made apart and added with one rounding: the tensor cores
+        // cut their sums off, and over a long context that adds up to 10^-5 of the result.
+        constexpr int IB = MT * NR <= 4 ? MT : 1;  // 16-column tiles at a time, as registers allow
         const uint32_t pa = smem_u32(pw) + (lane & 7) * PROW + (((lane >> 3) ^ (lane & 7)) * 16);
         const int vr = (lane >> 4) * 8 + (lane & 7);
         const uint32_t va = vs + vr * RB + swz_v<T, CPR>(warp * (CW / 8) + (lane >> 3 & 1), vr) * 16;
 #pragma unroll
-        for (int j = 0; j < TP / 32; ++j) {
-          if (j * 32 >= d.npos) break;  // rows from here on were not copied
-          uint32_t ph[NR][4], pl[NR][4];
+        for (int i0 = 0; i0 < MT; i0 += IB) {
+          float t[IB][NR][4];
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            if (!act(n)) break;
-            ldsm4((pa ^ (j * 64)) + n * 8 * PROW, ph[n]);
-            ldsm4((pa ^ (j * 64)) + (ROWS + n * 8) * PROW, pl[n]);
+          for (int i = 0; i < IB; ++i)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) t[i][n][0] = t[i][n][1] = t[i][n][2] = t[i][n][3] = 0.f;
+          if constexpr (L::ES == 2) {
+#pragma unroll
+            for (int j = 0; j < TP / 32; ++j) {
+              if (j * 32 >= d.npos) break;  // rows from here on were not copied
+              uint32_t ph[NR][4], pl[NR][4], pt[L::PARTS == 3 ? NR : 1][4];
+#pragma unroll
+              for (int n = 0; n < NR; ++n) {
+                if (!act(n)) break;
+                ldsm4((pa ^ (j * 64)) + n * 8 * PROW, ph[n]);
+                ldsm4((pa ^ (j * 64)) + (ROWS + n * 8) * PROW, pl[n]);
+                if constexpr (L::PARTS == 3)
+                  if (third) ldsm4((pa ^ (j * 64)) + (2 * ROWS + n * 8) * PROW, pt[n]);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < IB; ++i) {
+                  uint32_t v[4];
+                  ldsm4t((va ^ ((i0 + i) * 32)) + (j * 32 + h * 16) * RB, v);
+#pragma unroll
+                  for (int n = 0; n < NR; ++n)
+                    if (act(n)) mma16<T>(t[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
+#pragma unroll
+                  for (int n = 0; n < NR; ++n)
+                    if (act(n)) mma16<T>(t[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
+                  if constexpr (L::PARTS == 3) {
+                    if (third) {
+#pragma unroll
+                      for (int n = 0; n < NR; ++n)
+                        if (act(n)) mma16<T>(t[i][n], v, pt[n][2 * h], pt[n][2 * h + 1]);
+                    }
+                  }
+                }
+            }
+          } else {
+#pragma unroll 2
+            for (int k = 0; k * 8 < d.npos; ++k) {
+              uint32_t bh[NR][2], bl[NR][2];
+#pragma unroll
+              for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  split_tf32(*(const float*)(pw + (n * 8 + g) * PROW + (((2 * k + h) ^ g) * 16) + t4 * 4), bh[n][h], bl[n][h]);
+              const int r0 = k * 8 + t4;  // and r0 + 4: the same swizzle
+              const float* const vp = (const float*)(stage + L::KB + r0 * RB);
+#pragma unroll
+              for (int i = 0; i < IB; ++i) {
+                const int col = warp * CW + (i0 + i) * 16 + g;
+                const int c0 = swz_v<T, CPR>(col / 4, r0) * 4 + col % 4, c1 = swz_v<T, CPR>(col / 4 + 2, r0) * 4 + col % 4;
+                uint32_t ah[4], al[4];
+                split_tf32(vp[c0], ah[0], al[0]);
+                split_tf32(vp[c1], ah[1], al[1]);
+                split_tf32(vp[c0 + 4 * HD], ah[2], al[2]);
+                split_tf32(vp[c1 + 4 * HD], ah[3], al[3]);
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+                  if (act(n)) mma_f32(t[i][n], ah, al, bh[n], bl[n]);
+              }
+            }
           }
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              uint32_t v[4];
-              ldsm4t((va ^ (i * 32)) + (j * 32 + h * 16) * RB, v);
-#pragma unroll
-              for (int n = 0; n < NR; ++n)
-                if (act(n)) mma16<T>(acc[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
-#pragma unroll
-              for (int n = 0; n < NR; ++n)
-                if (act(n)) mma16<T>(acc[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
-            }
-        }
-      } else {
-#pragma unroll 2
-        for (int k = 0; k * 8 < d.npos; ++k) {
-          uint32_t bh[NR][2], bl[NR][2];
-#pragma unroll
-          for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              split_tf32(*(const float*)(pw + (n * 8 + g) * PROW + (((2 * k + h) ^ g) * 16) + t4 * 4), bh[n][h], bl[n][h]);
-          const int r0 = k * 8 + t4;  // and r0 + 4: the same swizzle
-          const float* const vp = (const float*)(stage + L::KB + r0 * RB);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const int col = warp * CW + i * 16 + g;
-            const int c0 = swz_v<T, CPR>(col / 4, r0) * 4 + col % 4, c1 = swz_v<T, CPR>(col / 4 + 2, r0) * 4 + col % 4;
-            uint32_t ah[4], al[4];
-            split_tf32(vp[c0], ah[0], al[0]);
-            split_tf32(vp[c1], ah[1], al[1]);
-            split_tf32(vp[c0 + 4 * HD], ah[2], al[2]);
-            split_tf32(vp[c1 + 4 * HD], ah[3], al[3]);
+          for (int i = 0; i < IB; ++i)
 #pragma unroll
             for (int n = 0; n < NR; ++n)
-              if (act(n)) mma_f32(acc[i][n], ah, al, bh[n], bl[n]);
-          }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i0 + i][n][e] = fmaf(acc[i0 + i][n][e], alpha[n][e & 1], t[i][n][e]);
         }
       }
     }

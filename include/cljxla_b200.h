@@ -257,7 +257,8 @@ typedef struct CLJXLA_VerifyDraftArgs {
   const int32_t* starts;    /* [num_seqs + 1], ascending; NULL: tokens / num_seqs rows each */
   const float* uniform;     /* [tokens] in [0, 1): row r decides on row r + 1's token; NULL when greedy */
   const float* race;        /* [num_seqs, vocab] positive, exponentially distributed; NULL when greedy */
-  int64_t tokens, num_seqs, vocab, max_tokens; /* max_tokens: upper bound of a sequence's rows, at most 128 */
+  int64_t tokens, num_seqs, vocab, max_tokens; /* max_tokens: upper bound of a sequence's rows, at most 128
+                                                  (drafts past it count as rejected) */
   int64_t target_stride, draft_stride, race_stride; /* elements from row to row */
   float temperature, draft_temperature; /* logits are divided by these, > 0 */
   int32_t dtype;  /* of target and draft: F32, F16 or BF16 */

@@ -203,6 +203,23 @@ def test_attend_rows_past_max_tokens_are_left(paged):
     check_rows(cache.attend(case.q.cuda(), out=buf, starts=case.dstarts, max_tokens=2), want, tol, before)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attend_and_append_without_pages(paged, dtype):
+    """A pool of no pages, and a table of no columns: rows see nothing, nothing is written."""
+    case = Case([5, 40], [1, 2], 2, 2, 64, 16, dtype, seed=4)
+    lens = torch.tensor(case.lens, dtype=torch.int32).cuda()
+    starts = torch.tensor(case.starts, dtype=torch.int32).cuda()
+    q, k, v = case.q.cuda(), case.kn.cuda(), case.vn.cuda()
+    none = torch.zeros((0, 2, 16, 64), dtype=TYPES[dtype], device="cuda")
+    pool = torch.full((3, 2, 16, 64), 5.0, dtype=TYPES[dtype], device="cuda")
+    for pages, table in ((none, case.table.cuda()), (pool, torch.zeros((2, 0), dtype=torch.int32, device="cuda"))):
+        cache = paged.PagedKV(pages, pages.clone(), table, lens)
+        cache.append(k, v, starts=starts)
+        out = torch.full_like(q, 3.0)
+        cache.attend(q, out=out, starts=starts, max_tokens=2)
+        assert bool((out == 0).all()) and bool((pool == 5.0).all())
+
+
 @pytest.mark.parametrize("hd,dtype", [(128, "bf16"), (64, "f32"), (256, "f16")])
 def test_attend_evicted_and_bad_pages_are_left_out(paged, hd, dtype):
     case = Case([200, 90, 40], [2, 1, 1], 2, 2, hd, 16, dtype, seed=5)
@@ -589,6 +606,78 @@ def test_verify_without_starts(paged):
     for n in ("target", "draft", "tokens", "uniform"):
         c[n] = c[n][:9].contiguous()
     verify_run(paged, c, use_starts=False, most=5)
+
+
+def test_verify_rows_past_max_tokens_count_as_rejected(paged):
+    c = verify_case(700, [5, 2, 4], "f32", False, True, seed=41)
+    cuda = {n: c[n].cuda() for n in ("target", "tokens")}
+    out, acc = torch.zeros((3, 3), dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([50, 60, 70], dtype=torch.int32, device="cuda")
+    paged.verify_draft(cuda["target"], cuda["tokens"], torch.tensor(c["starts"], dtype=torch.int32).cuda(), out_tokens=out,
+                       accepted=acc, greedy=True, seq_lens=lens, new_lens=lens)
+    want, taken, _ = verify_oracle(c["target"], None, c["tokens"], c["starts"], None, None, True, 1.0, 1.0, 3)
+    assert torch.equal(out.cpu(), want) and torch.equal(acc.cpu(), taken)
+    assert lens.tolist() == [50 - (4 - int(taken[0])), 60 - (1 - int(taken[1])), 70 - (3 - int(taken[2]))]
+
+
+def test_verify_captured_follows_its_inputs(paged):
+    c = verify_case(5000, [4, 1, 3], "bf16", True, False, seed=42)
+    d = {n: c[n].cuda() for n in ("target", "draft", "tokens", "uniform", "race")}
+    starts = torch.tensor(c["starts"], dtype=torch.int32).cuda()
+    out, acc = torch.zeros((3, 4), dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    run = lambda: paged.verify_draft(d["target"], d["tokens"], starts, out_tokens=out, accepted=acc, draft_logits=d["draft"],
+                                     uniform=d["uniform"], race=d["race"])
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed in (43, 44):
+        c = verify_case(5000, [2, 3, 3] if seed == 43 else [4, 4, 0], "bf16", True, False, seed=seed)
+        for n in d:
+            k = min(d[n].shape[0], c[n].shape[0])
+            d[n][:k].copy_(c[n][:k])
+        starts.copy_(torch.tensor(c["starts"], dtype=torch.int32))
+        graph.replay()
+        want, taken, _ = verify_oracle(c["target"], c["draft"], c["tokens"], c["starts"], c["uniform"], c["race"], False, 1.0, 1.0, 4)
+        assert torch.equal(out.cpu(), want) and torch.equal(acc.cpu(), taken)
+
+
+def test_first_calls_may_be_captured():
+    """A process whose first calls are made under capture (nothing is loaded or set up before)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys
+sys.path.insert(0, %r)
+import __graft_entry__ as g
+g._pkg()
+import torch
+from cljxla_b200.host import paged
+z = lambda *s, **k: torch.zeros(s, device="cuda", **k)
+i32 = torch.int32
+pages = z(9, 2, 16, 64, dtype=torch.bfloat16)
+cache = paged.PagedKV(pages, z(9, 2, 16, 64, dtype=torch.bfloat16) + 2, torch.arange(8, dtype=i32, device="cuda").view(1, 8), z(1, dtype=i32) + 100)
+q, k = z(2, 4, 64, dtype=torch.bfloat16), z(2, 2, 64, dtype=torch.bfloat16) + 2
+logits, toks, out, acc = z(2, 5000), z(2, dtype=i32), z(1, 2, dtype=i32), z(1, dtype=i32)
+uniform, race = z(2) + 0.5, z(1, 5000) + 1
+rope = paged.Rope(paged.rope_inv_freq(64, device="cuda"))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    cache.append(k, k, q=q, rope=rope)
+    o = cache.attend(q)
+    paged.verify_draft(logits, toks, out_tokens=out, accepted=acc, uniform=uniform, race=race)
+graph.replay()
+torch.cuda.synchronize()
+assert bool((o == 2).all()), o
+assert out.tolist()[0][0] in (0, 1), out
+print("captured")
+""" % root
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
 
 
 def test_verify_identical_draft_is_accepted_whole(paged):

@@ -102,7 +102,7 @@ def test_append_refuses_broadcast_pages(paged):
     (dict(tokens=3), "multiple of num_seqs"), (dict(max_tokens=1), "max_tokens"), (dict(max_tokens=-1), "max_tokens"),
     (dict(out_dtype=10), "out_dtype"), (dict(out_dtype=2), "dtype"), (dict(scale=float("nan")), "scale"),
     (dict(scale=float("inf")), "scale"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("inf")), "softcap"),
-    (dict(q=0x50008), "q must"), (dict(out=0x60004), "out must"), (dict(q_head_stride=65), "q must"),
+    (dict(scale=1e30, softcap=1e-30), "scale / softcap"), (dict(q=0x50008), "q must"), (dict(out=0x60004), "out must"), (dict(q_head_stride=65), "q must"),
     (dict(out_token_stride=0), "broadcast"), (dict(q=None), "null q"), (dict(out=None), "null q or out"),
     (dict(workspace=0x1008, workspace_bytes=1 << 40), "workspace"),
 ])
@@ -127,7 +127,7 @@ def test_verify_refusals(paged, kw, msg):
     assert rc == 3 and msg in err, (rc, err)
 
 
-def test_verify_refuses_a_short_workspace_and_null_structs(paged):
+def test_null_structs_are_refused(paged):
     lib = paged._library()
     rc, err = call(lib.append, None, append_args(paged))
     assert rc == 3 and "null cache" in err

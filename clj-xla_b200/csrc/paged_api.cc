@@ -211,12 +211,13 @@ VerifyParams verify_params(const CLJXLA_VerifyDraftArgs* a) {
        "draft rows overlap");
   need(a->greedy || a->num_seqs <= 1 || (a->race_stride >= a->vocab && a->race_stride <= kMaxStride),
        "race rows overlap");
-  need(a->temperature > 0.f && a->temperature - a->temperature == 0.f && 1.f / a->temperature - 1.f / a->temperature == 0.f,
-       "temperature must be positive and finite");
-  need(!a->draft || a->greedy ||
-           (a->draft_temperature > 0.f && a->draft_temperature - a->draft_temperature == 0.f &&
-            1.f / a->draft_temperature - 1.f / a->draft_temperature == 0.f),
-       "draft_temperature must be positive and finite");
+  auto usable = [](float t) {  // its reciprocal times log2(e) is finite too
+    const float c = 1.5f / t;
+    return t > 0.f && t - t == 0.f && c - c == 0.f;
+  };
+  need(usable(a->temperature), "temperature must be positive and finite, and not next to zero");
+  need(!a->draft || a->greedy || usable(a->draft_temperature),
+       "draft_temperature must be positive and finite, and not next to zero");
   p.target = (const char*)a->target;
   p.draft = a->greedy ? nullptr : (const char*)a->draft;  // a greedy decision needs no distribution
   p.tokens_in = a->tokens_in;

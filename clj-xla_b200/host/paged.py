@@ -173,7 +173,7 @@ def _rows(t: torch.Tensor, name: str, shape, dtype, device: int):
 
 
 def _vector(t: torch.Tensor, name: str, n: int, dtype, device: int) -> int:
-    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() != n or t.dim() != 1 or t.get_device() != device or not t.is_contiguous():
         _expected(name, (n,), dtype, device, t, ", contiguous,")
     return t.data_ptr()
 

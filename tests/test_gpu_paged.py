@@ -620,6 +620,64 @@ def test_verify_rows_past_max_tokens_count_as_rejected(paged):
     assert lens.tolist() == [50 - (4 - int(taken[0])), 60 - (1 - int(taken[1])), 70 - (3 - int(taken[2]))]
 
 
+def test_calls_without_rows(paged):
+    """No rows at all: attention and append leave everything, verification says so."""
+    case = Case([5, 40], [0, 0], 2, 2, 64, 16, "bf16", seed=4)
+    cache = case.cache(paged)
+    z = lambda *s, **k: torch.zeros(s, device="cuda", **k)
+    none = z(0, 4, 64, dtype=torch.bfloat16)
+    cache.append(z(0, 2, 64, dtype=torch.bfloat16), z(0, 2, 64, dtype=torch.bfloat16), q=none)
+    assert cache.attend(none).shape == (0, 4, 64)
+    assert torch.equal(cache.k_pages.cpu(), case.k)
+    for greedy in (False, True):
+        out, acc, logs = z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32) + 7, z(2, 3) + 7
+        lens = torch.tensor([9, 4], dtype=torch.int32, device="cuda")
+        paged.verify_draft(z(0, 50), z(0, dtype=torch.int32), out_tokens=out, accepted=acc, logprobs=logs, uniform=z(0),
+                           race=z(2, 50) + 1, greedy=greedy, seq_lens=lens, new_lens=lens)
+        assert out.tolist() == [[-1] * 3] * 2 and acc.tolist() == [0, 0] and lens.tolist() == [9, 4] and not logs.any()
+
+
+def test_python_refusals(paged):
+    case = Case([20, 40], [2, 1], 2, 2, 64, 16, "bf16", seed=4)
+    cache = case.cache(paged)
+    q, k, v = case.q.cuda(), case.kn.cuda(), case.vn.cuda()
+    z = lambda *s, **kw: torch.zeros(s, device="cuda", **kw)
+    with pytest.raises(ValueError, match="q:"):
+        cache.attend(q.float())
+    with pytest.raises(ValueError, match="q:"):
+        cache.attend(case.q)
+    with pytest.raises(ValueError, match="contiguous"):
+        cache.attend(q.transpose(1, 2).contiguous().transpose(1, 2), starts=case.dstarts)
+    with pytest.raises(ValueError, match="out"):
+        cache.attend(q, out=z(3, 4, 64, dtype=torch.float16), starts=case.dstarts)
+    with pytest.raises(ValueError, match="starts"):
+        cache.attend(q, starts=case.dstarts.long())
+    with pytest.raises(ValueError, match="starts"):
+        cache.attend(q, starts=case.dstarts[:2])
+    with pytest.raises(ValueError, match="v:"):  # the rows are counted by k
+        cache.append(k[:2], v, starts=case.dstarts)
+    with pytest.raises(ValueError, match="q_out"):
+        cache.append(k, v, q_out=q, starts=case.dstarts)
+    with pytest.raises(ValueError, match="page_table"):
+        paged.PagedKV(case.dk, case.dv, case.dtable.long(), case.dlens)
+    with pytest.raises(ValueError, match="seq_lens"):
+        paged.PagedKV(case.dk, case.dv, case.dtable, case.dlens[:1])
+    from cljxla_b200.host.pjrt import PJRTError
+    with pytest.raises(PJRTError, match="multiple of num_seqs"):
+        cache.attend(q)
+    with pytest.raises(PJRTError, match="multiple of kv_heads"):
+        cache.attend(z(3, 3, 64, dtype=torch.bfloat16), starts=case.dstarts)
+    with pytest.raises(PJRTError, match="head_dim"):
+        paged.PagedKV(z(2, 1, 16, 96), z(2, 1, 16, 96), z(1, 2, dtype=torch.int32), z(1, dtype=torch.int32)).attend(z(1, 1, 96))
+    with pytest.raises(PJRTError, match="16-byte"):
+        cache.attend(z(3, 4, 72, dtype=torch.bfloat16)[:, :, 4:68], starts=case.dstarts)
+    with pytest.raises(ValueError, match="uniform and race"):
+        paged.verify_draft(z(2, 9), z(2, dtype=torch.int32), out_tokens=z(1, 2, dtype=torch.int32), accepted=z(1, dtype=torch.int32))
+    with pytest.raises(PJRTError, match="max_tokens"):
+        paged.verify_draft(z(2, 9), z(2, dtype=torch.int32), out_tokens=z(1, 1, dtype=torch.int32),
+                           accepted=z(1, dtype=torch.int32), greedy=True)
+
+
 def test_verify_captured_follows_its_inputs(paged):
     c = verify_case(5000, [4, 1, 3], "bf16", True, False, seed=42)
     d = {n: c[n].cuda() for n in ("target", "draft", "tokens", "uniform", "race")}

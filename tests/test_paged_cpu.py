@@ -116,7 +116,7 @@ def test_attention_refusals(paged, kw, msg):
     (dict(max_tokens=129), "max_tokens"), (dict(max_tokens=1), "max_tokens"), (dict(tokens=3), "multiple of num_seqs"),
     (dict(target_stride=99), "target rows"), (dict(draft_stride=99), "draft rows"), (dict(race_stride=99), "race rows"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
-    (dict(temperature=float("inf")), "temperature"), (dict(draft_temperature=-1.0), "draft_temperature"),
+    (dict(temperature=float("inf")), "temperature"), (dict(temperature=4e-39), "temperature"), (dict(draft_temperature=-1.0), "draft_temperature"),
     (dict(dtype=4), "dtype"), (dict(tokens_out=None), "tokens_out"), (dict(accepted=None), "accepted"),
     (dict(seq_lens=None), "seq_lens"), (dict(target=None), "null target"), (dict(tokens_in=None), "tokens_in"),
     (dict(uniform=None), "uniform"), (dict(race=None), "race"), (dict(target=0x10001), "aligned"),

@@ -434,22 +434,39 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
         const int kr = warp * 16 + g;  // and kr + 8: the same swizzle
         const float* const kp = (const float*)(stage + kr * RB);
         const float* const qp = (const float*)(queries + g * RB);
-#pragma unroll 4
-        for (int k = 0; k < HD / 8; ++k) {
-          const int c0 = swz<CPR>(2 * k, g) * 4 + t4, c1 = swz<CPR>(2 * k + 1, g) * 4 + t4;
-          uint32_t ah[4], al[4];
-          split_tf32(kp[c0], ah[0], al[0]);
-          split_tf32(kp[c0 + 8 * HD], ah[1], al[1]);
-          split_tf32(kp[c1], ah[2], al[2]);
-          split_tf32(kp[c1 + 8 * HD], ah[3], al[3]);
+        // four steps' sums apart, the small products from the large, and added with
+        // rounding: the tensor cores cut sums off, which 96 times in one chain costs
+        // 3e-6 of a score
+#pragma unroll 1
+        for (int k4 = 0; k4 < HD / 8; k4 += 4) {
+          float big[NR][4], small[NR][4];
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            if (!act(n)) break;
-            uint32_t bh[2], bl[2];
-            split_tf32(qp[c0 + n * 8 * HD], bh[0], bl[0]);
-            split_tf32(qp[c1 + n * 8 * HD], bh[1], bl[1]);
-            mma_f32(s[n], ah, al, bh, bl);
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) big[n][e] = small[n][e] = 0.f;
+#pragma unroll
+          for (int k = k4; k < k4 + 4; ++k) {
+            const int c0 = swz<CPR>(2 * k, g) * 4 + t4, c1 = swz<CPR>(2 * k + 1, g) * 4 + t4;
+            uint32_t ah[4], al[4];
+            split_tf32(kp[c0], ah[0], al[0]);
+            split_tf32(kp[c0 + 8 * HD], ah[1], al[1]);
+            split_tf32(kp[c1], ah[2], al[2]);
+            split_tf32(kp[c1 + 8 * HD], ah[3], al[3]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              if (!act(n)) break;
+              uint32_t bh[2], bl[2];
+              split_tf32(qp[c0 + n * 8 * HD], bh[0], bl[0]);
+              split_tf32(qp[c1 + n * 8 * HD], bh[1], bl[1]);
+              mma_tf32(small[n], al, bh[0], bh[1]);
+              mma_tf32(small[n], ah, bl[0], bl[1]);
+              mma_tf32(big[n], ah, bh[0], bh[1]);
+            }
           }
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] += big[n][e] + small[n][e];
         }
       }
       // base-2 scores

@@ -6,8 +6,9 @@
 // and sum (a new maximum m' scales what is there by 2^(m - m')).
 //
 // What bounds it: each visible K and V row is read once from HBM for
-// 4 * head_dim FLOPs per query row, at most 64 rows to a byte pair, so the
-// bound is HBM bandwidth as long as enough copies are in flight.
+// 4 * head_dim FLOPs per query row.  A decode step's 1 to 16 rows are bound by
+// HBM bandwidth as long as enough copies are in flight; from about 32 rows per KV
+// head on the tensor and issue slots of the consumer warps are.
 //
 // Split.  A segment is (sequence, KV head, up to ROWS query rows of that head's
 // group), a row of tiles of its positions.  All tiles of the call, laid end to
@@ -72,7 +73,7 @@ struct Tile {
     return n;
   }
   static constexpr int pick() {
-    int ctas = KB > 16384 || NR == 8 ? 1 : 2;  // 64 rows need all registers
+    int ctas = KB > 16384 ? 1 : 2;
     while (ctas > 1 && fit(ctas) < 3) --ctas;
     return ctas;
   }
@@ -374,7 +375,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
     const uint32_t ks = smem_u32(stage), vs = ks + L::KB, qs = smem_u32(queries);
     unsigned char* const pw = L::P_IN_K ? stage : p_own;
     const uint64_t vis = TP == 64 ? (uint64_t)d.mask[1] << 32 | d.mask[0] : d.mask[0];
-    const auto act = [&](int n) { return NR == 1 || NR == 8 || n * 8 < d.nrows; };  // whether any of 8 rows is there (8: no registers to ask)
     const bool plain = (d.flags & T_FULL) && vis == (TP == 64 ? ~0ull : 0xffffffffull);
     // 8 query rows x 32 of head_dim: the second operands of two steps
     const uint32_t qa = qs + (lane & 7) * RB + swz<CPR>(lane >> 3, lane & 7) * 16;
@@ -414,7 +414,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
           ldsm4(ka ^ (j * 64 + 32), k1);
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
-            if (!act(n)) break;
             uint32_t q[4];
             if constexpr (Q_REGS) {
 #pragma unroll
@@ -454,7 +453,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
             split_tf32(kp[c1 + 8 * HD], ah[3], al[3]);
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-              if (!act(n)) break;
               uint32_t bh[2], bl[2];
               split_tf32(qp[c0 + n * 8 * HD], bh[0], bl[0]);
               split_tf32(qp[c1 + n * 8 * HD], bh[1], bl[1]);
@@ -485,7 +483,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
         for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            if (!act(n)) break;
             int jlo, jhi;
             row_view(P, d, n * 8 + 2 * t4 + r, jlo, jhi);
 #pragma unroll
@@ -497,7 +494,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
       }
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        if (!act(n)) break;
         float2 x = make_float2(fmaxf(s[n][0], s[n][2]), fmaxf(s[n][1], s[n][3]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
@@ -512,7 +508,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
     float alpha[NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      if (!act(n)) break;
       float2 x = make_float2(m[n][0], m[n][1]);
 #pragma unroll
       for (int w = 0; w < SCORERS; ++w) {
@@ -618,7 +613,7 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
       } else {
         // A tile's sum is made apart and added with one rounding: the tensor cores
         // cut their sums off, and over a long context that adds up to 10^-5 of the result.
-        constexpr int IB = MT * NR <= 4 ? MT : 1;  // 16-column tiles at a time, as registers allow
+        constexpr int IB = MT * NR <= 8 ? MT : 1;  // 16-column tiles at a time, as registers allow
         const uint32_t pa = smem_u32(pw) + (lane & 7) * PROW + (((lane >> 3) ^ (lane & 7)) * 16);
         const int vr = (lane >> 4) * 8 + (lane & 7);
         const uint32_t va = vs + vr * RB + swz_v<T, CPR>(warp * (CW / 8) + (lane >> 3 & 1), vr) * 16;
@@ -636,7 +631,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
               uint32_t ph[NR][4], pl[NR][4], pt[L::PARTS == 3 ? NR : 1][4];
 #pragma unroll
               for (int n = 0; n < NR; ++n) {
-                if (!act(n)) break;
                 ldsm4((pa ^ (j * 64)) + n * 8 * PROW, ph[n]);
                 ldsm4((pa ^ (j * 64)) + (ROWS + n * 8) * PROW, pl[n]);
                 if constexpr (L::PARTS == 3)
@@ -650,15 +644,15 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
                   ldsm4t((va ^ ((i0 + i) * 32)) + (j * 32 + h * 16) * RB, v);
 #pragma unroll
                   for (int n = 0; n < NR; ++n)
-                    if (act(n)) mma16<T>(t[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
+                    mma16<T>(t[i][n], v, ph[n][2 * h], ph[n][2 * h + 1]);
 #pragma unroll
                   for (int n = 0; n < NR; ++n)
-                    if (act(n)) mma16<T>(t[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
+                    mma16<T>(t[i][n], v, pl[n][2 * h], pl[n][2 * h + 1]);
                   if constexpr (L::PARTS == 3) {
                     if (third) {
 #pragma unroll
                       for (int n = 0; n < NR; ++n)
-                        if (act(n)) mma16<T>(t[i][n], v, pt[n][2 * h], pt[n][2 * h + 1]);
+                        mma16<T>(t[i][n], v, pt[n][2 * h], pt[n][2 * h + 1]);
                     }
                   }
                 }
@@ -685,7 +679,7 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
                 split_tf32(vp[c1 + 4 * HD], ah[3], al[3]);
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
-                  if (act(n)) mma_f32(t[i][n], ah, al, bh[n], bl[n]);
+                  mma_f32(t[i][n], ah, al, bh[n], bl[n]);
               }
             }
           }
@@ -705,7 +699,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
       if (SCORERS == 4 || warp < SCORERS) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          if (!act(n)) break;
           float2 x = make_float2(l[n][0], l[n][1]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
@@ -723,7 +716,6 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
       const int odd_g = g & 1;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        if (!act(n)) break;
         const int in_tile = n * 8 + 2 * t4 + odd_g;
         const bool mine = in_tile < d.nrows;
         float sum = 0.f;
@@ -1278,20 +1270,17 @@ __global__ void __launch_bounds__(AT_JOIN_THREADS) paged_attn_join_kernel(const 
 }
 
 // ------------------------------------------------------------------- host
-// Row tiles of 8, 16, 32 or 64 rows: the smallest that holds a sequence's rows
-// for one KV head (more rows than 64 take several tiles, each reading K and V
-// again, from L2).  f32 rows of 256 stop at 32: two stages of more do not fit.
+// Row tiles of 8, 16 or 32 rows: the smallest that holds a sequence's rows for one
+// KV head.  More rows than 32 take several tiles, each reading K and V again, from
+// L2: 64 at a time, with their spills and fewer CTAs, measured 264 against 157 us
+// (64 rows, head_dim 256), 124 against 108 (128) and 90 against 76 (32).
 // f32 with at most four rows: 1, 2 or 4 of them on the FMA units (a negative
 // count).
-template <typename T, int HD>
-constexpr int max_nr() {
-  return sizeof(T) == 4 && HD == 256 ? 4 : 8;
-}
-template <typename T, int HD>
+template <typename T>
 int pick_nr(const PagedAttnParams& p) {
   const int64_t rows = (int64_t)p.max_rows * p.group;
   if (sizeof(T) == 4 && rows <= 4) return rows <= 1 ? -1 : rows <= 2 ? -2 : -4;
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 || max_nr<T, HD>() == 4 ? 4 : 8;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
 
 // One tile at most in any segment: none is cut, and nothing needs joining.
@@ -1327,7 +1316,7 @@ void launch_nr(PagedAttnParams p, cudaStream_t s) {
 
 template <typename T, int HD, class F>
 auto with_nr(const PagedAttnParams& p, F f) {
-  const int nr = pick_nr<T, HD>(p);
+  const int nr = pick_nr<T>(p);
   if constexpr (sizeof(T) == 4) {
     if (nr == -1) return f(std::integral_constant<int, -1>());
     if (nr == -2) return f(std::integral_constant<int, -2>());
@@ -1336,8 +1325,7 @@ auto with_nr(const PagedAttnParams& p, F f) {
   switch (nr) {
     case 1: return f(std::integral_constant<int, 1>());
     case 2: return f(std::integral_constant<int, 2>());
-    case 4: return f(std::integral_constant<int, 4>());
-    default: return f(std::integral_constant<int, max_nr<T, HD>()>());
+    default: return f(std::integral_constant<int, 4>());
   }
 }
 template <typename T, class F>

@@ -77,10 +77,14 @@ struct Stat {
   int i;
 };
 __device__ __forceinline__ float vd_ref(float m, float c) { return m == -INFINITY ? 0.f : __fmul_rn(m, c); }
+// What brings a sum from its maximum's reference to that of a larger one.  A part
+// without a finite logit has none to bring: 2^(0 - R) is no factor for it, and
+// infinite where all logits are low (0 * inf would make the joined sum NaN).
+__device__ __forceinline__ float vd_scale(float m, float ref, float R) { return m == -INFINITY ? 0.f : vd_ex2(ref - R); }
 __device__ __forceinline__ void vd_join(Stat& a, const Stat& b, float c) {
   const float M = fmaxf(a.m, b.m), R = vd_ref(M, c);
   if (b.i >= 0 && (a.i < 0 || b.m > a.m || (b.m == a.m && b.i < a.i))) a.i = b.i;
-  a.s = a.s * vd_ex2(vd_ref(a.m, c) - R) + b.s * vd_ex2(vd_ref(b.m, c) - R);  // an empty part has sum 0
+  a.s = a.s * vd_scale(a.m, vd_ref(a.m, c), R) + b.s * vd_scale(b.m, vd_ref(b.m, c), R);
   a.m = M;
 }
 __device__ __forceinline__ void vd_join_warp(Stat& a, float c) {
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
             if (f[i] == top) a.i = (int)(head + (at + u * VD_THREADS) * V + i);
         }
         const float R = __fmul_rn(top, c);
-        a.s *= vd_ex2(ref - R);
+        a.s *= vd_scale(a.m, ref, R);
         a.m = top;
         ref = R;
       }

@@ -1,0 +1,150 @@
+"""Paged-cache operators where values are extreme: logits far from zero, finite
+masks, the ends of a type's range, dominant positions; and calls at the edge of
+what the interface allows.
+
+Forms and tolerances are those of test_gpu_paged.py; where a case adds to them,
+the count stands beside it.  Probabilities are held in f32, so one below 2^-126 is
+zero: the oracle here takes a residual weight max(p - q, 0) below that as nothing
+(the operator then draws from p, as documented), which 64 bits would still tell
+apart.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import INF, TYPES, paged, verify_case  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+LEAST = 2.0 ** -126
+
+
+# -------------------------------------------------------------- verification
+def decided(c, temp, most, got):
+    """The plain form in 64 bits: tokens, accepted counts, log-probabilities.  No
+    choice is nearer to its border than 1e-5, but for tokens without a probability
+    in f32 (there the accepted counts `got` decide)."""
+    seqs = len(c["starts"]) - 1
+    out, taken = torch.full((seqs, most), -1, dtype=torch.int32), torch.zeros(seqs, dtype=torch.int32)
+    logs = torch.zeros((seqs, most), dtype=torch.float64)
+    for b in range(seqs):
+        first, n = c["starts"][b], 0
+        count = min(c["starts"][b + 1] - first, most)
+        while n < count:
+            row, last = c["target"][first + n].double(), n == count - 1
+            log = torch.log_softmax(row / temp, 0)
+            p, best = log.exp(), int(torch.nonzero(row == row.max())[0])
+            x = None if last else int(c["tokens"][first + n + 1])
+            logq = torch.full_like(p, -INF)
+            if not last and c["draft"] is not None and not c["greedy"]:
+                logq = torch.log_softmax(c["draft"][first + n].double() / temp, 0)
+            elif not last:
+                logq[x] = 0.0
+            q = logq.exp()
+            if c["greedy"]:
+                good = x == best
+            elif not last:  # in logarithms: a masked token's p and q are below what 64 bits hold
+                left, right = math.log(float(c["uniform"][first + n])) + float(logq[x]), float(log[x])
+                good = left < right
+                # c, the product, log2 and the sums: at most 2^-21 of each side
+                if abs(left - right) <= 1e-5 + 2.0 ** -21 * (abs(left) + abs(right)) and right > -INF:
+                    assert right < math.log(LEAST)  # a token that neither side would give: f32 cannot tell, either answer is right
+                    good = int(got[b]) > n
+            if not last and good:
+                out[b, n], logs[b, n] = x, log[x]
+                n += 1
+                continue
+            token = best
+            if not c["greedy"]:
+                w = p if last else torch.where(q == 1.0, 0.0, p) if c["draft"] is None else p - q
+                w = w if float(w.max()) >= LEAST else p
+                key = w / c["race"][b].double()
+                two = torch.topk(key, 2).values
+                assert two[0] > two[1] * (1 + 1e-5)
+                token = int(key.argmax())
+            out[b, n], logs[b, n] = token, log[token]
+            break
+        taken[b] = n
+    return out, taken, logs
+
+
+def verify(paged, c, temp=1.0):
+    """One call, compared with the plain form."""
+    seqs = len(c["starts"]) - 1
+    most = max(b - a for a, b in zip(c["starts"], c["starts"][1:]))
+    d = {n: None if c[n] is None else c[n].cuda() for n in ("target", "draft", "tokens", "uniform", "race")}
+    out, acc = (torch.full(s, -77, dtype=torch.int32, device="cuda") for s in ((seqs, most), (seqs,)))
+    logs = torch.full((seqs, most), 77.0, device="cuda")
+    paged.verify_draft(d["target"], d["tokens"], torch.tensor(c["starts"], dtype=torch.int32).cuda(), out_tokens=out, accepted=acc,
+                       logprobs=logs, draft_logits=d["draft"], uniform=d["uniform"], race=d["race"], temperature=temp,
+                       greedy=c["greedy"])
+    want, taken, wlogs = decided(c, temp, most, acc.cpu())
+    assert torch.equal(acc.cpu(), taken), (acc.cpu(), taken)
+    assert torch.equal(out.cpu(), want), (out.cpu(), want)
+    assert bool(((logs.cpu().double() - wlogs).abs() <= 2.0 ** -18 + 2.0 ** -22 * wlogs.abs()).all())
+    return acc
+
+
+def low_case(dtype, drafts, greedy, temp, change, seed, which=("target", "draft"), vocab=6007):
+    """A case whose logits `change` has been over, with tokens that fit them: drafts drawn from the changed draft."""
+    c = verify_case(vocab, [4, 1, 5, 3, 2], dtype, drafts, greedy, seed)
+    for n in which:
+        if c[n] is not None:
+            c[n] = change(c[n].float()).to(TYPES[dtype])
+    g = torch.Generator().manual_seed(seed + 1)
+    noise = -torch.log(-torch.log(torch.rand(c["target"].shape, generator=g).clamp(1e-9, 1 - 1e-7)))
+    base = (c["draft"] if drafts else c["target"]).double() / temp
+    drawn = (base if greedy else base + noise).argmax(1)[:-1].int()
+    c["tokens"][1:] = torch.where(torch.rand(drawn.shape, generator=g) < 0.15, c["tokens"][1:], drawn)
+    if drafts or greedy:
+        c["uniform"] *= 0.5
+    else:
+        c["uniform"] *= 2.0 ** -20  # a guess without a distribution is rarely taken
+    return c
+
+
+def masked(value, how):
+    """Sets `value` in the first half (whole slices of a row), all but a few (whole vectors), or all but one."""
+    def change(x):
+        x = x.clone()
+        if how == "half":
+            x[:, :3400] = value
+        elif how == "most":
+            keep = torch.rand(x.shape, generator=torch.Generator().manual_seed(7)) < 0.01
+            keep[:, 5000] = True
+            x[~keep] = value
+        else:
+            x[:, :4100], x[:, 4101:] = value, value
+        return x
+    return change
+
+
+LOW = {
+    # name: (dtype, temperature, change)
+    **{f"shift_{d}_{v}": (d, 0.8, lambda x, v=v: x + v) for d in TYPES for v in (-100, -1000)},
+    "shift_f32_cold": ("f32", 0.01, lambda x: x * 0.01 - 3.0),
+    "shift_f32_far": ("f32", 1.0, lambda x: x * 512 - 2.0 ** 20),
+    "shift_f32_up": ("f32", 0.5, lambda x: x + 700.0),
+    **{f"mask_{d}_{how}_{v:g}": (d, 0.8, masked(v, how)) for d, vs in (("f32", (-1e4, -1e9)), ("bf16", (-1e4, -1e9)), ("f16", (-1e4, -65504.0)))
+       for v in vs for how in ("half", "most", "one")},
+}
+
+
+@pytest.mark.parametrize("mode", ["drafts", "guesses", "greedy"])
+@pytest.mark.parametrize("name", list(LOW))
+def test_verify_low_logits(paged, name, mode):
+    """A softmax does not see an offset, and a finite mask is as good as -inf: rows and vectors of very low logits."""
+    dtype, temp, change = LOW[name]
+    c = low_case(dtype, mode == "drafts", mode == "greedy", temp, change, seed=60)
+    acc = verify(paged, c, temp)
+    assert int(acc.sum()) >= 2
+
+
+@pytest.mark.parametrize("which", ["target", "draft"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_verify_one_side_low(paged, dtype, which):
+    c = low_case(dtype, True, False, 1.0, lambda x: x - 1000, seed=61, which=(which,))
+    verify(paged, c)
+    c = low_case(dtype, True, False, 1.0, masked(-1e4, "half"), seed=62, which=(which,))
+    verify(paged, c)

@@ -71,31 +71,67 @@ __device__ __forceinline__ void vd_unpack(const uint4& v, float* x) {
 // reference R = m c as it rounds (the same R wherever m is the same, so its
 // rounding cancels in every quotient and one FMA gives each exponent), and the
 // lowest index of the maximum.  Of nothing, or of -inf alone: (-inf, 0, -1).  A
-// NaN is no maximum and makes the sum one.
+// NaN is no maximum and makes the sum one, as a maximum of +inf does.
 struct Stat {
   float m, s;
   int i;
 };
 __device__ __forceinline__ float vd_ref(float m, float c) { return m == -INFINITY ? 0.f : __fmul_rn(m, c); }
-// What brings a sum from its maximum's reference to that of a larger one.  A part
-// without a finite logit has none to bring: 2^(0 - R) is no factor for it, and
-// infinite where all logits are low (0 * inf would make the joined sum NaN).
-__device__ __forceinline__ float vd_scale(float m, float ref, float R) { return m == -INFINITY ? 0.f : vd_ex2(ref - R); }
+// What the rounding of R leaves, 2^(m c - R), is a factor of the whole sum.  Past 2^24
+// (logits near the ends of f32 or bf16, or next to no temperature) it could be anything,
+// and R infinite: there sums go by m itself, at the price of more instructions.
+__device__ __forceinline__ bool vd_far(float ref) { return !(fabsf(ref) <= 16777216.f); }
+// base-2 logarithm of the weight of x in a sum with maximum m (NaN for x = m = +inf)
+__device__ __forceinline__ float vd_power(float x, float c, float m, float ref) {
+  return vd_far(ref) ? (x - m) * c : fmaf(x, c, -ref);
+}
+// What brings a sum from its maximum m, of reference `ref`, to a larger one's M, R: at
+// most 1.  A part without a finite logit (sum 0, reference 0) must not be scaled by
+// 2^(0 - R), infinite where all logits are low: 0 * inf would make the joined sum NaN.
+__device__ __forceinline__ float vd_scale(float m, float ref, float M, float R, float c) {
+  if (vd_far(ref) || vd_far(R))
+    return m == -INFINITY ? 0.f : vd_ex2((m - M) * c + vd_power(M, c, M, R) - vd_power(m, c, m, ref));
+  return vd_ex2(fminf(ref - R, 0.f));
+}
 __device__ __forceinline__ void vd_join(Stat& a, const Stat& b, float c) {
   const float M = fmaxf(a.m, b.m), R = vd_ref(M, c);
   if (b.i >= 0 && (a.i < 0 || b.m > a.m || (b.m == a.m && b.i < a.i))) a.i = b.i;
-  a.s = a.s * vd_scale(a.m, vd_ref(a.m, c), R) + b.s * vd_scale(b.m, vd_ref(b.m, c), R);
+  a.s = a.s * vd_scale(a.m, vd_ref(a.m, c), M, R, c) + b.s * vd_scale(b.m, vd_ref(b.m, c), M, R, c);
   a.m = M;
 }
+// The lanes' parts: their maximum, the sums brought to it and added, the lowest index.
 __device__ __forceinline__ void vd_join_warp(Stat& a, float c) {
+  float M = a.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.i = __shfl_xor_sync(0xffffffffu, a.i, o);
-    vd_join(a, b, c);
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  a.s *= vd_scale(a.m, vd_ref(a.m, c), M, vd_ref(M, c), c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+  a.i = (int)__reduce_min_sync(0xffffffffu, a.m == M ? (unsigned)a.i : 0xffffffffu);  // none: -1, the largest
+  a.m = M;
+}
+
+// one logit more
+__device__ __forceinline__ void vd_take(Stat& a, float f, int64_t v, float c) {
+  Stat one{f, f == -INFINITY ? 0.f : vd_ex2(vd_power(f, c, f, vd_ref(f, c))), f > -INFINITY ? (int)v : -1};
+  if (!(f == f)) one.m = -INFINITY;
+  vd_join(a, one, c);
+}
+// A thread's part of a slice whose references reach far, once more and one by one: the
+// element in front (if it is this thread's) and whole vectors.
+template <typename T>
+__device__ __noinline__ Stat vd_far_slice(const T* x, const T* front, const uint4* xv, int64_t at, int64_t hi, int64_t head,
+                                          float c) {
+  constexpr int V = 16 / sizeof(T);
+  Stat a{-INFINITY, 0.f, -1};
+  if (front) vd_take(a, vd_f(*front), front - x, c);
+  for (; at < hi; at += VD_THREADS) {
+    float f[V];
+    vd_unpack<T>(xv[at], f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) vd_take(a, f[i], head + at * V + i, c);
   }
+  return a;
 }
 
 // the largest of a 16-byte vector's values (NaN aside)
@@ -162,13 +198,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
   vd_rows(P, b, first, count, all);
   if (row - first >= count - which) return;  // not looked at; the draft of a sequence's last row is none
   Stat a{-INFINITY, 0.f, -1};
-  auto take = [&](float f, int64_t v) {
-    Stat one{f, f == -INFINITY ? 0.f : f == f ? 1.f : f, f > -INFINITY ? (int)v : -1};
-    if (!(f == f)) one.m = -INFINITY;
-    vd_join(a, one, c);
-  };
+  auto take = [&](float f, int64_t v) { vd_take(a, f, v, c); };
   if (split == 0 && tid < head) take(vd_f(x[tid]), tid);
-  float ref = vd_ref(a.m, c);
+  float ref = vd_ref(a.m, c), reach = fabsf(ref);
   for (int64_t at = lo + tid; at < hi; at += U * VD_THREADS) {
     uint4 raw[U];
 #pragma unroll
@@ -187,9 +219,10 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
             if (f[i] == top) a.i = (int)(head + (at + u * VD_THREADS) * V + i);
         }
         const float R = __fmul_rn(top, c);
-        a.s *= vd_scale(a.m, ref, R);
+        a.s *= vd_ex2(fminf(ref - R, 0.f));
         a.m = top;
         ref = R;
+        reach = fmaxf(reach, fabsf(R));
       }
       float sum = 0.f;
 #pragma unroll
@@ -197,6 +230,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
       a.s += sum;
     }
   }
+  if (vd_far(reach)) a = vd_far_slice<T>(x, split == 0 && tid < head ? x + tid : nullptr, xv, lo + tid, hi, head, c);
   const int64_t rest = head + vecs * V + tid;
   if (split == P.splits - 1 && rest < P.vocab) take(vd_f(x[rest]), rest);
   __shared__ Stat s_warp[VD_THREADS / 32];
@@ -287,7 +321,7 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   }
   __syncthreads();
   auto logp = [&](float l, int r) {
-    return (fmaf(l, c, -vd_ref(s_max[0][r], c)) - log2f(s_sum[0][r])) * 0.6931471805599453f;
+    return (vd_power(l, c, s_max[0][r], vd_ref(s_max[0][r], c)) - log2f(s_sum[0][r])) * 0.6931471805599453f;
   };
   if (tid < count - 1) {
     bool good = valid;
@@ -295,8 +329,8 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
     if (good && !P.greedy) {
       // in logarithms: both sides may lie far below the smallest float
       float lq = 0.f;
-      if (P.draft) lq = fmaf(dx, cd, -vd_ref(s_max[1][tid], cd)) - log2f(s_sum[1][tid]);
-      good = log2f(ux) + lq < fmaf(lx, c, -vd_ref(s_max[0][tid], c)) - log2f(s_sum[0][tid]);
+      if (P.draft) lq = vd_power(dx, cd, s_max[1][tid], vd_ref(s_max[1][tid], cd)) - log2f(s_sum[1][tid]);
+      good = log2f(ux) + lq < vd_power(lx, c, s_max[0][tid], vd_ref(s_max[0][tid], c)) - log2f(s_sum[0][tid]);
     }
     if (!good) atomicMin(&s_taken, tid);
   }
@@ -319,12 +353,22 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
     // the race for w; once more for p in the rare case that w is nothing
     for (int pass = 0; pass < 2 && token < 0; ++pass) {
       Best best{0.f, 1.f, 0.f, -1};
+      auto enter = [&](float w, float lv, float ev, int64_t v) {
+        if (w * best.e > best.w * ev && (int)v != out) best = {w, ev, lv, (int)v};  // a thread's indices ascend
+      };
       auto race = [&](float lv, float dv, float ev, int64_t v) {
         float w = vd_ex2(fmaf(lv, c, -ref)) * inv;
         if (residual) w -= vd_ex2(fmaf(dv, cd, -refd)) * invd;
-        if (w * best.e > best.w * ev && (int)v != out) best = {w, ev, lv, (int)v};  // a thread's indices ascend
+        enter(w, lv, ev, v);
       };
-      if (aligned) {
+      const int64_t end = min(hi * V, P.vocab);
+      if (vd_far(ref) || vd_far(refd)) {
+        for (int64_t v = lo * V + tid; v < end; v += THREADS) {
+          float w = vd_ex2(vd_power(vd_f(l[v]), c, s_max[0][taken], ref)) * inv;
+          if (residual) w -= vd_ex2(vd_power(vd_f(d[v]), cd, s_max[1][taken], refd)) * invd;
+          enter(w, vd_f(l[v]), e[v], v);
+        }
+      } else if (aligned) {
         uint4 la, da = {}, ln, dn = {};
         float4 ea[V / 4], en[V / 4];
         auto fetch = [&](int64_t at) {  // one lot ahead of the one in work
@@ -358,7 +402,6 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
         }
       } else {
         // rows that start anywhere: element by element, a warp's loads side by side
-        const int64_t end = min(hi * V, P.vocab);
 #pragma unroll 8
         for (int64_t v = lo * V + tid; v < end; v += THREADS) race(vd_f(l[v]), residual ? vd_f(d[v]) : 0.f, e[v], v);
       }

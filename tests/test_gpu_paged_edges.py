@@ -47,8 +47,10 @@ def decided(c, temp, most, got):
             elif not last:  # in logarithms: a masked token's p and q are below what 64 bits hold
                 left, right = math.log(float(c["uniform"][first + n])) + float(logq[x]), float(log[x])
                 good = left < right
-                # c, the product, log2 and the sums: at most 2^-21 of each side
-                if abs(left - right) <= 1e-5 + 2.0 ** -21 * (abs(left) + abs(right)) and right > -INF:
+                # c, the product, log2 and the sums: at most 2^-21 of each side; a base-2
+                # logarithm past f32's largest (2.35e38 of a natural one) is -inf
+                beyond = max(left, right) < -2.35e38
+                if (abs(left - right) <= 1e-5 + 2.0 ** -21 * (abs(left) + abs(right)) or beyond) and right > -INF:
                     assert right < math.log(LEAST)  # a token that neither side would give: f32 cannot tell, either answer is right
                     good = int(got[b]) > n
             if not last and good:
@@ -148,3 +150,45 @@ def test_verify_one_side_low(paged, dtype, which):
     verify(paged, c)
     c = low_case(dtype, True, False, 1.0, masked(-1e4, "half"), seed=62, which=(which,))
     verify(paged, c)
+
+
+ENDS = {
+    # name: (dtype, temperature, change): a maximum times log2(e) / temperature does not fit f32
+    **{f"{d}_lowest_{how}_{t}": (d, t, masked(torch.finfo(TYPES[d]).min, how)) for d in ("f32", "bf16") for how in ("half", "most", "one")
+       for t in (0.8, 1.0, 2.0)},
+    "f32_all_lowest": ("f32", 0.8, lambda x: torch.full_like(x, torch.finfo(torch.float32).min)),
+    "bf16_all_lowest": ("bf16", 0.7, lambda x: torch.full_like(x, torch.finfo(torch.bfloat16).min)),
+    "f32_all_highest": ("f32", 0.8, lambda x: torch.full_like(x, torch.finfo(torch.float32).max)),
+    "f32_low_two": ("f32", 0.5, lambda x: torch.where(x > 5.0, -2.5e38, -3e38)),
+    "bf16_high_two": ("bf16", 0.5, lambda x: torch.where(x > 5.0, 3e38, 2.9e38)),
+    "f32_high_some": ("f32", 0.8, lambda x: torch.where(x > 5.0, 3.3e38, x)),
+    "f16_coldest": ("f16", 1e-35, lambda x: x * 5000),
+    "f32_middle": ("f32", 40.0, lambda x: x * 1024 - 2.0 ** 30),  # products of 2^25, whole steps of 2
+    "f32_border": ("f32", 1.0, lambda x: x * 3 - 11629080.0),  # products on both sides of 2^24
+    "f32_border_high": ("f32", 1.0, lambda x: x * 3 + 11629080.0),
+    "bf16_far_mask": ("bf16", 0.03, masked(-1e9, "most")),
+    "f32_wide": ("f32", 0.9, lambda x: x * 3e37),
+}
+
+
+@pytest.mark.parametrize("mode", ["drafts", "guesses", "greedy"])
+@pytest.mark.parametrize("name", list(ENDS))
+def test_verify_logits_at_the_ends_of_the_range(paged, name, mode):
+    """Every row with a finite maximum has an answer, the type's lowest and largest values included."""
+    dtype, temp, change = ENDS[name]
+    c = low_case(dtype, mode == "drafts", mode == "greedy", temp, change, seed=63)
+    verify(paged, c, temp)
+
+
+@pytest.mark.parametrize("mode", ["drafts", "guesses", "greedy"])
+def test_verify_a_row_with_plus_infinity_has_no_token(paged, mode):
+    def change(x):
+        x = x.clone()
+        x[:, [17, 4000]] = INF
+        return x
+    c = low_case("f32", mode == "drafts", mode == "greedy", 1.0, change, seed=64, which=("target",))
+    d = {n: None if c[n] is None else c[n].cuda() for n in ("target", "draft", "tokens", "uniform", "race")}
+    out, acc = torch.zeros((5, 5), dtype=torch.int32, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    paged.verify_draft(d["target"], d["tokens"], torch.tensor(c["starts"], dtype=torch.int32).cuda(), out_tokens=out, accepted=acc,
+                       draft_logits=d["draft"], uniform=d["uniform"], race=d["race"], greedy=c["greedy"])
+    assert bool((out == -1).all()) and not acc.any()

@@ -71,67 +71,46 @@ __device__ __forceinline__ void vd_unpack(const uint4& v, float* x) {
 // reference R = m c as it rounds (the same R wherever m is the same, so its
 // rounding cancels in every quotient and one FMA gives each exponent), and the
 // lowest index of the maximum.  Of nothing, or of -inf alone: (-inf, 0, -1).  A
-// NaN is no maximum and makes the sum one, as a maximum of +inf does.
+// NaN is no maximum and makes the sum one.
+//
+// R is kept within 2^24, so that it is finite and its rounding at most half a bit.
+// Parts whose maximum is lower (finite masks) so have sums next to zero or zero, as
+// they should beside any other; a whole row beyond that (logits near the ends of f32
+// or bf16, or next to no temperature) is "far": its sum is made again from x - m.
 struct Stat {
   float m, s;
   int i;
 };
-__device__ __forceinline__ float vd_ref(float m, float c) { return m == -INFINITY ? 0.f : __fmul_rn(m, c); }
-// What the rounding of R leaves, 2^(m c - R), is a factor of the whole sum.  Past 2^24
-// (logits near the ends of f32 or bf16, or next to no temperature) it could be anything,
-// and R infinite: there sums go by m itself, at the price of more instructions.
-__device__ __forceinline__ bool vd_far(float ref) { return !(fabsf(ref) <= 16777216.f); }
-// base-2 logarithm of the weight of x in a sum with maximum m (NaN for x = m = +inf)
-__device__ __forceinline__ float vd_power(float x, float c, float m, float ref) {
-  return vd_far(ref) ? (x - m) * c : fmaf(x, c, -ref);
+constexpr float kFar = 16777216.f;
+__device__ __forceinline__ float vd_ref(float m, float c) { return fminf(fmaxf(__fmul_rn(m, c), -kFar), kFar); }
+__device__ __forceinline__ bool vd_far(float m, float c) { return fabsf(m * c) > kFar && m > -INFINITY; }
+// base-2 logarithm of the weight of x in a row with maximum m (NaN for x = m = +inf)
+__device__ __forceinline__ float vd_power(float x, float m, float c) {
+  return vd_far(m, c) ? (x - m) * c : fmaf(x, c, -vd_ref(m, c));
 }
-// What brings a sum from its maximum m, of reference `ref`, to a larger one's M, R: at
-// most 1.  A part without a finite logit (sum 0, reference 0) must not be scaled by
-// 2^(0 - R), infinite where all logits are low: 0 * inf would make the joined sum NaN.
-__device__ __forceinline__ float vd_scale(float m, float ref, float M, float R, float c) {
-  if (vd_far(ref) || vd_far(R))
-    return m == -INFINITY ? 0.f : vd_ex2((m - M) * c + vd_power(M, c, M, R) - vd_power(m, c, m, ref));
-  return vd_ex2(fminf(ref - R, 0.f));
-}
-__device__ __forceinline__ void vd_join(Stat& a, const Stat& b, float c) {
-  const float M = fmaxf(a.m, b.m), R = vd_ref(M, c);
-  if (b.i >= 0 && (a.i < 0 || b.m > a.m || (b.m == a.m && b.i < a.i))) a.i = b.i;
-  a.s = a.s * vd_scale(a.m, vd_ref(a.m, c), M, R, c) + b.s * vd_scale(b.m, vd_ref(b.m, c), M, R, c);
-  a.m = M;
+// one logit more
+__device__ __forceinline__ void vd_take(Stat& a, float f, int v, float c) {
+  const float s = vd_ex2(fmaf(f, c, -vd_ref(f, c)));
+  if (f > a.m) {
+    a.s *= vd_ex2(vd_ref(a.m, c) - vd_ref(f, c));
+    a.m = f;
+    a.i = v;
+    a.s += s;
+  } else {
+    a.s += s * vd_ex2(f == f ? vd_ref(f, c) - vd_ref(a.m, c) : 0.f);
+    if (f == a.m && f > -INFINITY) a.i = min(a.i, v);
+  }
 }
 // The lanes' parts: their maximum, the sums brought to it and added, the lowest index.
 __device__ __forceinline__ void vd_join_warp(Stat& a, float c) {
   float M = a.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  a.s *= vd_scale(a.m, vd_ref(a.m, c), M, vd_ref(M, c), c);
+  a.s *= vd_ex2(vd_ref(a.m, c) - vd_ref(M, c));  // at most 1
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
   a.i = (int)__reduce_min_sync(0xffffffffu, a.m == M ? (unsigned)a.i : 0xffffffffu);  // none: -1, the largest
   a.m = M;
-}
-
-// one logit more
-__device__ __forceinline__ void vd_take(Stat& a, float f, int64_t v, float c) {
-  Stat one{f, f == -INFINITY ? 0.f : vd_ex2(vd_power(f, c, f, vd_ref(f, c))), f > -INFINITY ? (int)v : -1};
-  if (!(f == f)) one.m = -INFINITY;
-  vd_join(a, one, c);
-}
-// A thread's part of a slice whose references reach far, once more and one by one: the
-// element in front (if it is this thread's) and whole vectors.
-template <typename T>
-__device__ __noinline__ Stat vd_far_slice(const T* x, const T* front, const uint4* xv, int64_t at, int64_t hi, int64_t head,
-                                          float c) {
-  constexpr int V = 16 / sizeof(T);
-  Stat a{-INFINITY, 0.f, -1};
-  if (front) vd_take(a, vd_f(*front), front - x, c);
-  for (; at < hi; at += VD_THREADS) {
-    float f[V];
-    vd_unpack<T>(xv[at], f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) vd_take(a, f[i], head + at * V + i, c);
-  }
-  return a;
 }
 
 // the largest of a 16-byte vector's values (NaN aside)
@@ -198,9 +177,8 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
   vd_rows(P, b, first, count, all);
   if (row - first >= count - which) return;  // not looked at; the draft of a sequence's last row is none
   Stat a{-INFINITY, 0.f, -1};
-  auto take = [&](float f, int64_t v) { vd_take(a, f, v, c); };
-  if (split == 0 && tid < head) take(vd_f(x[tid]), tid);
-  float ref = vd_ref(a.m, c), reach = fabsf(ref);
+  if (split == 0 && tid < head) vd_take(a, vd_f(x[tid]), tid, c);
+  float ref = vd_ref(a.m, c);
   for (int64_t at = lo + tid; at < hi; at += U * VD_THREADS) {
     uint4 raw[U];
 #pragma unroll
@@ -218,11 +196,10 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
           for (int i = V - 1; i >= 0; --i)
             if (f[i] == top) a.i = (int)(head + (at + u * VD_THREADS) * V + i);
         }
-        const float R = __fmul_rn(top, c);
-        a.s *= vd_ex2(fminf(ref - R, 0.f));
+        const float R = vd_ref(top, c);
+        a.s *= vd_ex2(ref - R);
         a.m = top;
         ref = R;
-        reach = fmaxf(reach, fabsf(R));
       }
       float sum = 0.f;
 #pragma unroll
@@ -230,9 +207,8 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
       a.s += sum;
     }
   }
-  if (vd_far(reach)) a = vd_far_slice<T>(x, split == 0 && tid < head ? x + tid : nullptr, xv, lo + tid, hi, head, c);
   const int64_t rest = head + vecs * V + tid;
-  if (split == P.splits - 1 && rest < P.vocab) take(vd_f(x[rest]), rest);
+  if (split == P.splits - 1 && rest < P.vocab) vd_take(a, vd_f(x[rest]), (int)rest, c);
   __shared__ Stat s_warp[VD_THREADS / 32];
   vd_join_warp(a, c);
   if ((tid & 31) == 0) s_warp[tid >> 5] = a;
@@ -268,6 +244,22 @@ __device__ __forceinline__ void vd_best_warp(Best& a) {
   }
 }
 
+// The sum of a far row's weights, by all threads of a CTA; the same in each.
+template <typename T>
+__device__ __noinline__ float vd_far_sum(const T* x, int64_t vocab, float m, float c, float* s_far) {
+  float sum = 0.f;
+#pragma unroll 8
+  for (int64_t v = threadIdx.x; v < vocab; v += VD_PICK_THREADS) sum += vd_ex2((vd_f(x[v]) - m) * c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();  // what a call before left there is read
+  if ((threadIdx.x & 31) == 0) s_far[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.f;
+  for (int w = 0; w < VD_PICK_THREADS / 32; ++w) sum += s_far[w];
+  return sum;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const __grid_constant__ VerifyParams P) {
   constexpr int THREADS = VD_PICK_THREADS, WARPS = THREADS / 32;
@@ -275,6 +267,7 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   __shared__ float s_max[2][VD_MAX_ROWS], s_sum[2][VD_MAX_ROWS];
   __shared__ int s_arg[VD_MAX_ROWS], s_taken;
   __shared__ Best s_best[WARPS], s_mine[2];
+  __shared__ float s_far[WARPS];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -302,6 +295,7 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
   }
   pdl_enter();
   // the rows' slices, joined
+  bool far = false;
   for (int i = warp; i < 2 * count; i += WARPS) {
     const int which = i >= count, r = which ? i - count : i;
     if (which && (!P.draft || r == count - 1)) continue;
@@ -313,24 +307,29 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
       if (P.greedy) a.i = vd_index(P, first + r)[lane];
     }
     vd_join_warp(a, which ? cd : c);
+    far = far || vd_far(a.m, which ? cd : c);
     if (lane == 0) {
       s_max[which][r] = a.m;
       s_sum[which][r] = a.s;
       if (!which) s_arg[r] = a.m - a.m == 0.f ? a.i : -1;
     }
   }
-  __syncthreads();
-  auto logp = [&](float l, int r) {
-    return (vd_power(l, c, s_max[0][r], vd_ref(s_max[0][r], c)) - log2f(s_sum[0][r])) * 0.6931471805599453f;
-  };
+  far = __syncthreads_or(far);
+  for (int i = 0; far && i < 2 * count; ++i) {
+    const int which = i >= count, r = which ? i - count : i;
+    if (which && (!P.draft || r == count - 1)) break;
+    const float m = s_max[which][r], k = which ? cd : c;
+    if (vd_far(m, k)) s_sum[which][r] = vd_far_sum<T>(which ? draft(r) : target(r), P.vocab, m, k, s_far);
+  }
+  auto logp = [&](float l, int r) { return (vd_power(l, s_max[0][r], c) - log2f(s_sum[0][r])) * 0.6931471805599453f; };
   if (tid < count - 1) {
     bool good = valid;
     if (good && P.greedy) good = x == s_arg[tid];
     if (good && !P.greedy) {
       // in logarithms: both sides may lie far below the smallest float
       float lq = 0.f;
-      if (P.draft) lq = vd_power(dx, cd, s_max[1][tid], vd_ref(s_max[1][tid], cd)) - log2f(s_sum[1][tid]);
-      good = log2f(ux) + lq < vd_power(lx, c, s_max[0][tid], vd_ref(s_max[0][tid], c)) - log2f(s_sum[0][tid]);
+      if (P.draft) lq = vd_power(dx, s_max[1][tid], cd) - log2f(s_sum[1][tid]);
+      good = log2f(ux) + lq < vd_power(lx, s_max[0][tid], c) - log2f(s_sum[0][tid]);
     }
     if (!good) atomicMin(&s_taken, tid);
   }
@@ -362,10 +361,10 @@ __global__ void __launch_bounds__(VD_PICK_THREADS, 2) verify_pick_kernel(const _
         enter(w, lv, ev, v);
       };
       const int64_t end = min(hi * V, P.vocab);
-      if (vd_far(ref) || vd_far(refd)) {
+      if (vd_far(s_max[0][taken], c) || (residual && vd_far(s_max[1][taken], cd))) {
         for (int64_t v = lo * V + tid; v < end; v += THREADS) {
-          float w = vd_ex2(vd_power(vd_f(l[v]), c, s_max[0][taken], ref)) * inv;
-          if (residual) w -= vd_ex2(vd_power(vd_f(d[v]), cd, s_max[1][taken], refd)) * invd;
+          float w = vd_ex2(vd_power(vd_f(l[v]), s_max[0][taken], c)) * inv;
+          if (residual) w -= vd_ex2(vd_power(vd_f(d[v]), s_max[1][taken], cd)) * invd;
           enter(w, vd_f(l[v]), e[v], v);
         }
       } else if (aligned) {

@@ -163,19 +163,21 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const __grid_co
   const int64_t vecs = (P.vocab - head) / V;
   const int64_t lo = vecs * split / P.splits, hi = vecs * (split + 1) / P.splits;
   const uint4* const xv = (const uint4*)(x + head);
-  // U vectors ahead of the ones in work, the first while the row's sequence is looked up
+  // U vectors ahead of the ones in work, the target's first while the row's sequence is
+  // looked up.  A sequence's last row of the draft need not be there: not before.
   uint4 ahead[U];
   auto fetch = [&](int64_t at) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (at + u * VD_THREADS < hi) ahead[u] = xv[at + u * VD_THREADS];
   };
-  fetch(lo + tid);
+  if (!which) fetch(lo + tid);
   const int b = seq_of_row(P.starts, P.num_seqs, P.each, row);
   if (b < 0) return;
   int first, count, all;
   vd_rows(P, b, first, count, all);
   if (row - first >= count - which) return;  // not looked at; the draft of a sequence's last row is none
+  if (which) fetch(lo + tid);
   Stat a{-INFINITY, 0.f, -1};
   if (split == 0 && tid < head) vd_take(a, vd_f(x[tid]), tid, c);
   float ref = vd_ref(a.m, c);

@@ -192,3 +192,26 @@ def test_verify_a_row_with_plus_infinity_has_no_token(paged, mode):
     paged.verify_draft(d["target"], d["tokens"], torch.tensor(c["starts"], dtype=torch.int32).cuda(), out_tokens=out, accepted=acc,
                        draft_logits=d["draft"], uniform=d["uniform"], race=d["race"], greedy=c["greedy"])
     assert bool((out == -1).all()) and not acc.any()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("with_starts", [False, True])
+def test_verify_draft_without_the_last_row(paged, dtype, with_starts):
+    """A draft model gives one distribution fewer than there are rows: through the C entry, where the draft's
+    last row may be missing.  Here it is memory of this test's own that holds NaN."""
+    import ctypes
+    vocab, rows = 6007, 4
+    c = verify_case(vocab, [rows], dtype, True, False, seed=65)
+    d = {n: c[n].cuda() for n in ("target", "tokens", "uniform", "race")}
+    draft = torch.cat([c["draft"][:rows - 1], torch.full((1, vocab), math.nan, dtype=TYPES[dtype])]).cuda()
+    out, acc = torch.zeros((1, rows), dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    a = paged._VerifyArgs(ctypes.sizeof(paged._VerifyArgs), d["target"].data_ptr(), draft.data_ptr(), d["tokens"].data_ptr(),
+                          starts.data_ptr() if with_starts else None, d["uniform"].data_ptr(), d["race"].data_ptr(), rows, 1, vocab,
+                          rows, vocab, vocab, vocab, 1.0, 1.0, paged._TYPES[TYPES[dtype]], 0, out.data_ptr(), acc.data_ptr(), None,
+                          None, None, work.data_ptr(), work.numel())
+    err = ctypes.create_string_buffer(512)
+    assert paged._library().verify(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream, err, 512) == 0, err.value
+    want, taken, _ = decided(c, 1.0, rows, acc.cpu())
+    assert torch.equal(out.cpu(), want) and torch.equal(acc.cpu(), taken)

@@ -1,0 +1,20 @@
+"""What the paged-cache entries promise at their edges, as far as the host shows it."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_verification_reads_no_row_of_the_draft_before_it_is_known_to_be_needed():
+    """The interface lets a sequence's last row of `draft` be missing, so the kernel may load from a row of it
+    only behind the look-up that says the row is looked at.  Loads out of a buffer cannot be shown on a GPU
+    without faulting it, so the order is checked in the source: of the calls that load a row's vectors, the ones
+    in front of the look-up are the target's alone."""
+    with open(os.path.join(ROOT, "clj-xla_b200", "csrc", "k_verify.cu")) as f:
+        text = f.read()
+    kernel = text[text.index("verify_rows_kernel(const"):text.index("// The race's best so far")]
+    known = kernel.index("if (row - first >= count - which) return;")
+    early = [m.group(0) for m in re.finditer(r"[^\n]*\bfetch\(lo \+ tid\)[^\n]*", kernel[:known])]
+    assert [s.strip() for s in early] == ["if (!which) fetch(lo + tid);"]
+    assert "*x" not in kernel[:known] and "x[" not in kernel[:known].replace("xv[at + u * VD_THREADS]", "")
+    assert kernel.index("if (which) fetch(lo + tid);") > known

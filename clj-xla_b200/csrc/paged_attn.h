@@ -374,6 +374,11 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
   constexpr bool Q_REGS = L::ES == 2 && (NR == 1 || (NR == 2 && L::CTAS == 1));
   uint32_t qf[Q_REGS ? QK : 1][Q_REGS ? NR : 1][4];  // the queries, where they fit registers
   const bool third = L::PARTS == 3 && P.out_f32;    // a third part of the weights
+  // f16 has no exponents to spare: its weights are taken relative to the tile's own
+  // maximum, 2^15 times as large (`beta` brings the tile's sums to the running maximum,
+  // the 2^15 cancels in the quotient).  Relative to the running one, a dominant position
+  // (2^25 times the others) would leave the others' weights no bits.
+  constexpr bool HALF = std::is_same<T, __half>::value;
   // this thread's positions and columns: g, g + 8; its rows: 2 t4, 2 t4 + 1
   const int g = lane >> 2, t4 = lane & 3;
   for (int tile = 0;; ++tile) {
@@ -516,28 +521,36 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
     }
     bar_sync<AT_CONSUMERS>(INNER);  // maxima are there, and K is read: its rows may take the weights
 
-    float alpha[NR][2];
+    float alpha[NR][2], beta[HALF ? NR : 1][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      float2 x = make_float2(m[n][0], m[n][1]);
+      float2 top = make_float2(-INFINITY, -INFINITY);  // the tile's
 #pragma unroll
       for (int w = 0; w < SCORERS; ++w) {
         const float2 y = *(const float2*)(wmax + w * ROWS + n * 8 + 2 * t4);
-        x.x = fmaxf(x.x, y.x);
-        x.y = fmaxf(x.y, y.y);
+        top.x = fmaxf(top.x, y.x);
+        top.y = fmaxf(top.y, y.y);
       }
-      const float b0 = x.x == -INFINITY ? 0.f : x.x, b1 = x.y == -INFINITY ? 0.f : x.y;
+      const float2 x = make_float2(fmaxf(m[n][0], top.x), fmaxf(m[n][1], top.y));
+      float b0 = x.x == -INFINITY ? 0.f : x.x, b1 = x.y == -INFINITY ? 0.f : x.y;
       alpha[n][0] = ex2(m[n][0] - b0);
       alpha[n][1] = ex2(m[n][1] - b1);
       m[n][0] = x.x;
       m[n][1] = x.y;
+      if constexpr (HALF) {
+        beta[n][0] = ex2(top.x - b0);
+        beta[n][1] = ex2(top.y - b1);
+        b0 = top.x == -INFINITY ? 0.f : top.x - 15.f;
+        b1 = top.y == -INFINITY ? 0.f : top.y - 15.f;
+      }
       if (SCORERS == 4 || warp < SCORERS) {
         const float p0 = ex2(s[n][0] - b0), p1 = ex2(s[n][1] - b1), p2 = ex2(s[n][2] - b0), p3 = ex2(s[n][3] - b1);
-        l[n][0] = l[n][0] * alpha[n][0] + (p0 + p2);
-        l[n][1] = l[n][1] * alpha[n][1] + (p1 + p3);
+        l[n][0] = fmaf(l[n][0], alpha[n][0], HALF ? beta[HALF ? n : 0][0] * (p0 + p2) : p0 + p2);
+        l[n][1] = fmaf(l[n][1], alpha[n][1], HALF ? beta[HALF ? n : 0][1] * (p1 + p3) : p1 + p3);
         if constexpr (L::ES == 2) {
-          // Parts of a weight, each what the ones before leave: two keep 22 bits in
-          // f16 and 16 in bf16, enough for its own outputs; an f32 one takes a third.
+          // Parts of a weight, each what the ones before leave.  f16: two keep 22 bits, or
+          // all above 2^-40 of the tile's largest.  bf16: two keep 16, enough for its own
+          // outputs; an f32 one takes a third.
           const uint32_t h0 = pack2<T>(p0, p1), h1 = pack2<T>(p2, p3);
           const float2 f0 = unpack2<T>(h0), f1 = unpack2<T>(h1);
           const float q0 = p0 - f0.x, q1 = p1 - f0.y, q2 = p2 - f1.x, q3 = p3 - f1.y;
@@ -610,6 +623,7 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
               } else {
                 p = *(const float*)(pw + row * PROW + (((j >> 2) ^ (row & 7)) * 16) + (j & 3) * 4);
               }
+              if constexpr (HALF) p *= beta[n][r];
 #pragma unroll
               for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -701,7 +715,9 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[i0 + i][n][e] = fmaf(acc[i0 + i][n][e], alpha[n][e & 1], t[i][n][e]);
+              for (int e = 0; e < 4; ++e)
+                acc[i0 + i][n][e] = fmaf(acc[i0 + i][n][e], alpha[n][e & 1],
+                                         HALF ? t[i][n][e] * beta[HALF ? n : 0][e & 1] : t[i][n][e]);
         }
       }
     }

@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import INF, TYPES, paged, verify_case  # noqa: F401 (a fixture)
+from test_gpu_paged import INF, TYPES, Case, half_step, paged, verify_case  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -215,3 +215,92 @@ def test_verify_draft_without_the_last_row(paged, dtype, with_starts):
     assert paged._library().verify(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream, err, 512) == 0, err.value
     want, taken, _ = decided(c, 1.0, rows, acc.cpu())
     assert torch.equal(out.cpu(), want) and torch.equal(acc.cpu(), taken)
+
+
+# ----------------------------------------------------------------- attention
+SINKS = {
+    # name: (length, position of the dominant key, head_dim, query heads per KV head, rows)
+    "one_tile": (50, 0, 64, 2, 1),
+    "middle": (5000, 2400, 128, 2, 1),
+    "long": (131071, 0, 64, 1, 1),
+    "long_last": (40000, 39990, 256, 2, 1),
+    "sixteen_rows": (3000, 1, 32, 4, 4),
+    "many_rows": (3000, 1500, 64, 8, 5),
+    "wide_many_rows": (2000, 700, 256, 16, 3),
+}
+
+
+@pytest.mark.parametrize("gap", [4.0, 11.0, 17.0, 17.4, 18.0, 22.0])
+@pytest.mark.parametrize("dtype,out", [("f16", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("name", list(SINKS))
+def test_attend_one_position_outweighs_the_others(paged, name, dtype, out, gap):
+    """An attention sink: one key whose score is far above all others, which are equal, and whose value is 0, so
+    that the result is what the others' small weights leave.
+
+    All scores are exact (one element of q and k each) but for their factor log2(e), 2^-23 of at most 32, so a
+    weight is off by 2^-18 relatively (exp2 in it); sums over tiles and ranges add at most 64 terms in a row,
+    2^-18.  bf16 weights for bf16 outputs have 16 bits, 2^-16; f16 ones have steps of 2^-39 of their tile's
+    largest, so in the dominant one's tile each of the 63 others is off by up to 2^-40 e^gap of itself.
+    Then the output's own half step; f16 outputs below 2^-14 have steps of 2^-24."""
+    length, at, hd, group, rows = SINKS[name]
+    c = Case([length], [rows], 2, group, hd, 64, dtype, seed=70)
+    c.k.zero_()
+    col = torch.arange(hd) % 16
+    c.v[:] = (1 + col / 16.0).to(c.dtype)
+    page, row = int(c.table[0, at // 64]), at % 64
+    c.k[page, :, row, 3] = 2.0
+    c.v[page, :, row] = 0.0
+    c.q.zero_()
+    c.q[:, :, 3] = gap / 2  # exact in bf16
+    c.q[:, :, 3] += (torch.arange(rows)[:, None] + torch.arange(2 * group)) % 2 * 0.5
+    real = 2.0 * c.q[:, :, 3].double()  # [rows, heads]
+    others = torch.tensor([length - rows + i for i in range(rows)], dtype=torch.float64)[:, None]
+    want = (others / (others + real.exp()))[..., None] * (1 + col / 16.0).double()
+    got = torch.empty((rows, 2 * group, hd), dtype=TYPES[out], device="cuda")
+    c.cache(paged).attend(c.q.cuda(), out=got, starts=c.dstarts, scale=1.0)
+    rel = 2.0 ** -18 + 2.0 ** -18 + (2.0 ** -16 if dtype == "bf16" and out == "bf16" else 0)
+    if dtype == "f16":
+        rel = rel + (63 / others.clamp(min=63)) * (2.0 ** -40 * real.exp())
+    tol = want * (rel[..., None] if torch.is_tensor(rel) else rel)
+    own = half_step(TYPES[out])
+    tol = tol + (want + tol) * own + (2.0 ** -25 if out == "f16" else 0)
+    off = (got.cpu().double() - want).abs()
+    assert bool((off <= tol).all()), float((off / want).max())
+
+
+@pytest.mark.parametrize("hd,group,rows", [(64, 1, 1), (128, 2, 5), (256, 4, 8)])
+def test_attend_f16_weights_after_a_dominant_tile(paged, hd, group, rows):
+    """Random scores, one key 20 above them whose value is 0, unseen positions that hold NaN (products made one by
+    one there).  Per weight: its score's sum, (head_dim + 8) 2^-24 of sum |q k|, and 2^-17 as in the test before;
+    the quotient has that twice; 64 weights of the dominant one's tile are off by 2^-40 of it."""
+    c = Case([3000, 700], [rows, rows], 2, group, hd, 16, "f16", seed=71)
+    scale = 0.125
+    c.k *= 0.25
+    c.q[:, :, 0], c.k[..., 0] = 1.0, 0.0
+    sinks = (1234, 0)
+    for b, at in enumerate(sinks):
+        p = int(c.table[b, at // 16])
+        c.k[p, :, at % 16] = 0.0
+        c.k[p, :, at % 16, 0] = 20.0 / scale
+        c.v[p, :, at % 16] = 0.0
+    want, tol = [], []
+    for b in (0, 1):
+        r, n = c.starts[b], c.lens[b] - rows + 1
+        j = torch.arange(n)
+        k, v = (x[c.table[b, j // 16].long(), :, j % 16].double() for x in (c.k, c.v))  # [n, nkv, hd]
+        q = c.q[r].double().view(2, group, hd)
+        w = torch.softmax(torch.einsum("hgd,nhd->hgn", q, k) * scale, -1)
+        size = torch.einsum("hgd,nhd->hgn", q.abs(), k.abs()) * scale
+        size[..., sinks[b]] = 0.0
+        want.append(torch.einsum("hgn,nhd->hgd", w, v).reshape(-1, hd))
+        one = (hd + 8) * 2.0 ** -24 * float(size.max()) + 2.0 ** -17
+        tol.append((2 * one * torch.einsum("hgn,nhd->hgd", w, v.abs()) + 64 * 2.0 ** -40 * float(v.abs().max())).reshape(-1, hd))
+        for at in range(n, c.lens[b]):  # the later rows' own positions
+            c.v[int(c.table[b, at // 16]), :, at % 16] = math.nan
+    got = torch.zeros(c.q.shape, device="cuda")
+    c.cache(paged).attend(c.q.cuda(), out=got, starts=c.dstarts, scale=scale)
+    for b in (0, 1):
+        r = c.starts[b]
+        off = (got[r].cpu().double() - want[b]).abs()
+        assert bool((off <= tol[b]).all()), float((off / tol[b]).max())
+        assert bool(got[r + 1:r + rows].isnan().all())

@@ -133,6 +133,8 @@ int64_t attention_workspace(const PagedAttnParams& p) {
 }
 
 bool nothing_to_do(const PagedView& c) { return c.tokens == 0 || c.num_seqs == 0; }
+// nor where no row of a sequence is computed
+bool nothing_to_do(const PagedAttnParams& p) { return nothing_to_do(p.c) || p.max_rows == 0; }
 
 PagedAttnParams attention_params(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAttentionArgs* a, bool pointers) {
   need(a != nullptr, "null arguments");
@@ -181,7 +183,7 @@ PagedAttnParams attention_params(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAtt
   need(vec16(a->tokens, p.q_tok) && vec16(a->q_heads, p.q_head), "q must have 16-byte aligned rows");
   need(vec16(a->tokens, p.o_tok) && vec16(a->q_heads, p.o_head), "out must have 16-byte aligned rows");
   need((a->tokens <= 1 || p.o_tok > 0) && (a->q_heads <= 1 || p.o_head > 0), "out must not be a broadcast");
-  if (pointers && !nothing_to_do(p.c)) {
+  if (pointers && !nothing_to_do(p)) {
     need(a->q && a->out, "null q or out");
     need(vec16(a->q), "q must have 16-byte aligned rows");
     need(vec16(a->out), "out must have 16-byte aligned rows");
@@ -316,7 +318,7 @@ extern "C" CLJXLA_EXPORT int cljxla_b200_paged_attention_workspace(const CLJXLA_
   return entry("paged_attention_workspace", err, errcap, [&] {
     need(bytes != nullptr, "null bytes");
     const PagedAttnParams p = attention_params(kv, a, false);
-    *bytes = nothing_to_do(p.c) ? 0 : attention_workspace(p);
+    *bytes = nothing_to_do(p) ? 0 : attention_workspace(p);
   });
 }
 
@@ -324,7 +326,7 @@ extern "C" CLJXLA_EXPORT int cljxla_b200_paged_attention(const CLJXLA_PagedKV* k
                                                          void* stream, char* err, size_t errcap) {
   return entry("paged_attention", err, errcap, [&] {
     PagedAttnParams p = attention_params(kv, a, true);
-    if (nothing_to_do(p.c)) return;
+    if (nothing_to_do(p)) return;
     const int64_t want = attention_workspace(p);
     if (want > 0 && (!a->workspace || a->workspace_bytes < want))
       fail(E_INVALID, "workspace of " + std::to_string(a->workspace ? a->workspace_bytes : 0) + " bytes, " +

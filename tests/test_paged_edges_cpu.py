@@ -1,6 +1,13 @@
 """What the paged-cache entries promise at their edges, as far as the host shows it."""
+import ctypes
 import os
 import re
+
+import pytest
+
+pytest.importorskip("torch")
+
+from test_paged_cpu import append_args, attention_args, cache, call, paged, verify_args  # noqa: E402,F401 (a fixture)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -18,3 +25,13 @@ def test_verification_reads_no_row_of_the_draft_before_it_is_known_to_be_needed(
     assert [s.strip() for s in early] == ["if (!which) fetch(lo + tid);"]
     assert "*x" not in kernel[:known] and "x[" not in kernel[:known].replace("xv[at + u * VD_THREADS]", "")
     assert kernel.index("if (which) fetch(lo + tid);") > known
+
+
+def test_attention_of_no_rows_of_a_sequence_does_nothing(paged):
+    """max_tokens 0 with starts: no row is computed, nothing is enqueued (a table of more than one tile, too)."""
+    lib, n = paged._library(), ctypes.c_int64(-1)
+    for c in (cache(paged), cache(paged, pages_per_seq=400, page_table_stride=400)):
+        a = attention_args(paged, starts=0xa0000, max_tokens=0)
+        assert call(lib.attend, c, a) == (0, "")
+        err = ctypes.create_string_buffer(512)
+        assert lib.attend_size(ctypes.addressof(c), ctypes.addressof(a), ctypes.byref(n), err, 512) == 0 and n.value == 0

@@ -60,6 +60,13 @@ constexpr int64_t kMaxStride = (int64_t)1 << 40;
 void need_stride(int64_t stride, const char* msg) { need(stride >= 0 && stride <= kMaxStride, msg); }
 
 bool vec16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+template <class... P>
+bool aligned(int64_t bytes, const P*... p) {  // 2 or 4; a null pointer is
+  return (((uintptr_t)p | ...) & (uintptr_t)(bytes - 1)) == 0;
+}
+void need_words(const PagedView& c) {
+  need(aligned(4, c.table, c.lens, c.starts), "page_table, seq_lens and starts must be aligned to their type");
+}
 // strides of dimensions with one entry are never used
 bool vec16(int64_t extent, int64_t stride_bytes) { return extent <= 1 || stride_bytes % 16 == 0; }
 
@@ -184,6 +191,7 @@ PagedAttnParams attention_params(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAtt
   need(vec16(a->tokens, p.o_tok) && vec16(a->q_heads, p.o_head), "out must have 16-byte aligned rows");
   need((a->tokens <= 1 || p.o_tok > 0) && (a->q_heads <= 1 || p.o_head > 0), "out must not be a broadcast");
   if (pointers && !nothing_to_do(p)) {
+    need_words(p.c);
     need(a->q && a->out, "null q or out");
     need(vec16(a->q), "q must have 16-byte aligned rows");
     need(vec16(a->out), "out must have 16-byte aligned rows");
@@ -284,6 +292,9 @@ extern "C" CLJXLA_EXPORT int cljxla_b200_paged_append(const CLJXLA_PagedKV* kv, 
     }
     if (nothing_to_do(p.c)) return;
     need(a->k && a->v, "null k or v");
+    need_words(p.c);
+    need(aligned(4, a->inv_freq), "inv_freq must be aligned to its type");
+    need(aligned(es, a->k, a->v, a->q, (const void*)a->q_out), "k, v, q and q_out must be aligned to their type");
     p.ks = (const char*)a->k;
     p.vs = (const char*)a->v;
     p.qs = (const char*)a->q;
@@ -360,7 +371,11 @@ extern "C" CLJXLA_EXPORT int cljxla_b200_verify_draft(const CLJXLA_VerifyDraftAr
     need(p.tokens == 0 || (a->target && a->tokens_in), "null target or tokens_in");
     need(p.tokens == 0 || a->greedy || (a->uniform && a->race), "null uniform or race");
     const int64_t es = element_size(p.dt);
-    need((uintptr_t)a->target % es == 0 && (uintptr_t)a->draft % es == 0, "logits must be aligned to their type");
+    need(aligned(es, a->target, p.draft), "logits must be aligned to their type");
+    need(aligned(4, a->tokens_in, a->starts, p.greedy ? nullptr : a->uniform, p.greedy ? nullptr : a->race),
+         "tokens_in, starts, uniform and race must be aligned to their type");
+    need(aligned(4, a->tokens_out, a->accepted, a->logprobs, a->new_lens, a->new_lens ? a->seq_lens : nullptr),
+         "tokens_out, accepted, logprobs, seq_lens and new_lens must be aligned to their type");
     p.splits = verify_splits(p.tokens, p.vocab, p.draft != nullptr);
     const int64_t want = verify_workspace(p);
     if (want > 0 && (!a->workspace || a->workspace_bytes < want))

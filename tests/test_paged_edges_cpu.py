@@ -35,3 +35,36 @@ def test_attention_of_no_rows_of_a_sequence_does_nothing(paged):
         assert call(lib.attend, c, a) == (0, "")
         err = ctypes.create_string_buffer(512)
         assert lib.attend_size(ctypes.addressof(c), ctypes.addressof(a), ctypes.byref(n), err, 512) == 0 and n.value == 0
+
+
+@pytest.mark.parametrize("where", ["k", "v", "q", "q_out", "inv_freq", "starts", "seq_lens", "page_table"])
+@pytest.mark.parametrize("dtype,step", [("bf16", 1), ("f16", 1), ("f32", 1), ("f32", 2)])
+def test_append_refuses_misaligned_pointers(paged, where, dtype, step):
+    """An address between elements would be a misaligned access on the device."""
+    c, a = cache(paged, dtype=paged.DTYPE_ENUM[dtype]), append_args(paged)
+    s = c if hasattr(c, where) else a
+    setattr(s, where, (getattr(s, where) or 0xb0000) + step)
+    rc, err = call(paged._library().append, c, a)
+    assert rc == 3 and where in err and "aligned" in err, (rc, err)
+
+
+@pytest.mark.parametrize("where", ["starts", "seq_lens", "page_table"])
+def test_attention_refuses_misaligned_pointers(paged, where):
+    c, a = cache(paged), attention_args(paged)
+    s = c if hasattr(c, where) else a
+    setattr(s, where, (getattr(s, where) or 0xb0000) + 2)
+    rc, err = call(paged._library().attend, c, a)
+    assert rc == 3 and where in err and "aligned" in err, (rc, err)
+
+
+@pytest.mark.parametrize("where", ["tokens_in", "starts", "uniform", "race", "tokens_out", "accepted", "logprobs", "seq_lens", "new_lens"])
+def test_verify_refuses_misaligned_pointers(paged, where):
+    a = verify_args(paged)
+    setattr(a, where, (getattr(a, where) or 0xb0000) + 2)
+    rc, err = call(paged._library().verify, a)
+    assert rc == 3 and where in err and "aligned" in err, (rc, err)
+
+
+def test_verify_refuses_misaligned_logits_of_the_draft(paged):
+    rc, err = call(paged._library().verify, verify_args(paged, draft=0x20001))
+    assert rc == 3 and "aligned" in err, (rc, err)

@@ -23,7 +23,9 @@ rows behind the last sequence are left alone.
 
 Calls enqueue on torch's current stream of the tensors' device and never
 synchronise.  Tensors of another shape, type, device or layout raise
-``ValueError``; what the library refuses raises :class:`~.pjrt.PJRTError`.
+``ValueError``, as do tensors that require gradients outside ``torch.no_grad()``
+(these operators serve, they have no backward pass); what the library refuses
+raises :class:`~.pjrt.PJRTError`.
 """
 from __future__ import annotations
 
@@ -164,11 +166,17 @@ def _expected(name: str, shape, dtype, device: int, t: torch.Tensor, what: str =
                      f"{t.device} with strides {t.stride()}")
 
 
+def _tracked(name: str):
+    raise ValueError(f"{name}: no gradient flows through the paged-cache operators; detach it, or call under torch.no_grad()")
+
+
 def _rows(t: torch.Tensor, name: str, shape, dtype, device: int):
     """Strides of a [rows, heads, head_dim] tensor whose last axis is contiguous."""
     s = t.stride()
     if t.dtype is not dtype or t.shape != shape or t.get_device() != device or s[2] != 1:
         _expected(name, shape, dtype, device, t, " with head_dim contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        _tracked(name)
     return s
 
 
@@ -181,6 +189,8 @@ def _vector(t: torch.Tensor, name: str, n: int, dtype, device: int) -> int:
 def _matrix(t: torch.Tensor, name: str, rows: int, cols: int, dtype, device: int) -> int:
     if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != device or (cols > 1 and t.stride(1) != 1):
         _expected(name, (rows, cols), dtype, device, t, " with contiguous rows")
+    if t.requires_grad and torch.is_grad_enabled():
+        _tracked(name)
     return t.data_ptr()
 
 
@@ -225,6 +235,8 @@ class Rope:
         if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
                 or not inv_freq.is_cuda:
             raise ValueError("Rope: inv_freq must be a contiguous f32 vector on a CUDA device")
+        if inv_freq.requires_grad:
+            _tracked("inv_freq")
         self.inv_freq, self.interleaved, self.scale = inv_freq, bool(interleaved), float(scale)
         self.device = inv_freq.get_device()
         self._args = (inv_freq.data_ptr(), 2 * inv_freq.shape[0], self.interleaved, self.scale)
@@ -244,6 +256,8 @@ class PagedKV:
         dev = k_pages.get_device()
         if v_pages.shape != k_pages.shape or v_pages.dtype is not k_pages.dtype or v_pages.get_device() != dev:
             raise ValueError("v_pages: the shape, type and device of k_pages expected")
+        if k_pages.requires_grad or v_pages.requires_grad:
+            _tracked("pages")
         if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
             raise ValueError("pages: head_dim must be contiguous")
         if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != dev \
@@ -383,6 +397,8 @@ def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, starts: Opti
         if uniform is None or race is None:
             raise ValueError("uniform and race are needed unless greedy")
         up = _vector(uniform, "uniform", rows, f32, dev)
+        if uniform.requires_grad and torch.is_grad_enabled():
+            _tracked("uniform")
         rp, rs = _matrix(race, "race", seqs, vocab, f32, dev), race.stride(0)
         if draft_logits is not None:
             dp, ds = _matrix(draft_logits, "draft_logits", rows, vocab, dt, dev), draft_logits.stride(0)

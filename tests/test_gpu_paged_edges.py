@@ -304,3 +304,35 @@ def test_attend_f16_weights_after_a_dominant_tile(paged, hd, group, rows):
         off = (got[r].cpu().double() - want[b]).abs()
         assert bool((off <= tol[b]).all()), float((off / tol[b]).max())
         assert bool(got[r + 1:r + rows].isnan().all())
+
+
+# ------------------------------------------------------------------ refusals
+def test_tensors_that_need_gradients_are_refused(paged):
+    """The operators have no backward pass: a gradient would be lost in silence."""
+    c = Case([20, 40], [2, 1], 2, 2, 64, 16, "bf16", seed=4)
+    cache = c.cache(paged)
+    q, k, v = c.q.cuda(), c.kn.cuda(), c.vn.cuda()
+    want = lambda t: t.detach().clone().requires_grad_()
+    for kw in (dict(q=want(q)), dict(q=q, out=want(q))):
+        with pytest.raises(ValueError, match="gradient"):
+            cache.attend(starts=c.dstarts, **kw)
+    for a in ((want(k), v, q), (k, want(v), q), (k, v, want(q)), (k, v, q, want(q))):
+        with pytest.raises(ValueError, match="gradient"):
+            cache.append(*a, starts=c.dstarts)
+    with pytest.raises(ValueError, match="gradient"):
+        paged.PagedKV(want(c.dk), c.dv, c.dtable, c.dlens)
+    with pytest.raises(ValueError, match="gradient"):
+        paged.PagedKV(c.dk, want(c.dv), c.dtable, c.dlens)
+    with pytest.raises(ValueError, match="gradient"):
+        paged.Rope(torch.ones(4, device="cuda", requires_grad=True))
+    z = lambda *s, **kw: torch.zeros(s, device="cuda", **kw)
+    out, acc = z(1, 2, dtype=torch.int32), z(1, dtype=torch.int32)
+    f = dict(target_logits=z(2, 9), draft_logits=z(2, 9), uniform=z(2), race=z(1, 9) + 1)
+    for n in f:
+        with pytest.raises(ValueError, match="gradient"):
+            paged.verify_draft(**{**f, n: want(f[n])}, tokens=z(2, dtype=torch.int32), out_tokens=out, accepted=acc)
+    # without gradients being recorded, the same tensors serve
+    with torch.no_grad():
+        assert torch.equal(cache.attend(want(q), starts=c.dstarts), cache.attend(q, starts=c.dstarts))
+        paged.verify_draft(**{n: want(f[n]) for n in f}, tokens=z(2, dtype=torch.int32), out_tokens=out, accepted=acc)
+    assert int(out[0, 0]) == 0

@@ -540,11 +540,15 @@ __device__ __forceinline__ void consume_mma(const PagedAttnParams& P, unsigned c
       if constexpr (HALF) {
         beta[n][0] = ex2(top.x - b0);
         beta[n][1] = ex2(top.y - b1);
-        b0 = top.x == -INFINITY ? 0.f : top.x - 15.f;
-        b1 = top.y == -INFINITY ? 0.f : top.y - 15.f;
+        b0 = top.x == -INFINITY ? 0.f : top.x;
+        b1 = top.y == -INFINITY ? 0.f : top.y;
       }
       if (SCORERS == 4 || warp < SCORERS) {
-        const float p0 = ex2(s[n][0] - b0), p1 = ex2(s[n][1] - b1), p2 = ex2(s[n][2] - b0), p3 = ex2(s[n][3] - b1);
+        auto weight = [](float x, float b) {
+          if constexpr (HALF) return ex2(x - b + 15.f);  // added last: scores of 2^30 have steps above 15
+          else return ex2(x - b);
+        };
+        const float p0 = weight(s[n][0], b0), p1 = weight(s[n][1], b1), p2 = weight(s[n][2], b0), p3 = weight(s[n][3], b1);
         l[n][0] = fmaf(l[n][0], alpha[n][0], HALF ? beta[HALF ? n : 0][0] * (p0 + p2) : p0 + p2);
         l[n][1] = fmaf(l[n][1], alpha[n][1], HALF ? beta[HALF ? n : 0][1] * (p1 + p3) : p1 + p3);
         if constexpr (L::ES == 2) {

@@ -306,6 +306,25 @@ def test_attend_f16_weights_after_a_dominant_tile(paged, hd, group, rows):
         assert bool(got[r + 1:r + rows].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("hd,group,rows", [(64, 1, 1), (128, 4, 2), (32, 8, 3)])
+def test_attend_huge_scores(paged, hd, group, rows, dtype):
+    """Scores whose steps are wider than any weight's exponent: the positions of the largest share the result."""
+    c = Case([300], [rows], 2, group, hd, 16, dtype, seed=72)
+    c.q.zero_()
+    c.k.zero_()
+    c.q[..., 0] = 60000.0
+    at = [3, 70, 250]
+    for sign in (1.0, -1.0):
+        for j in range(300):
+            c.k[int(c.table[0, j // 16]), :, j % 16, 0] = sign * (60000.0 if (j in at) == (sign > 0) else 30000.0)
+        want = torch.stack([c.v[int(c.table[0, j // 16]), :, j % 16].double() for j in at]).mean(0)  # [nkv, hd]
+        got = torch.empty((rows, 2 * group, hd), device="cuda")
+        c.cache(paged).attend(c.q.cuda(), out=got, starts=c.dstarts, scale=1.0)
+        off = (got.cpu().double().view(rows, 2, group, hd) - want[None, :, None]).abs()
+        assert bool((off <= 2.0 ** -15 * 4).all()), float(off.max())  # bf16 weights of 1, a third in f32: 2^-22 and less
+
+
 # ------------------------------------------------------------------ refusals
 def test_tensors_that_need_gradients_are_refused(paged):
     """The operators have no backward pass: a gradient would be lost in silence."""

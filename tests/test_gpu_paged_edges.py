@@ -181,6 +181,17 @@ def test_verify_logits_at_the_ends_of_the_range(paged, name, mode):
 
 
 @pytest.mark.parametrize("mode", ["drafts", "guesses", "greedy"])
+@pytest.mark.parametrize("name", ["shift_f32_-1000", "shift_bf16_-100", "shift_f16_-1000", "mask_bf16_half_-1e+09", "mask_f16_one_-65504",
+                                  "f32_lowest_half_0.8", "bf16_lowest_most_1.0", "bf16_all_lowest", "f32_border"])
+@pytest.mark.parametrize("vocab", [8192, 40000])
+def test_verify_low_logits_in_aligned_rows(paged, vocab, name, mode):
+    """Vocabularies of whole vectors, raced by one CTA's and by a whole cluster's vector loads."""
+    dtype, temp, change = {**LOW, **ENDS}[name]
+    c = low_case(dtype, mode == "drafts", mode == "greedy", temp, change, seed=66, vocab=vocab)
+    verify(paged, c, temp)
+
+
+@pytest.mark.parametrize("mode", ["drafts", "guesses", "greedy"])
 def test_verify_a_row_with_plus_infinity_has_no_token(paged, mode):
     def change(x):
         x = x.clone()

@@ -8,10 +8,12 @@
 //
 // What bounds it: every element is read and written once, so HBM bandwidth for
 // prompts and the chain starts -> length -> page -> store for a decode step.
-// Angles cost more than the copies they turn: a CTA takes TOK rows (8 of a long
+// Angles cost more than the copies they turn: a CTA takes TOK rows (4 of a long
 // prompt, 1 of a decode step, where rows are few and CTAs share a row's heads
 // instead), computes their cos and sin once in shared memory for all heads, and
-// each thread keeps its pairs of one row in registers over the heads it serves.
+// each thread has its pairs of all the CTA's rows in flight for one head after another.
+// Measured (B200): 4968 f16 rows of 16 + 16 heads of 256 31 to 33 us (24.8 at the copy
+// rate); one element off a 16-byte boundary 74, with a rotated part of 60 elements 102.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

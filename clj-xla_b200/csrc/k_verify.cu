@@ -15,9 +15,9 @@
 //   over its slice of the one deciding row, and the first CTA takes the best
 //   of the cluster through distributed shared memory.  A single sequence so still
 //   has eight SMs, and no CTA waits for another launch.
-// Measured (B200): 102 rows of 262144 bf16 logits with drafts 40 us, of which the
-// first kernel 22 (4.1 TB/s; its issue slots are 66 % busy) and the race 11; greedily
-// 161 rows of 256000 23 us; five rows of 50257 in f32 10 us.
+// Measured (B200): 102 rows of 262144 bf16 logits with drafts 39 us, of which the
+// first kernel 22 (4.1 TB/s; its issue slots are 64 % busy) and the race 11; greedily
+// 161 rows of 256000 22 us; five rows of 50257 in f32 10 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -457,8 +457,8 @@ void launch_t(const VerifyParams& p, cudaStream_t s) {
 
 }  // namespace
 
-// Slices of a row: up to eight CTAs per SM over all rows, none below two vectors
-// a thread.
+// Slices of a row: up to eight CTAs per SM over all rows, none below eight logits
+// (one 16-bit vector or two of f32) a thread.
 int verify_splits(int64_t tokens, int64_t vocab, bool draft) {
   const int64_t rows = std::max<int64_t>(tokens * (draft ? 2 : 1), 1);
   const int64_t want = std::max<int64_t>(8 * (int64_t)device_sm_count() / rows, 1);

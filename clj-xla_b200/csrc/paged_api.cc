@@ -53,7 +53,8 @@ int element_type(int32_t dtype) {
 int64_t element_size(int dt) { return dt == KDT_F32 ? 4 : 2; }
 
 // every extent that takes part in address arithmetic stays below this, and every
-// stride below 2^40, so that products of the two fit 64 bits with room to add
+// stride below 2^40 elements: no product of an index that memory can hold and its
+// stride comes near 64 bits
 constexpr int64_t kMaxCount = 1 << 30;
 constexpr int64_t kMaxStride = (int64_t)1 << 40;
 

@@ -33,7 +33,7 @@
 // warp holds partials.  Stages change hands over named barriers.
 //
 // Measured (B200, device time): 1.07 GB of bf16 pages in one sequence 160 us (6.7
-// TB/s, the copy rate), 32 sequences of 3 to 8447 positions at head_dim 256 28 us
+// TB/s, the copy rate), 32 sequences of 2 to 8447 positions at head_dim 256 28 us
 // (4.3 TB/s; 9 us of that are the first tile's three dependent reads and the join),
 // 256 sequences of 1 to 601 positions 49 us (4.3 TB/s).
 #pragma once

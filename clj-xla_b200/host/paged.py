@@ -319,7 +319,9 @@ class PagedKV:
         their sequences' pages, into ``out`` (same shape; the pages' type or
         f32).  A row sees the positions up to its own, with ``window`` >= 0 only
         that many before its own; a row that sees nothing is zero.  ``max_tokens``
-        bounds a sequence's rows (default: all rows), ``scale`` is ``head_dim **
+        bounds a sequence's rows; give it with ``starts``: the default, all rows,
+        takes tiles of up to 32 rows where a decode step needs one (64 sequences of
+        2048 positions: 419 us instead of 165).  ``scale`` is ``head_dim **
         -0.5`` by default, ``softcap`` > 0 caps the scores as ``softcap *
         tanh(score / softcap)``.  Returns ``out``."""
         dt, dev, dim = self.dtype, self.device, self.head_dim

@@ -167,10 +167,11 @@ CLJXLA_EXPORT int cljxla_b200_attention_decode_static(const void* q, const void*
  * Every pointer below is a device pointer unless it says otherwise.  starts,
  * seq_lens and page_table are read by the kernels when they run, so a captured
  * graph follows their contents.  What the host cannot see is bounded in the
- * kernels: seq_lens is clamped to [0, pages_per_seq * page_size], starts to
- * [0, tokens], and a page number outside [0, num_pages) is a page that is not
- * there: append leaves its rows out, attention leaves its positions out (so a
- * sliding-window layer may give pages back and mark them -1).
+ * kernels: seq_lens is clamped to [0, 2^30], starts to [0, tokens], and a page
+ * number outside [0, num_pages) is a page that is not there, as is every page
+ * past pages_per_seq (a longer length keeps its rows' positions): append leaves
+ * such rows out, attention leaves such positions out (so a sliding-window layer
+ * may give pages back and mark them -1).
  *
  * Work is enqueued on `stream` (a cudaStream_t; NULL = legacy default stream)
  * of the calling thread's current device, without synchronising and without
@@ -211,9 +212,9 @@ typedef struct CLJXLA_PagedAppendArgs {
  * (x1, x2) -> rope_scale * (x1 cos a - x2 sin a, x2 cos a + x1 sin a) with a =
  * position * inv_freq[i] (the angle reduced in 64 bits), computed in f32 and
  * rounded once.  Two rows of one call must not share a (page, row): which of
- * them stays is not defined.  Tensors of any element alignment; 16-byte
- * aligned ones with rotary_dim / 2 (interleaved: rotary_dim) a multiple of 16
- * bytes are the fast ones. */
+ * them stays is not defined.  K and V pages must be 16-byte aligned rows; k, v, q
+ * and q_out may begin at any element, but 16-byte aligned ones with rotary_dim / 2
+ * (interleaved: rotary_dim) a multiple of 16 bytes are two to three times as fast. */
 CLJXLA_EXPORT int cljxla_b200_paged_append(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAppendArgs* args, void* stream,
                                            char* err, size_t errcap);
 
@@ -224,7 +225,9 @@ typedef struct CLJXLA_PagedAttentionArgs {
   int64_t tokens, q_heads; /* q_heads a multiple of kv_heads */
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
   const int32_t* starts; /* [num_seqs + 1], ascending; NULL: tokens / num_seqs rows each */
-  int64_t max_tokens;    /* upper bound of a sequence's rows (rows past it are not computed) */
+  int64_t max_tokens;    /* upper bound of a sequence's rows (rows past it are not computed).  Row tiles are
+                            chosen for it, so give a tight one: 64 sequences of one row and 2048 positions take
+                            165 us with 1, 419 with 64 */
   int64_t window;        /* >= 0: a row sees its own position and `window` before it; < 0: all */
   float scale, softcap;  /* score = softcap * tanh(scale * q.k / softcap), or scale * q.k with softcap 0 */
   int32_t out_dtype;     /* the pages' type, or F32 */
@@ -236,9 +239,11 @@ typedef struct CLJXLA_PagedAttentionArgs {
 
 /* Row r at position p of its sequence: out = sum_j w_j v_j / sum_j w_j over the
  * positions j <= p (and j >= p - window) of the sequence's pages, w_j =
- * exp(score_j - max).  A row that sees no position is zero.  What a row does
- * not see (later drafts, evicted pages, page tails) may hold anything, NaN and
- * infinities included.  K and V pages must be 16-byte aligned rows. */
+ * exp(score_j - max).  A row that sees no position is zero, as is one whose scores
+ * are all -inf.  What a row does not see (later drafts, evicted pages, page tails)
+ * may hold anything, NaN and infinities included; an infinity in a value that it
+ * does see makes the result infinite or NaN.  K and V pages must be 16-byte aligned
+ * rows. */
 CLJXLA_EXPORT int cljxla_b200_paged_attention(const CLJXLA_PagedKV* kv, const CLJXLA_PagedAttentionArgs* args,
                                               void* stream, char* err, size_t errcap);
 
@@ -252,7 +257,8 @@ typedef struct CLJXLA_VerifyDraftArgs {
   size_t struct_size;
   const void* target; /* [tokens, vocab] logits: row r is the distribution of the token behind row r */
   const void* draft;  /* [tokens, vocab] logits row r + 1's token was drawn from; NULL: the guesses have no
-                         distribution (each counts as certain). A sequence's last row is not read */
+                         distribution (each counts as certain). A sequence's last row is not read: the
+                         buffer may end before it */
   const int32_t* tokens_in; /* [tokens] the tokens the rows were fed: rows past a sequence's first are drafts */
   const int32_t* starts;    /* [num_seqs + 1], ascending; NULL: tokens / num_seqs rows each */
   const float* uniform;     /* [tokens] in [0, 1): row r decides on row r + 1's token; NULL when greedy */
@@ -279,7 +285,10 @@ typedef struct CLJXLA_VerifyDraftArgs {
  * without x where draft is NULL; p where that leaves nothing), p behind the last
  * draft.  greedy: x is accepted while it is the argmax, and the argmax follows.
  * Ties go to the lowest index.  A draft outside [0, vocab) is rejected.  Logits
- * may be -inf (probability 0); a row without a finite maximum gives token -1. A
+ * may be -inf (probability 0) or any finite value.  p and q are held in f32: in w
+ * one below 2^-126 is 0, and a difference below 2^-22 of them is rounding (drafts
+ * drawn from q meet such a w less than once in 2^22).  A NaN is never an argmax, and
+ * leaves a sampled row without a token; a row without a finite maximum gives token -1. A
  * sequence without rows gives 0 accepted, -1 throughout and its length. */
 CLJXLA_EXPORT int cljxla_b200_verify_draft(const CLJXLA_VerifyDraftArgs* args, void* stream, char* err,
                                            size_t errcap);
